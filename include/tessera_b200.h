@@ -360,6 +360,89 @@ size_t ts_linear_q8_0_workspace_bytes(uint32_t m, uint32_t n, uint32_t k);
 int ts_linear_q8_0(const void *x, const void *w_q8_0, const void *a0, void *out, uint32_t m, uint32_t n, uint32_t k,
                    int epilogue, float scale, int out_dtype, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * Kept rows in 8 bits.  The reference keeps K and V rows in the activations' type
+ * (engine/plan/codegen/src/kept.rs:135-194); this form holds them as signed codes with one f32 scale per block of
+ * `block` positions and kv head, at half the bytes.  It has no counterpart in the reference.
+ *   k, v              int8 [blocks, kv_heads, block, width]; a kept value is code * scale
+ *   k_scale, v_scale  f32 [blocks, kv_heads]
+ *   k_bounds          int8 [blocks, kv_heads, 2, width]: the lowest, then the highest key code of each channel; only
+ *                     ts_select_blocks_q8 reads them; NULL when no block is ever selected
+ * `block` is 16, 32 or 64, `width` 64, 128 or 256.  The ts_kept that goes with it is dense with a stride that is a
+ * multiple of `block`, or paged with pages of at least `block` rows (table_len set); interleaved rows have no blocks
+ * and are refused.  Block b of a slot's positions [b * block, (b + 1) * block) is the pool's block
+ *   dense  slot * (kept_scalar / block) + b          paged  table[entry] * (page / block) + b % (page / block)
+ * so that pages copy with ts_kv_copy_pages as they do in bf16: codes with row_bytes = block * kv_heads * width, scales
+ * with 4 * kv_heads, bounds with 2 * kv_heads * width, the rows of a copy rounded up to whole blocks and page_rows in
+ * blocks.  A slot, a position or a table entry that leads outside the pool is skipped: nothing is written, keys there
+ * are not seen, and a read gives zeros.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    void *k_bounds;
+    uint32_t block;  /* positions a scale covers */
+    uint32_t blocks; /* blocks the buffers hold */
+} ts_rows_q8;
+
+/* ts_qk_norm_rope_append_bf16 into such rows: per-head norm (gains or NULL) and rotation of q and k (angle = position *
+ * inv_freq[j], reduced in 64 bits so that far positions keep their digits), q -> q_out bf16, k and v -> codes, rounded once
+ * from 32 bits.  For each block and kv head that rows of the call write, with a = max |x| over them,
+ *     s_new = max(s_old, a / 127, 2^-60),    code = round(x / s_new) within [-127, 127]
+ * where s_old is the block's scale, or 0 when a row of the call writes the block's first position (it starts the
+ * block afresh: what the block held before has no value until it is written again).  A scale never shrinks
+ * otherwise; where it grows, the codes that the call does not write become round(code * s_old / s_new).  The bounds
+ * follow: those of the new key codes alone in a fresh block, else joined with round(bound * s_old / s_new).
+ * NaN stores the code 0, an infinity the largest code, and counts as the largest finite bf16 in `a`, so that
+ * what is kept reads back finite.
+ * Rows of one call that fall into the same block must stand next to one another, in any order; of rows with the
+ * same slot and position the last one counts (a launch that repeats its last row to fill up is fine). */
+int ts_qk_norm_rope_append_q8(const void *qkv, const float *q_norm, const float *k_norm, const float *inv_freq,
+                              const uint32_t *slots, const uint32_t *positions, void *q_out, const ts_rows_q8 *kv,
+                              const ts_kept *kept, uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                              float eps, void *stream);
+
+/* k_out, v_out bf16 [rows, kv_heads, width] = the kept rows at (slots[r], positions[r]), rounded once: for a prompt
+ * whose first part is already kept (its whole-sequence attention, ts_attend_bf16, takes bf16 rows back to back). */
+int ts_rows_unpack_q8(const ts_rows_q8 *kv, const uint32_t *slots, const uint32_t *positions, void *k_out, void *v_out,
+                      const ts_kept *kept, uint32_t rows, uint32_t kv_heads, uint32_t width, void *stream);
+
+/* ts_attend_rows_bf16 over such rows: q, out bf16 [rows, heads, width], row r sees keys [max(0, pos - back),
+ * min(pos + 1, keys)) of its slot; a row that sees none gets zeros.  Neighbouring rows of one slot (drafted tokens, a
+ * part of a prompt) share what they read.  Scores and sums are f32, probabilities f16. */
+size_t ts_attend_rows_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                                         uint32_t back);
+
+int ts_attend_rows_q8(const void *q, const ts_rows_q8 *kv, void *out, const uint32_t *slots, const uint32_t *positions,
+                      const ts_kept *kept, uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                      uint32_t back, float scale, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Which blocks each row and kv head should read: ids u32 [rows, kv_heads, count], ascending, spare entries UINT32_MAX.
+ * With the group's query codes c = round(q * 127 / max |q|) (the largest over all the group's heads), up = sum over the
+ * heads of max(c, 0) and down = that of min(c, 0), a block scores
+ *     f32(sum_d up[d] * highest[d] + down[d] * lowest[d]) * k_scale
+ * (a whole number, so the choice does not depend on an order of summation): never less than what any key of the block
+ * gives the group's heads together, up to the rounding of q.  Of the blocks [0, n) that hold positions <= min(pos,
+ * keys - 1), the `first` first and the `recent` last are always taken, the rest by score, ties to the lower index;
+ * first + recent <= count <= 4096.  With n <= count every block is taken. */
+size_t ts_select_blocks_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t kv_heads, uint32_t block, uint32_t count);
+
+int ts_select_blocks_q8(const void *q, const ts_rows_q8 *kv, uint32_t *ids, const uint32_t *slots, const uint32_t *positions,
+                        const ts_kept *kept, uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                        uint32_t count, uint32_t first, uint32_t recent, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/* Causal attention over listed blocks only: ids u32 [rows, kv_heads, count] in any order (a block listed twice counts
+ * twice); entries without a position <= min(pos, keys - 1), UINT32_MAX among them, are skipped, and a row and kv head
+ * with nothing to see gets zeros. */
+size_t ts_attend_blocks_q8_workspace_bytes(uint32_t rows, uint32_t count, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                                           uint32_t block);
+
+int ts_attend_blocks_q8(const void *q, const ts_rows_q8 *kv, const uint32_t *ids, void *out, const uint32_t *slots,
+                        const uint32_t *positions, const ts_kept *kept, uint32_t rows, uint32_t keys, uint32_t heads,
+                        uint32_t kv_heads, uint32_t width, uint32_t count, float scale, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
 /* The B200 entry of the reference's platform table plus what the current device reports, as JSON text:
  *   {"row": <the table row: matches "cuda sm_100", tile = bf16_tile = [128, 256, 16] (tcgen05.mma, M x N x K with
  *            N up to 256), pdl, check ["sm_100a"], and under "b200" what the reference's `Needs` has no field for

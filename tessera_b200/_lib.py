@@ -31,6 +31,11 @@ class TsLinearFused(C.Structure):
     _fields_ = [("row_ss", vp), ("row_parts", u32), ("row_eps", f32), ("ss_out", vp), ("xs_out", vp), ("xs_gain", vp)]
 
 
+class TsRowsQ8(C.Structure):
+    """ts_rows_q8: kept rows as 8-bit codes, a scale per block of positions and kv head."""
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("k_bounds", vp), ("block", u32), ("blocks", u32)]
+
+
 class TsArg(C.Structure):
     class _V(C.Union):
         _fields_ = [("ptr", vp), ("u32", u32), ("f32", f32)]
@@ -75,6 +80,14 @@ SIGNATURES = {
     "ts_attend_bf16": (i32, [vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, u32, u32, f32, vp, sz, vp]),
     "ts_scatter_bf16": (i32, [vp, vp, vp, vp, C.POINTER(TsKept), u32, u32, vp]),
     "ts_qk_norm_rope_append_bf16": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, C.POINTER(TsKept), u32, u32, u32, u32, f32, vp]),
+    "ts_qk_norm_rope_append_q8": (i32, [vp, vp, vp, vp, vp, vp, vp, C.POINTER(TsRowsQ8), C.POINTER(TsKept), u32, u32, u32, u32, f32, vp]),
+    "ts_rows_unpack_q8": (i32, [C.POINTER(TsRowsQ8), vp, vp, vp, vp, C.POINTER(TsKept), u32, u32, u32, vp]),
+    "ts_attend_rows_q8_workspace_bytes": (sz, [u32, u32, u32, u32, u32, u32]),
+    "ts_attend_rows_q8": (i32, [vp, C.POINTER(TsRowsQ8), vp, vp, vp, C.POINTER(TsKept), u32, u32, u32, u32, u32, u32, f32, vp, sz, vp]),
+    "ts_select_blocks_q8_workspace_bytes": (sz, [u32, u32, u32, u32, u32]),
+    "ts_select_blocks_q8": (i32, [vp, C.POINTER(TsRowsQ8), vp, vp, vp, C.POINTER(TsKept), u32, u32, u32, u32, u32, u32, u32, u32, vp, sz, vp]),
+    "ts_attend_blocks_q8_workspace_bytes": (sz, [u32, u32, u32, u32, u32, u32]),
+    "ts_attend_blocks_q8": (i32, [vp, C.POINTER(TsRowsQ8), vp, vp, vp, vp, C.POINTER(TsKept), u32, u32, u32, u32, u32, u32, f32, vp, sz, vp]),
     "ts_rope_inv_freq": (None, [f32, u32, vp]),
     "ts_rope_angles": (i32, [vp, vp, u32, u32, f32, u32, vp]),
     "ts_rope": (i32, [vp, i32, vp, u32, u32, u32, i32, vp]),

@@ -4,6 +4,7 @@
 #include <cstdlib>
 #include <mutex>
 
+#include "rows_q8.cuh"
 #include "ts_common.cuh"
 #include "ts_kernels.cuh"
 #include "ts_ptx.cuh"
@@ -197,6 +198,110 @@ int ts_linear_q8_0(const void *x, const void *w, const void *a0, void *out, uint
     TS_REQUIRE(out_dtype == TS_BF16 || out_dtype == TS_F32, "linear (q8_0): out dtype %d is unknown", out_dtype);
     TS_REQUIRE(epilogue != TS_EPI_ADD || a0 != nullptr, "linear (q8_0): the add epilogue needs its operand");
     return linear_q8_0(x, w, a0, out, m, n, k, epilogue, scale, out_dtype, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+int ts_qk_norm_rope_append_q8(const void *qkv, const float *q_norm, const float *k_norm, const float *inv_freq,
+                              const uint32_t *slots, const uint32_t *positions, void *q_out, const ts_rows_q8 *kv,
+                              const ts_kept *kept, uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                              float eps, void *stream) {
+    TS_REQUIRE(qkv && inv_freq && slots && positions && q_out, "qk_norm_rope_append (q8): a buffer is NULL");
+    TS_REQUIRE(aligned16(qkv) && aligned16(q_out), "qk_norm_rope_append (q8): buffers must be 16-byte aligned");
+    RowsQ8Dev dev;
+    const int rc = rows_q8_to_dev("qk_norm_rope_append (q8)", kv, kept, kv_heads, width, &dev);
+    if (rc != TS_OK) return rc;
+    TS_REQUIRE(heads > 0, "qk_norm_rope_append (q8): no query heads");
+    if (rows == 0) return TS_OK;
+    return append_q8(qkv, q_norm, k_norm, inv_freq, slots, positions, q_out, dev, rows, heads, kv_heads, width, eps,
+                     (cudaStream_t)stream);
+}
+
+int ts_rows_unpack_q8(const ts_rows_q8 *kv, const uint32_t *slots, const uint32_t *positions, void *k_out, void *v_out,
+                      const ts_kept *kept, uint32_t rows, uint32_t kv_heads, uint32_t width, void *stream) {
+    TS_REQUIRE(slots && positions && k_out && v_out, "rows_unpack (q8): a buffer is NULL");
+    TS_REQUIRE(aligned16(k_out) && aligned16(v_out), "rows_unpack (q8): buffers must be 16-byte aligned");
+    RowsQ8Dev dev;
+    const int rc = rows_q8_to_dev("rows_unpack (q8)", kv, kept, kv_heads, width, &dev);
+    if (rc != TS_OK) return rc;
+    if (rows == 0) return TS_OK;
+    return unpack_q8(dev, slots, positions, k_out, v_out, rows, kv_heads, width, (cudaStream_t)stream);
+}
+
+size_t ts_attend_rows_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                                         uint32_t back) {
+    return attend_q8_workspace_bytes(rows, keys, heads, kv_heads, width, back, 0, 16);
+}
+
+// The checks that both attentions share; *done: there is nothing to launch.
+static int check_attend_q8(const char *what, const void *q, const ts_rows_q8 *kv, void *out, const uint32_t *slots,
+                           const uint32_t *positions, const ts_kept *kept, uint32_t rows, uint32_t keys, uint32_t heads,
+                           uint32_t kv_heads, uint32_t width, RowsQ8Dev *dev, bool *done, void *stream) {
+    TS_REQUIRE(q && out && slots && positions, "%s: a buffer is NULL", what);
+    TS_REQUIRE(aligned16(q) && aligned16(out), "%s: buffers must be 16-byte aligned", what);
+    const int rc = rows_q8_to_dev(what, kv, kept, kv_heads, width, dev);
+    if (rc != TS_OK) return rc;
+    TS_REQUIRE(heads > 0 && heads % kv_heads == 0, "%s: %u heads do not split over %u kv heads", what, heads, kv_heads);
+    *done = rows == 0 || keys == 0;
+    if (rows != 0 && keys == 0)  // nothing is kept: every row sees nothing
+        TS_CUDA(cudaMemsetAsync(out, 0, (size_t)rows * heads * width * 2, (cudaStream_t)stream));
+    return TS_OK;
+}
+
+int ts_attend_rows_q8(const void *q, const ts_rows_q8 *kv, void *out, const uint32_t *slots, const uint32_t *positions,
+                      const ts_kept *kept, uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                      uint32_t back, float scale, void *workspace, size_t workspace_bytes, void *stream) {
+    RowsQ8Dev dev;
+    bool done = false;
+    const int rc = check_attend_q8("attend_rows (q8)", q, kv, out, slots, positions, kept, rows, keys, heads, kv_heads, width, &dev,
+                                   &done, stream);
+    if (rc != TS_OK || done) return rc;
+    return attend_q8(q, dev, nullptr, out, slots, positions, rows, keys, heads, kv_heads, width, back, 0, scale, workspace,
+                     workspace_bytes, (cudaStream_t)stream);
+}
+
+size_t ts_select_blocks_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t kv_heads, uint32_t block, uint32_t count) {
+    return select_q8_workspace_bytes(rows, keys, kv_heads, block, count);
+}
+
+int ts_select_blocks_q8(const void *q, const ts_rows_q8 *kv, uint32_t *ids, const uint32_t *slots, const uint32_t *positions,
+                        const ts_kept *kept, uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                        uint32_t count, uint32_t first, uint32_t recent, void *workspace, size_t workspace_bytes,
+                        void *stream) {
+    TS_REQUIRE(q && ids && slots && positions, "select_blocks (q8): a buffer is NULL");
+    TS_REQUIRE(aligned16(q), "select_blocks (q8): q must be 16-byte aligned");
+    RowsQ8Dev dev;
+    const int rc = rows_q8_to_dev("select_blocks (q8)", kv, kept, kv_heads, width, &dev);
+    if (rc != TS_OK) return rc;
+    TS_REQUIRE(dev.bounds != nullptr, "select_blocks (q8): the rows have no key bounds");
+    TS_REQUIRE(heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 256,
+               "select_blocks (q8): %u heads do not split over %u kv heads, at most 256 each", heads, kv_heads);
+    TS_REQUIRE(count >= 1 && count <= 4096 && first <= count && recent <= count - first,
+               "select_blocks (q8): %u first and %u recent of %u blocks (1 to 4096)", first, recent, count);
+    if (rows == 0) return TS_OK;
+    if (keys == 0) {  // no block holds a position: every entry is spare
+        TS_CUDA(cudaMemsetAsync(ids, 0xFF, (size_t)rows * kv_heads * count * 4, (cudaStream_t)stream));
+        return TS_OK;
+    }
+    return select_q8(q, dev, ids, slots, positions, rows, keys, heads, kv_heads, width, count, first, recent, workspace,
+                     workspace_bytes, (cudaStream_t)stream);
+}
+
+size_t ts_attend_blocks_q8_workspace_bytes(uint32_t rows, uint32_t count, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                                           uint32_t block) {
+    return count == 0 ? 0 : attend_q8_workspace_bytes(rows, 1, heads, kv_heads, width, 0xFFFFFFFFu, count, block);
+}
+
+int ts_attend_blocks_q8(const void *q, const ts_rows_q8 *kv, const uint32_t *ids, void *out, const uint32_t *slots,
+                        const uint32_t *positions, const ts_kept *kept, uint32_t rows, uint32_t keys, uint32_t heads,
+                        uint32_t kv_heads, uint32_t width, uint32_t count, float scale, void *workspace,
+                        size_t workspace_bytes, void *stream) {
+    RowsQ8Dev dev;
+    bool done = false;
+    TS_REQUIRE(ids != nullptr && count > 0 && count <= (1u << 24), "attend_blocks (q8): ids is NULL or %u blocks are not 1 to 2^24", count);
+    const int rc = check_attend_q8("attend_blocks (q8)", q, kv, out, slots, positions, kept, rows, keys, heads, kv_heads, width,
+                                   &dev, &done, stream);
+    if (rc != TS_OK || done) return rc;
+    return attend_q8(q, dev, ids, out, slots, positions, rows, keys, heads, kv_heads, width, 0xFFFFFFFFu, count, scale, workspace,
+                     workspace_bytes, (cudaStream_t)stream);
 }
 
 int ts_wait_runs_out(uint64_t wait_ns, void *stream) {

@@ -12,7 +12,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import EPILOGUE, KEPT_KIND, KEPT_PAGE, LINEAR_PATH, TS_BF16, TS_F32, TsKept, check, lib
+from ._lib import EPILOGUE, KEPT_KIND, KEPT_PAGE, LINEAR_PATH, TS_BF16, TS_F32, TsKept, TsRowsQ8, check, lib
 
 _workspaces: dict = {}
 
@@ -188,6 +188,166 @@ def attend_rows_append(qkv, q_norm, k_norm, inv_freq, k_rows, v_rows, slots, pos
     check(lib.ts_attend_rows_append_bf16(_ptr(qkv), _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq), _ptr(k_rows), _ptr(v_rows),
                                          _ptr(out), _ptr(slots), _ptr(positions), C.byref(kc), rows, keys, heads, kv_heads,
                                          width, eps, scale, _ptr(ws), nbytes, _stream()))
+    return out
+
+
+@dataclass(frozen=True)
+class RowsQ8:
+    """Kept K and V rows as 8-bit codes: ts_rows_q8.  k, v int8 [blocks, kv_heads, block, width], k_scale, v_scale
+    f32 [blocks, kv_heads], k_bounds int8 [blocks, kv_heads, 2, width] or None (needed only to select blocks).  The
+    record holds the tensors; calls read their addresses each time."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    k_bounds: torch.Tensor | None = None
+
+    def __post_init__(self):
+        if self.k.dim() != 4:
+            _refuse("k must be int8 [blocks, kv_heads, block, width]")
+        blocks, kv_heads, block, width = self.k.shape
+        shapes = [(self.k, self.k.shape, torch.int8), (self.v, self.k.shape, torch.int8),
+                  (self.k_scale, (blocks, kv_heads), torch.float32), (self.v_scale, (blocks, kv_heads), torch.float32)]
+        if self.k_bounds is not None:
+            shapes.append((self.k_bounds, (blocks, kv_heads, 2, width), torch.int8))
+        for t, shape, dtype in shapes:
+            if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous() or t.device != self.k.device:
+                _refuse(f"8-bit rows: expected contiguous {dtype} {tuple(shape)} on {self.k.device}, got {t.dtype} "
+                        f"{tuple(t.shape)} on {t.device}")
+
+    @staticmethod
+    def empty(rows: int, kv_heads: int, width: int, block: int = 64, *, bounds: bool = True, device="cuda") -> "RowsQ8":
+        """Room for `rows` kept rows (a multiple of `block`); every scale 0, so that every row reads zero."""
+        if block not in (16, 32, 64) or rows <= 0 or rows % block:
+            _refuse(f"{rows} rows are not whole blocks of {block} (16, 32 or 64)")
+        blocks = rows // block
+        make = lambda *shape, dtype=torch.int8: torch.zeros(shape, dtype=dtype, device=device)  # noqa: E731
+        return RowsQ8(make(blocks, kv_heads, block, width), make(blocks, kv_heads, block, width),
+                      make(blocks, kv_heads, dtype=torch.float32), make(blocks, kv_heads, dtype=torch.float32),
+                      make(blocks, kv_heads, 2, width) if bounds else None)
+
+    def c(self) -> TsRowsQ8:
+        blocks, _, block, _ = self.k.shape
+        return TsRowsQ8(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                        self.k_bounds.data_ptr() if self.k_bounds is not None else None, block, blocks)
+
+
+def _refuse(message: str):
+    raise _lib.TesseraError(_lib.TS_ERR_BAD_INPUT, message)
+
+
+def _q8_call(kv: RowsQ8, kept: Kept, **tensors) -> tuple:
+    """Checks what a call over 8-bit rows is given, name -> (tensor or None, dtype, shape or None), and returns the
+    stream it goes to (the current one of the rows' device) and the addresses in order."""
+    dev = kv.k.device
+    if dev.type != "cuda":
+        _refuse("tensors must live on a CUDA device (there is no CPU path)")
+    if dev.index != torch.cuda.current_device():
+        _refuse(f"the rows are on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+    if kept.table is not None:
+        tensors["page table"] = (kept.table, torch.int32, None)
+    at = []
+    for name, (t, dtype, shape) in tensors.items():
+        if t is None:
+            at.append(None)
+            continue
+        if t.dtype != dtype or t.device != dev or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
+            _refuse(f"{name}: expected contiguous {dtype}{'' if shape is None else ' ' + str(list(shape))} on {dev}, got "
+                    f"{t.dtype} {list(t.shape)} on {t.device}")
+        at.append(t.data_ptr())
+    return _stream(), at
+
+
+def _scratch(nbytes: int, device) -> torch.Tensor | None:
+    """Scratch of one call, from the caching allocator: eager calls reuse it in stream order, a captured call keeps its
+    own in the graph's pool, so that two graphs never share it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def qk_norm_rope_append_q8(qkv, q_norm, k_norm, inv_freq, slots, positions, kv: RowsQ8, kept: Kept, heads: int, *, eps: float,
+                           out=None):
+    """Per-head norm (gains f32 [width] or None) and rotation, q out in bf16 [rows, heads, width], k and v into their
+    blocks: ts_qk_norm_rope_append_q8.  Rows that fall into the same block stand next to one another."""
+    rows = qkv.shape[0]
+    _, kv_heads, _, width = kv.k.shape
+    if out is None:
+        out = torch.empty((rows, heads, width), dtype=torch.bfloat16, device=qkv.device)
+    stream, (a_qkv, a_qn, a_kn, a_freq, a_slots, a_pos, a_out, *_) = _q8_call(
+        kv, kept, qkv=(qkv, torch.bfloat16, (rows, (heads + 2 * kv_heads) * width)), q_norm=(q_norm, torch.float32, (width,)),
+        k_norm=(k_norm, torch.float32, (width,)), inv_freq=(inv_freq, torch.float32, (width // 2,)),
+        slots=(slots, torch.int32, (rows,)), positions=(positions, torch.int32, (rows,)),
+        out=(out, torch.bfloat16, (rows, heads, width)))
+    if rows:
+        check(lib.ts_qk_norm_rope_append_q8(a_qkv, a_qn, a_kn, a_freq, a_slots, a_pos, a_out, kv.c(), kept.c(), rows, heads,
+                                            kv_heads, width, eps, stream))
+    return out
+
+
+def rows_unpack_q8(kv: RowsQ8, slots, positions, kept: Kept):
+    """The kept rows at (slots[r], positions[r]) as bf16 [rows, kv_heads, width], keys and values: ts_rows_unpack_q8."""
+    rows = slots.numel()
+    _, kv_heads, _, width = kv.k.shape
+    k_out = torch.empty((rows, kv_heads, width), dtype=torch.bfloat16, device=kv.k.device)
+    v_out = torch.empty_like(k_out)
+    stream, (a_slots, a_pos, *_) = _q8_call(kv, kept, slots=(slots, torch.int32, (rows,)), positions=(positions, torch.int32, (rows,)))
+    if rows:
+        check(lib.ts_rows_unpack_q8(kv.c(), a_slots, a_pos, k_out.data_ptr(), v_out.data_ptr(), kept.c(), rows, kv_heads, width,
+                                    stream))
+    return k_out, v_out
+
+
+def _heads_of(q, kv: RowsQ8) -> tuple:
+    _, kv_heads, block, width = kv.k.shape
+    if q.dim() != 3 or q.shape[2] != width or q.shape[1] % kv_heads:
+        _refuse(f"q {list(q.shape)} does not go with {kv_heads} kv heads of width {width}")
+    return q.shape[0], q.shape[1], kv_heads, block, width
+
+
+def attend_rows_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, *, scale: float, back=0xFFFFFFFF, out=None):
+    """Ragged causal attention over 8-bit kept rows, q and result bf16 [rows, heads, width]: ts_attend_rows_q8."""
+    rows, heads, kv_heads, _, width = _heads_of(q, kv)
+    if out is None:
+        out = torch.empty_like(q)
+    stream, (a_q, a_slots, a_pos, a_out, *_) = _q8_call(
+        kv, kept, q=(q, torch.bfloat16, None), slots=(slots, torch.int32, (rows,)), positions=(positions, torch.int32, (rows,)),
+        out=(out, torch.bfloat16, (rows, heads, width)))
+    nbytes = lib.ts_attend_rows_q8_workspace_bytes(rows, keys, heads, kv_heads, width, back)
+    ws = _scratch(nbytes, q.device)
+    if rows:
+        check(lib.ts_attend_rows_q8(a_q, kv.c(), a_out, a_slots, a_pos, kept.c(), rows, keys, heads, kv_heads, width, back, scale,
+                                    ws.data_ptr() if nbytes else None, nbytes, stream))
+    return out
+
+
+def select_blocks_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, count: int, *, first: int = 1, recent: int = 1):
+    """The `count` blocks of positions each row and kv head should read, ascending, int32 [rows, kv_heads, count] with -1
+    (UINT32_MAX) in spare entries: ts_select_blocks_q8."""
+    rows, heads, kv_heads, block, width = _heads_of(q, kv)
+    stream, (a_q, a_slots, a_pos, *_) = _q8_call(
+        kv, kept, q=(q, torch.bfloat16, None), slots=(slots, torch.int32, (rows,)), positions=(positions, torch.int32, (rows,)))
+    ids = torch.empty((rows, kv_heads, max(count, 0)), dtype=torch.int32, device=q.device)
+    nbytes = lib.ts_select_blocks_q8_workspace_bytes(rows, keys, kv_heads, block, count)
+    ws = _scratch(nbytes, q.device)
+    if rows:
+        check(lib.ts_select_blocks_q8(a_q, kv.c(), ids.data_ptr(), a_slots, a_pos, kept.c(), rows, keys, heads, kv_heads, width,
+                                      count, first, recent, ws.data_ptr() if nbytes else None, nbytes, stream))
+    return ids
+
+
+def attend_blocks_q8(q, kv: RowsQ8, ids, slots, positions, kept: Kept, keys: int, *, scale: float, out=None):
+    """Causal attention over the listed blocks only (ids int32 [rows, kv_heads, count], -1 = none): ts_attend_blocks_q8."""
+    rows, heads, kv_heads, block, width = _heads_of(q, kv)
+    count = ids.shape[-1]
+    if out is None:
+        out = torch.empty_like(q)
+    stream, (a_q, a_ids, a_slots, a_pos, a_out, *_) = _q8_call(
+        kv, kept, q=(q, torch.bfloat16, None), ids=(ids, torch.int32, (rows, kv_heads, count)), slots=(slots, torch.int32, (rows,)),
+        positions=(positions, torch.int32, (rows,)), out=(out, torch.bfloat16, (rows, heads, width)))
+    nbytes = lib.ts_attend_blocks_q8_workspace_bytes(rows, count, heads, kv_heads, width, block)
+    ws = _scratch(nbytes, q.device)
+    if rows:
+        check(lib.ts_attend_blocks_q8(a_q, kv.c(), a_ids, a_out, a_slots, a_pos, kept.c(), rows, keys, heads, kv_heads, width,
+                                      count, scale, ws.data_ptr() if nbytes else None, nbytes, stream))
     return out
 
 
