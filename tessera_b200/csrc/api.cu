@@ -114,6 +114,22 @@ int make_tensor_map_2d_plain(CUtensorMap *map, const void *base, uint64_t rows, 
     return TS_OK;
 }
 
+int make_tensor_map_codes(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint32_t box_cols, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return fail(TS_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {cols};
+    cuuint32_t box[2] = {box_cols, box_rows};
+    cuuint32_t elem[2] = {1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, elem,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(TS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %llu x %llu bytes, box %u x %u", (int)r,
+                    (unsigned long long)rows, (unsigned long long)cols, box_rows, box_cols);
+    return TS_OK;
+}
+
 int make_tensor_map_3d(CUtensorMap *map, const void *base, uint64_t outer, uint64_t rows, uint64_t cols,
                        uint64_t outer_stride, uint64_t row_stride, uint32_t box_rows, uint32_t box_cols) {
     EncodeTiledFn fn = encode_tiled();
@@ -170,8 +186,8 @@ int ts_set_pdl(int enabled) {
 
 int ts_device_status(void) {
     const int a = umma_take_status(), b = stream_take_status(), c = flash_take_status(), d = moe_take_status();
-    const int e = rows_take_status(), f = pair_take_status(), g = step_take_status();
-    return a ? a : b ? b : c ? c : d ? d : e ? e : f ? f : g;
+    const int e = rows_take_status(), f = pair_take_status(), g = step_take_status(), h = attend_q8_take_status();
+    return a ? a : b ? b : c ? c : d ? d : e ? e : f ? f : g ? g : h;
 }
 
 size_t ts_q8_0_bytes(size_t elements) { return q8_0_bytes(elements); }

@@ -1,26 +1,52 @@
 // Ragged attention over kept rows in 8 bits, whole slots or listed blocks.
 //
-// A tile of 16 query rows is (token, head) pairs: the G heads of a kv head's group times the T = 16 / G neighbouring
-// rows that share a slot (drafted tokens, a part of a prompt); the other rows of the tile repeat nothing and are never
-// stored.  Both products run on warp MMAs (m16n8k16, f16 in, f32 out): a code is exact in f16, a query row is brought
-// into f16's range by a power of two, which is exact for bf16 (values below 2^-24 of the row's largest lose digits that
-// no sum would keep).  Codes become f16 by setting them as the low bits of 1024 + 128 + code and subtracting 1152.
+// A tile is up to 16 query rows, (token, head) pairs: the G heads of a kv head's group times up to T = 16 / G neighbouring
+// rows that are the next positions of one slot (drafted tokens, a part of a prompt).  Both products run on warp MMAs
+// (m16n8k16, f16 in, f32 out) with the keys, then the channels, as the 16 rows and the queries as the 8 columns:
+//     S^T[16 keys x 8 queries] = K Q^T,      O^T[16 channels x 8 queries] += V^T P^T
+// so that a decode row of up to eight heads wastes nothing of the accumulators, and a second eight of queries shares the
+// converted K and V.  (With the queries as rows, half of every accumulator quad of a decode row is padding: 64 more
+// registers and twice the MMAs.)  A code is exact in f16: the bytes are set as the low bits of 1024 + (128 + code) and 1152
+// is subtracted; a query row is brought into f16's range by a power of two, which is exact for bf16 (values below 2^-24
+// of the row's largest lose digits that no sum would keep).
 //
 // The scales leave the products alone.  With s = raw * scale * k_scale in powers of two and
 //     x = s + log2(v_scale),   M = max x,   P = 2^(x - M)  <= 1   (f16 operand of P V)
 // the output is sum P code / sum P / v_scale: the block's value scale rides in the exponent, so that P needs no second
 // factor and stays within f16's range whatever the scales are, and M cancels.  A scale of zero counts as 2^-60, the
 // smallest that append writes.
+//
+// What feeds it.  Every warp is a worker of its own: it streams a step's codes (4 KB of K, 4 KB of V: 32 keys of width
+// 128) into its own ring with TMA, so that no warp waits for another and the only barrier is the one a copy completes on.
+// Lanes look up the pool's blocks and their scales 32 blocks at a time, one group ahead.  TMA swizzles the tiles (16-byte
+// pieces XORed with the row), which makes every ldmatrix read free of bank conflicts: K as it lies, V transposed in
+// 16-bit units (two channels), whose bytes the conversion separates.
+//
+// How the work is shared out.  The steps of all tiles, laid end to end, are cut into equal runs, one a worker: lengths
+// may be as uneven as they like.  A run has at most one tile that began before it and one that goes on after it, so a
+// worker leaves at most two partial results (M, sum, output) in the workspace; tiles that lie within a run go straight
+// to the output.  A second kernel folds the partials of a tile in the order of their keys: no atomics, the same bits on
+// every run.  With little work every tile is cut into pieces of four steps instead.
 #include <cmath>
 
 #include "rows_q8.cuh"
+#include "ts_ptx.cuh"
 
 namespace ts {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kHalfStage = 4096, kStage = 2 * kHalfStage;  // K codes, then V codes
+constexpr int kPiece = 4;                                  // steps of a worker's run at least
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kScaleFloor = 8.673617379884035e-19f;  // 2^-60
+
+// Blocks an SM holds and stages a warp has.  Twelve warps keep the issue slots busy where registers allow it (width
+// 256 needs up to 255 of them).
+template <int W>
+struct Shape {
+    static constexpr int CTAS = W == 256 ? 2 : 3, STAGES = W == 256 ? 3 : 2;
+};
 
 struct AttendParams {
     const uint16_t *q;
@@ -31,10 +57,13 @@ struct AttendParams {
     uint32_t rows, keys, heads, kv_heads, back, count;
     uint32_t group, part, parts;  // heads per kv head; heads of it in a tile, tiles it takes
     uint32_t tokens;              // rows a tile may hold
-    uint32_t chunk, chunks;       // 16-key steps per item, items per tile
+    uint32_t most;                // tile rows a partial has room for: tokens * part
+    uint32_t workers;
+    int merged;                   // whether the second kernel runs
     float scale;
-    float *part_o;   // [rows, heads, chunks, W]
-    float *part_ml;  // [rows, heads, chunks, 2]
+    float *part_o;    // [workers, 2, most, W]
+    float *part_ml;   // [workers, 2, most, 2]
+    uint4 *places;    // [rows, kv_heads * parts]: first and last worker of the row's tile, slot of the first, tile row
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -57,373 +86,621 @@ __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(v) : "r"(a), "r"(b));
     return v;
 }
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
 }
-// Bytes 0, 1 (sel 0x4140) or 2, 3 (sel 0x4342) of biased codes (code + 128) as two f16.
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
+    uint32_t v;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(v) : "r"(a));
+    return v;
+}
+// Two of the four biased codes (code + 128) as f16: bytes 0, 1 (0x4140), 2, 3 (0x4342), 0, 2 (0x4240) or 1, 3 (0x4341).
 __device__ __forceinline__ uint32_t codes_f16(uint32_t biased, uint32_t sel) {
     return sub_f16x2(__byte_perm(biased, 0x64646464u, sel), 0x64806480u);  // 1152 = 0x6480
 }
 
-// What a thread holds of the query tile: rows r0 = lane / 4 and r0 + 8.  The k index of an MMA step is permuted so that
-// a thread's bytes of a key are contiguous: in 64-wide chunk c, step s, thread j = lane % 4 has dims 64 c + 16 j + 4 s + 0..3.
-template <int W>
-struct QueryTile {
-    uint32_t a[W / 16][4];
-    float f0, f1;  // raw score -> power-of-two exponent, without the key scale
+// ---- a tile: which rows, which keys ----
+struct Tile {
+    uint32_t row, tokens, slot;
+    uint32_t from, to;  // keys that any of its rows sees (from >= to: none)
+    uint32_t base;      // the first block of positions it reads (whole slots)
+    uint32_t entries;   // blocks it reads, or listed blocks
+    uint32_t steps;     // at least one, so that every row's result is somebody's work
 };
 
-// Row m of the tile: token m / part, head m % part.
 template <int W>
-__device__ __forceinline__ void load_query(const AttendParams &p, uint32_t row, uint32_t tokens, uint32_t head0, uint32_t part,
-                                           uint32_t lane, QueryTile<W> &t) {
-    const uint32_t j = lane & 3;
-    float f[2];
-#pragma unroll
-    for (int half = 0; half < 2; half++) {
-        const uint32_t m = (lane >> 2) + 8 * half, token = m / part, head = m % part;
-        uint2 v[W / 16];
-        float most = 0.0f;
-#pragma unroll
-        for (int s = 0; s < W / 16; s++) {
-            v[s] = make_uint2(0, 0);
-            if (token < tokens)
-                v[s] = *reinterpret_cast<const uint2 *>(p.q + ((size_t)(row + token) * p.heads + head0 + head) * W + (s / 4) * 64 + j * 16 + (s % 4) * 4);
-            most = fmaxf(most, fmaxf(fmaxf(fabsf(bf16_lo(v[s].x)), fabsf(bf16_hi(v[s].x))), fmaxf(fabsf(bf16_lo(v[s].y)), fabsf(bf16_hi(v[s].y)))));
-        }
-        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-        uint32_t e = __float_as_uint(most) >> 23;  // the largest magnitude's exponent; 255: infinity
-        e = e < 1 ? 1 : e > 253 ? 253 : e;
-        const float down = __uint_as_float((254 - e) << 23);
-        f[half] = __uint_as_float(e << 23) * (p.scale * kLog2e);
-#pragma unroll
-        for (int s = 0; s < W / 16; s++) {
-            t.a[s][half] = pack_f16(bf16_lo(v[s].x) * down, bf16_hi(v[s].x) * down);
-            t.a[s][2 + half] = pack_f16(bf16_lo(v[s].y) * down, bf16_hi(v[s].y) * down);
-        }
-    }
-    t.f0 = f[0];
-    t.f1 = f[1];
-}
-
-template <int N>
-__device__ __forceinline__ void load_codes(const int8_t *p, uint32_t (&w)[N]) {
-    if constexpr (N == 2) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        w[0] = v.x; w[1] = v.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N / 4; i++) {
-            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
-            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) w[i] ^= 0x80808080u;
-}
-
-// Running softmax and output of a tile: rows r0 and r0 + 8, dims [lane % 4 * W / 4, + W / 4) of each.
-// o[i][0], [1]: row r0, dims 2 j * W / 8 + i and (2 j + 1) * W / 8 + i; [2], [3]: row r0 + 8.
-template <int W>
-struct Running {
-    float o[W / 8][4];
-    float m0, m1, l0, l1;
+struct Step {
+    static constexpr int KEYS = kHalfStage / W, UNITS = KEYS / 16;  // 64, 32, 16 keys; units of 16
+    static constexpr int HALVES = W == 256 ? 2 : 1, COLS = W == 64 ? 64 : 128;
 };
-
-// Sixteen keys: k, v point at their codes (row pitch W), the first key's position is `key0`; row r0 sees [lo0, hi0).
-template <int W>
-__device__ __forceinline__ void step16(const QueryTile<W> &t, Running<W> &run, const int8_t *k, const int8_t *v, float k_scale,
-                                       float v_scale, uint32_t key0, uint32_t lo0, uint32_t hi0, uint32_t lo1, uint32_t hi1,
-                                       uint32_t lane) {
-    const uint32_t r = lane >> 2, j = lane & 3;
-    float s[2][4];
-#pragma unroll
-    for (int n = 0; n < 2; n++) {
-        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < W / 64; c++) {
-            uint32_t w[4];
-            load_codes<4>(k + (8 * n + r) * W + c * 64 + j * 16, w);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                mma_f16(s[n], t.a[4 * c + i][0], t.a[4 * c + i][1], t.a[4 * c + i][2], t.a[4 * c + i][3], codes_f16(w[i], 0x4140),
-                        codes_f16(w[i], 0x4342));
-        }
-    }
-    const float vs = fmaxf(v_scale, kScaleFloor), lvs = log2_approx(vs), ivs = 1.0f / vs;
-    const float f0 = t.f0 * k_scale, f1 = t.f1 * k_scale;
-    float x[2][4], most0 = -INFINITY, most1 = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < 2; n++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const uint32_t key = key0 + 8 * n + 2 * j + e;
-            x[n][e] = key >= lo0 && key < hi0 ? fmaf(s[n][e], f0, lvs) : -INFINITY;
-            x[n][2 + e] = key >= lo1 && key < hi1 ? fmaf(s[n][2 + e], f1, lvs) : -INFINITY;
-            most0 = fmaxf(most0, x[n][e]);
-            most1 = fmaxf(most1, x[n][2 + e]);
-        }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        most0 = fmaxf(most0, __shfl_xor_sync(0xFFFFFFFFu, most0, o));
-        most1 = fmaxf(most1, __shfl_xor_sync(0xFFFFFFFFu, most1, o));
-    }
-    const float n0 = fmaxf(run.m0, most0), n1 = fmaxf(run.m1, most1);
-    const float z0 = n0 == -INFINITY ? 0.0f : n0, z1 = n1 == -INFINITY ? 0.0f : n1;  // nothing seen yet: 2^(-inf - 0) = 0
-    const float a0 = exp2_approx(run.m0 - z0), a1 = exp2_approx(run.m1 - z1);
-    run.m0 = n0;
-    run.m1 = n1;
-    float p[2][4], sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-    for (int n = 0; n < 2; n++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            p[n][e] = exp2_approx(x[n][e] - z0);
-            p[n][2 + e] = exp2_approx(x[n][2 + e] - z1);
-            sum0 += p[n][e];
-            sum1 += p[n][2 + e];
-        }
-    run.l0 = fmaf(sum0, ivs, run.l0 * a0);
-    run.l1 = fmaf(sum1, ivs, run.l1 * a1);
-    if (!__all_sync(0xFFFFFFFFu, a0 == 1.0f && a1 == 1.0f)) {
-#pragma unroll
-        for (int i = 0; i < W / 8; i++) {
-            run.o[i][0] *= a0;
-            run.o[i][1] *= a0;
-            run.o[i][2] *= a1;
-            run.o[i][3] *= a1;
-        }
-    }
-    const uint32_t pa0 = pack_f16(p[0][0], p[0][1]), pa1 = pack_f16(p[0][2], p[0][3]), pa2 = pack_f16(p[1][0], p[1][1]),
-                   pa3 = pack_f16(p[1][2], p[1][3]);
-    uint32_t w[4][W / 32];  // keys 2 j, 2 j + 1, 2 j + 8, 2 j + 9, this thread's W / 8 dims
-#pragma unroll
-    for (int i = 0; i < 4; i++) load_codes<W / 32>(v + (2 * j + (i & 1) + 8 * (i >> 1)) * W + r * (W / 8), w[i]);
-#pragma unroll
-    for (int i = 0; i < W / 32; i++) {
-        const uint32_t ab = __byte_perm(w[0][i], w[1][i], 0x5140), AB = __byte_perm(w[0][i], w[1][i], 0x7362);
-        const uint32_t cd = __byte_perm(w[2][i], w[3][i], 0x5140), CD = __byte_perm(w[2][i], w[3][i], 0x7362);
-        mma_f16(run.o[4 * i], pa0, pa1, pa2, pa3, codes_f16(ab, 0x4140), codes_f16(cd, 0x4140));
-        mma_f16(run.o[4 * i + 1], pa0, pa1, pa2, pa3, codes_f16(ab, 0x4342), codes_f16(cd, 0x4342));
-        mma_f16(run.o[4 * i + 2], pa0, pa1, pa2, pa3, codes_f16(AB, 0x4140), codes_f16(CD, 0x4140));
-        mma_f16(run.o[4 * i + 3], pa0, pa1, pa2, pa3, codes_f16(AB, 0x4342), codes_f16(CD, 0x4342));
-    }
-}
-
-// An item: (first row of a tile, kv head, heads' part, chunk).  `first_row` false: another item covers this row.
-struct Item {
-    uint32_t row, tokens, kvh, head0, part, chunk, slot;
-};
-
-__device__ __forceinline__ bool item_of(const AttendParams &p, uint32_t index, Item *it) {
-    it->chunk = index % p.chunks;
-    index /= p.chunks;
-    const uint32_t hp = index % p.parts;
-    index /= p.parts;
-    it->kvh = index % p.kv_heads;
-    it->row = index / p.kv_heads;
-    it->head0 = it->kvh * p.group + hp * p.part;
-    it->part = min(p.part, p.group - hp * p.part);
-    it->slot = p.slots[it->row];
-    it->tokens = 1;
-    if (p.tokens == 1) return true;
-    // Tiles begin at multiples of `tokens` and where a row is not the next position of the slot before it (or the same
-    // again): what a tile sees then spans at most back + tokens keys, which the number of chunks counts on.
-    auto follows = [&](uint32_t r) {
-        return r % p.tokens != 0 && p.slots[r] == p.slots[r - 1] && p.positions[r] - p.positions[r - 1] <= 1u;
-    };
-    if (follows(it->row)) return false;
-    while (it->row + it->tokens < p.rows && follows(it->row + it->tokens)) it->tokens++;
-    return true;
-}
 
 __device__ __forceinline__ void seen(const AttendParams &p, uint32_t pos, uint32_t *lo, uint32_t *hi) {
     *lo = pos > p.back ? pos - p.back : 0;
     *hi = pos < p.keys ? pos + 1 : p.keys;
 }
 
+// The tile that begins at `row`; false if the row lies in a tile that begins before it.
+template <int W, bool LIST>
+__device__ __forceinline__ bool tile_of(const AttendParams &p, uint32_t row, Tile *t) {
+    t->row = row;
+    t->tokens = 1;
+    t->slot = p.slots[row];
+    if (!LIST && p.tokens > 1) {
+        // Tiles begin at multiples of `tokens` and where a row is not the next position of the slot before it (or the same
+        // again).
+        auto follows = [&](uint32_t r) {
+            if (r % p.tokens == 0 || p.slots[r] != p.slots[r - 1]) return false;  // also: row 0 has none before it
+            const uint32_t was = p.positions[r - 1], is = p.positions[r];
+            return is >= was && is - was <= 1u;
+        };
+        if (follows(row)) return false;
+        while (row + t->tokens < p.rows && follows(row + t->tokens)) t->tokens++;
+    }
+    // positions ascend within a tile: the first row sees the earliest key, the last one the latest
+    uint32_t a, b;
+    seen(p, p.positions[row], &t->from, &b);
+    seen(p, p.positions[row + t->tokens - 1], &a, &t->to);
+    if (t->from >= t->to) t->from = t->to = 0;
+    if (LIST) {
+        t->base = 0;
+        t->entries = p.count;
+        t->steps = ((p.count << (p.kv.shift - 4)) + Step<W>::UNITS - 1) / Step<W>::UNITS;
+    } else {
+        t->base = t->from >> p.kv.shift;
+        t->entries = t->from < t->to ? ((t->to - 1) >> p.kv.shift) + 1 - t->base : 0;
+        t->steps = t->from < t->to ? (t->to - 1 - (t->base << p.kv.shift)) / Step<W>::KEYS + 1 : 1;
+    }
+    return true;
+}
+
+__device__ __forceinline__ uint32_t warp_total(uint32_t v) { return __reduce_add_sync(0xFFFFFFFFu, v); }
+
+// ---- the query operand: column r of eight is tile row 8 t + r; thread j of its four has channels 16 s + 4 j + 0..3 ----
+template <int W, int NT>
+struct Queries {
+    uint32_t b[NT][W / 16][2];
+    float f[NT][2];            // raw score -> power-of-two exponent, without the key scale, for columns 2 j, 2 j + 1
+    uint32_t lo[NT][2], hi[NT][2];  // keys those columns see
+};
+
+template <int W, int NT>
+__device__ __forceinline__ void load_queries(const AttendParams &p, const Tile &tile, uint32_t head0, uint32_t part, uint32_t lane,
+                                             Queries<W, NT> &qs) {
+    const uint32_t r = lane >> 2, j = lane & 3;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const uint32_t m = 8 * t + r, token = m / part, head = m - token * part;
+        uint2 v[W / 16];
+        float most = 0.0f;
+#pragma unroll
+        for (int s = 0; s < W / 16; s++) {
+            v[s] = make_uint2(0, 0);
+            if (token < tile.tokens) v[s] = *reinterpret_cast<const uint2 *>(p.q + ((size_t)(tile.row + token) * p.heads + head0 + head) * W + 16 * s + 4 * j);
+        }
+#pragma unroll
+        for (int s = 0; s < W / 16; s++)
+            most = fmaxf(most, fmaxf(fmaxf(fabsf(bf16_lo(v[s].x)), fabsf(bf16_hi(v[s].x))), fmaxf(fabsf(bf16_lo(v[s].y)), fabsf(bf16_hi(v[s].y)))));
+        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+        uint32_t e = __float_as_uint(most) >> 23;  // the largest magnitude's exponent; 255: infinity
+        e = e < 1 ? 1 : e > 253 ? 253 : e;
+        const float down = __uint_as_float((254 - e) << 23), f = __uint_as_float(e << 23) * (p.scale * kLog2e);
+#pragma unroll
+        for (int s = 0; s < W / 16; s++) {
+            qs.b[t][s][0] = pack_f16(bf16_lo(v[s].x) * down, bf16_hi(v[s].x) * down);
+            qs.b[t][s][1] = pack_f16(bf16_lo(v[s].y) * down, bf16_hi(v[s].y) * down);
+        }
+#pragma unroll
+        for (int e2 = 0; e2 < 2; e2++) {
+            qs.f[t][e2] = __shfl_sync(0xFFFFFFFFu, f, (2 * j + e2) * 4);
+            const uint32_t tok = (8 * t + 2 * j + e2) / part;
+            qs.lo[t][e2] = 1;
+            qs.hi[t][e2] = 0;
+            if (tok < tile.tokens) seen(p, p.positions[tile.row + tok], &qs.lo[t][e2], &qs.hi[t][e2]);
+        }
+    }
+}
+
+// ---- running softmax and output: columns 2 j + e; o[i][t][e], [2 + e]: channels 16 i + 2 r and 16 i + 2 r + 1 ----
+template <int W, int NT>
+struct Running {
+    float o[W / 16][NT][4];
+    float m[NT][2], l[NT][2];
+};
+
+// Shared-memory address of this lane's row for an ldmatrix.x4 of pieces c and c + 1 (c even) of unit u: matrices are
+// (keys 0-7, c), (keys 8-15, c), (keys 0-7, c + 1), (keys 8-15, c + 1).
+// Rows of 64 bytes (W = 64): piece ^ (key / 2 % 4); of 128 bytes: piece ^ (key % 8); W = 256: two such tiles.
 template <int W>
-__global__ void __launch_bounds__(kThreads) attend_q8_kernel(const AttendParams p) {
-    extern __shared__ float sm[];  // o [kWarps][16][W], then m, l [kWarps][16][2]
-    float *sm_o = sm, *sm_ml = sm + kWarps * 16 * W;
+__device__ __forceinline__ uint32_t piece_at(uint32_t tile, int u, int c, uint32_t lane) {
+    const uint32_t key = 16 * u + (lane & 15), side = lane >> 4;
+    if constexpr (W == 64) return tile + key * 64 + (((c + side) ^ (key >> 1 & 3)) << 4);
+    else return tile + (c >> 3) * (Step<W>::KEYS * 128) + key * 128 + ((((c & 7) + side) ^ (key & 7)) << 4);
+}
+
+// One step.  EDGE: some key of it is not seen by some row.  A unit without keys has key0 past every row's.
+template <int W, int NT, bool EDGE>
+__device__ __forceinline__ void step(const Queries<W, NT> &qs, Running<W, NT> &run, uint32_t tile, const float (&ks)[Step<W>::UNITS],
+                                     const float (&vs)[Step<W>::UNITS], const uint32_t (&key0)[Step<W>::UNITS], uint32_t lane) {
+    constexpr int U = Step<W>::UNITS;
+    const uint32_t r = lane >> 2;
+    float x[U][NT][4], most[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; t++) most[t][0] = most[t][1] = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) x[u][t][0] = x[u][t][1] = x[u][t][2] = x[u][t][3] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < W / 16; c += 2) {
+            uint32_t w[4];
+            ldsm_x4(piece_at<W>(tile, u, c, lane), w);
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] ^= 0x80808080u;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t a0 = codes_f16(w[2 * i], 0x4140), a1 = codes_f16(w[2 * i + 1], 0x4140), a2 = codes_f16(w[2 * i], 0x4342),
+                               a3 = codes_f16(w[2 * i + 1], 0x4342);
+#pragma unroll
+                for (int t = 0; t < NT; t++) mma_f16(x[u][t], a0, a1, a2, a3, qs.b[t][c + i]);
+            }
+        }
+        const float lv = log2_approx(fmaxf(vs[u], kScaleFloor));
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float f = qs.f[t][e] * ks[u];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    float &y = x[u][t][2 * k + e];
+                    y = fmaf(y, f, lv);
+                    if (EDGE) {
+                        const uint32_t key = key0[u] + 8 * k + r;
+                        if (key < qs.lo[t][e] || key >= qs.hi[t][e]) y = -INFINITY;
+                    }
+                    most[t][e] = fmaxf(most[t][e], y);
+                }
+            }
+    }
+    float scale[NT][2], top[NT][2];
+    bool same = true;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) most[t][e] = fmaxf(most[t][e], __shfl_xor_sync(0xFFFFFFFFu, most[t][e], o));
+            const float now = fmaxf(run.m[t][e], most[t][e]);
+            top[t][e] = now == -INFINITY ? 0.0f : now;  // nothing seen yet: 2^(-inf - 0) = 0
+            scale[t][e] = exp2_approx(run.m[t][e] - top[t][e]);
+            same = same && scale[t][e] == 1.0f;
+            run.m[t][e] = now;
+            run.l[t][e] *= scale[t][e];
+        }
+    if (!__all_sync(0xFFFFFFFFu, same)) {
+#pragma unroll
+        for (int i = 0; i < W / 16; i++)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    run.o[i][t][e] *= scale[t][e];
+                    run.o[i][t][2 + e] *= scale[t][e];
+                }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const float inv = __fdividef(1.0f, fmaxf(vs[u], kScaleFloor));
+        uint32_t b[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                p[e] = exp2_approx(x[u][t][e] - top[t][e]);
+                p[2 + e] = exp2_approx(x[u][t][2 + e] - top[t][e]);
+                run.l[t][e] = fmaf(p[e] + p[2 + e], inv, run.l[t][e]);
+            }
+            b[t][0] = transpose_8x8(pack_f16(p[0], p[1]));
+            b[t][1] = transpose_8x8(pack_f16(p[2], p[3]));
+        }
+#pragma unroll
+        for (int c = 0; c < W / 16; c += 2) {
+            uint32_t w[4];
+            ldsm_x4_trans(piece_at<W>(tile + kHalfStage, u, c, lane), w);
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] ^= 0x80808080u;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t a0 = codes_f16(w[2 * i], 0x4240), a1 = codes_f16(w[2 * i], 0x4341), a2 = codes_f16(w[2 * i + 1], 0x4240),
+                               a3 = codes_f16(w[2 * i + 1], 0x4341);
+#pragma unroll
+                for (int t = 0; t < NT; t++) mma_f16(run.o[c + i][t], a0, a1, a2, a3, b[t]);
+            }
+        }
+    }
+}
+
+// 32 blocks' places in the pool and scales, one a lane: entry `first` + lane of the tile's blocks.
+struct Group {
+    uint32_t blk, id;  // pool block or kNoBlock; which block of the slot's positions it is
+    float ks, vs;
+};
+
+template <bool LIST>
+__device__ __forceinline__ Group group_of(const AttendParams &p, const Tile &t, uint32_t kvh, uint32_t first, uint32_t lane) {
+    Group g = {kNoBlock, 0, 0.0f, 0.0f};
+    const uint32_t e = first + lane;
+    if (e < t.entries) {
+        g.id = LIST ? p.ids[((size_t)t.row * p.kv_heads + kvh) * p.count + e] : t.base + e;
+        if (((uint64_t)g.id << p.kv.shift) < t.to) g.blk = block_of(p.kv, t.slot, g.id);
+        if (g.blk != kNoBlock) {
+            const size_t at = (size_t)g.blk * p.kv_heads + kvh;
+            g.ks = p.kv.k_scale[at];
+            g.vs = p.kv.v_scale[at];
+        }
+    }
+    return g;
+}
+
+// A warp's ring: the next stage to complete and the parity each completes with.
+struct Ring {
+    uint32_t tiles;  // shared-memory address
+    uint64_t *full;
+    uint32_t stage, parity;
+    bool ok;  // false: a wait ran out, nothing is copied or computed any more
+};
+
+// Where a tile's result goes: the output, or a partial.
+struct Target {
+    bool partial;
+    size_t slot;  // worker * 2 + 0 or 1
+};
+
+template <int W, int NT, bool LIST>
+__device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtensorMap *map_k, const CUtensorMap *map_v, const Tile &tile,
+                                             uint32_t kvh, uint32_t head0, uint32_t part, uint32_t begin, uint32_t end, Target to,
+                                             Ring &ring, int *status, uint32_t lane) {
+    using namespace ptx;
+    constexpr int KEYS = Step<W>::KEYS, U = Step<W>::UNITS, HALVES = Step<W>::HALVES, COLS = Step<W>::COLS, STAGES = Shape<W>::STAGES;
+    const uint32_t in_block = p.kv.shift - 4;  // log2 of a block's 16-key units
+    Running<W, NT> run;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int i = 0; i < W / 16; i++) run.o[i][t][0] = run.o[i][t][1] = run.o[i][t][2] = run.o[i][t][3] = 0.0f;
+        run.m[t][0] = run.m[t][1] = -INFINITY;
+        run.l[t][0] = run.l[t][1] = 0.0f;
+    }
+    if (tile.from < tile.to) {
+        uint32_t first = (begin * U) >> in_block;  // entry of lane 0 of the current group
+        Group now = group_of<LIST>(p, tile, kvh, first, lane);
+        Group next = group_of<LIST>(p, tile, kvh, first + 32, lane);
+        // Copies of step s into stage `at`; the current or the next group has its blocks.
+        auto copy = [&](uint32_t s, uint32_t at) {
+            const uint32_t dst = ring.tiles + at * kStage, bar = smem_addr(&ring.full[at]);
+            uint32_t blk[U], bytes = 0;
+            const uint32_t per = 1u << in_block, span = per < (uint32_t)U ? per : U;  // units of one copy
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint32_t e = ((s * U + u) >> in_block) - first;
+                const uint32_t a = __shfl_sync(0xFFFFFFFFu, now.blk, e & 31), b = __shfl_sync(0xFFFFFFFFu, next.blk, e & 31);
+                blk[u] = e < 32 ? a : b;
+                if ((u & (span - 1)) == 0 && blk[u] != kNoBlock) bytes += span * 16 * W * 2;
+            }
+            if (lane == 0) {
+                mbar_expect_tx(&ring.full[at], bytes);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if ((u & (span - 1)) != 0 || blk[u] == kNoBlock) continue;
+                    const int32_t y = (int32_t)(((blk[u] * p.kv_heads + kvh) << p.kv.shift) + (((s * U + u) & (per - 1)) << 4));
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++) {
+                        copy_codes(dst + (h * KEYS + 16 * u) * COLS, map_k, bar, h * COLS, y);
+                        copy_codes(dst + kHalfStage + (h * KEYS + 16 * u) * COLS, map_v, bar, h * COLS, y);
+                    }
+                }
+            }
+        };
+        uint32_t ahead = begin;
+        for (; ahead < end && ahead < begin + STAGES; ahead++) copy(ahead, (ring.stage + (ahead - begin)) % STAGES);
+        Queries<W, NT> qs;
+        load_queries<W, NT>(p, tile, head0, part, lane, qs);
+        uint32_t all_lo = 0, all_hi = 0;  // keys that every row of the tile sees
+        {
+            uint32_t x;
+            seen(p, p.positions[tile.row], &x, &all_hi);
+            seen(p, p.positions[tile.row + tile.tokens - 1], &all_lo, &x);
+        }
+        for (uint32_t s = begin; s < end; s++) {
+            if (((s * U) >> in_block) - first >= 32) {
+                first += 32;
+                now = next;
+                next = group_of<LIST>(p, tile, kvh, first + 32, lane);
+            }
+            float ks[U], vs[U];
+            uint32_t key0[U];
+            bool edge = false;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint32_t unit = s * U + u, e = ((unit >> in_block) - first) & 31;
+                ks[u] = __shfl_sync(0xFFFFFFFFu, now.ks, e);
+                vs[u] = __shfl_sync(0xFFFFFFFFu, now.vs, e);
+                const uint32_t blk = __shfl_sync(0xFFFFFFFFu, now.blk, e), id = __shfl_sync(0xFFFFFFFFu, now.id, e);
+                key0[u] = blk == kNoBlock ? 0xFFFFFFF0u : (id << p.kv.shift) + ((unit & ((1u << in_block) - 1)) << 4);
+                edge = edge || key0[u] < all_lo || key0[u] + 16 > all_hi || blk == kNoBlock;
+            }
+            ring.ok = mbar_wait(&ring.full[ring.stage], ring.parity >> ring.stage & 1);
+            ring.parity ^= 1u << ring.stage;
+            if (!__all_sync(0xFFFFFFFFu, ring.ok)) {
+                ring.ok = false;  // the other copies are waited for, as long, before the block may end
+                for (uint32_t i = s + 1; i < ahead; i++) {
+                    ring.stage = (ring.stage + 1) % STAGES;
+                    mbar_wait(&ring.full[ring.stage], ring.parity >> ring.stage & 1);
+                }
+                if (lane == 0) atomicExch(status, TS_ERR_TIMEOUT);
+                return;
+            }
+            const uint32_t at = ring.tiles + ring.stage * kStage;
+            if (edge) step<W, NT, true>(qs, run, at, ks, vs, key0, lane);
+            else step<W, NT, false>(qs, run, at, ks, vs, key0, lane);
+            __syncwarp();
+            if (ahead < end) {
+                copy(ahead, ring.stage);
+                ahead++;
+            }
+            ring.stage = (ring.stage + 1) % STAGES;
+        }
+    }
+    // ---- this thread's channels of tile rows 8 t + 2 j + e ----
+    const uint32_t r = lane >> 2, j = lane & 3;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float l = run.l[t][e];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+            const uint32_t m = 8 * t + 2 * j + e;
+            if (m >= tile.tokens * part) continue;
+            if (!to.partial) {
+                const uint32_t token = m / part;
+                uint16_t *out = p.out + ((size_t)(tile.row + token) * p.heads + head0 + m - token * part) * W + 2 * r;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                for (int i = 0; i < W / 16; i++)
+                    *reinterpret_cast<uint32_t *>(out + 16 * i) = pack_bf16(run.o[i][t][e] * inv, run.o[i][t][2 + e] * inv);
+            } else {
+                float *o = p.part_o + (to.slot * p.most + m) * W + 2 * r;
+#pragma unroll
+                for (int i = 0; i < W / 16; i++) *reinterpret_cast<float2 *>(o + 16 * i) = make_float2(run.o[i][t][e], run.o[i][t][2 + e]);
+                if (r == 0) *reinterpret_cast<float2 *>(p.part_ml + (to.slot * p.most + m) * 2) = make_float2(run.m[t][e], l);
+            }
+        }
+}
+
+template <int W, bool LIST>
+__global__ void __launch_bounds__(kThreads, Shape<W>::CTAS)
+attend_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttendParams p, int *status) {
+    using namespace ptx;
+    constexpr int STAGES = Shape<W>::STAGES;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ uint64_t bars[kWarps][STAGES];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t worker = warp * gridDim.x + blockIdx.x;  // few workers spread over the SMs
+    Ring ring = {smem_addr(smem) + warp * (STAGES * kStage), bars[warp], 0, 0, true};
+    if (lane == 0) {
+        for (int s = 0; s < STAGES; s++) mbar_init(&ring.full[s], 1);
+        fence_barrier_init();
+    }
+    __syncwarp();
     pdl_wait();
-    Item it;
-    if (!item_of(p, blockIdx.x, &it)) {
-        pdl_launch_dependents();
-        return;
-    }
-    const uint32_t B = 1u << p.kv.shift;
-    uint32_t lo0 = 1, hi0 = 0, lo1 = 1, hi1 = 0, lo = 0xFFFFFFFFu, hi = 0;
-    for (uint32_t t = 0; t < it.tokens; t++) {
-        uint32_t a, b;
-        seen(p, p.positions[it.row + t], &a, &b);
-        if (a < b) {
-            lo = min(lo, a);
-            hi = max(hi, b);
-        }
-        if ((lane >> 2) / it.part == t) lo0 = a, hi0 = b;
-        if (((lane >> 2) + 8) / it.part == t) lo1 = a, hi1 = b;
-    }
-    QueryTile<W> tile;
-    load_query<W>(p, it.row, it.tokens, it.head0, it.part, lane, tile);
-    Running<W> run;
-#pragma unroll
-    for (int i = 0; i < W / 8; i++) run.o[i][0] = run.o[i][1] = run.o[i][2] = run.o[i][3] = 0.0f;
-    run.m0 = run.m1 = -INFINITY;
-    run.l0 = run.l1 = 0.0f;
-    // 16-key steps [begin, end) of this item
-    const uint32_t base = p.ids ? 0 : lo >> 4, steps = p.ids ? p.count << (p.kv.shift - 4) : lo < hi ? ((hi + 15) >> 4) - base : 0;
-    const uint32_t begin = it.chunk * p.chunk, end = min(steps, begin + p.chunk);
-    const uint32_t *list = p.ids ? p.ids + ((size_t)it.row * p.kv_heads + it.kvh) * p.count : nullptr;
-    for (uint32_t s = begin + warp; s < end; s += kWarps) {
-        uint32_t key0;
-        if (p.ids) {
-            const uint32_t b = list[s >> (p.kv.shift - 4)];
-            if (((uint64_t)b << p.kv.shift) >= hi) continue;
-            key0 = (b << p.kv.shift) + ((s << 4) & (B - 1));
-            if (key0 >= hi) continue;
+    if (worker < p.workers) {
+        // ---- the steps of all tiles, and this worker's run of them ----
+        const uint32_t per_row = p.kv_heads * p.parts;
+        auto steps_of = [&](uint32_t row) {
+            Tile t;
+            return row < p.rows && tile_of<W, LIST>(p, row, &t) ? t.steps : 0u;
+        };
+        uint64_t steps = 0, pieces = 0;
+        if (LIST) {
+            const uint32_t n = steps_of(0);
+            steps = (uint64_t)n * p.rows;
+            pieces = (uint64_t)((n + kPiece - 1) / kPiece) * p.rows;
         } else {
-            key0 = (base + s) << 4;
+            for (uint32_t base = 0; base < p.rows; base += 32) {
+                const uint32_t n = steps_of(base + lane);
+                steps += warp_total(n);
+                pieces += warp_total((n + kPiece - 1) / kPiece);
+            }
         }
-        const uint32_t blk = block_of(p.kv, it.slot, key0 >> p.kv.shift);
-        if (blk == kNoBlock) continue;
-        const size_t at = (size_t)blk * p.kv_heads + it.kvh;
-        const size_t off = ((at << p.kv.shift) + (key0 & (B - 1))) * W;
-        step16<W>(tile, run, p.kv.k + off, p.kv.v + off, p.kv.k_scale[at], p.kv.v_scale[at], key0, lo0, hi0, lo1, hi1, lane);
-    }
-    // ---- fold the warps ----
+        const bool padded = pieces * per_row <= p.workers;  // every tile in pieces of its own
+        const uint64_t total = (padded ? pieces * kPiece : steps) * per_row;
+        const uint32_t run = padded ? kPiece : (uint32_t)((total + p.workers - 1) / p.workers);
+        uint64_t at = (uint64_t)worker * run;
+        const uint64_t end = at + run < total ? at + run : total;
+        // the row in whose steps the run begins
+        uint64_t before = 0;  // steps of earlier rows, all kv heads
+        uint32_t row = 0;
+        if (at < end) {
+            auto taken = [&](uint32_t n) { return (uint64_t)(padded ? (n + kPiece - 1) / kPiece * kPiece : n) * per_row; };
+            if (LIST) {
+                const uint64_t each = taken(steps_of(0));
+                row = (uint32_t)(at / each);
+                before = row * each;
+            } else {
+                for (uint32_t base = 0; base < p.rows; base += 32) {
+                    const uint32_t n = steps_of(base + lane);
+                    uint64_t mine = taken(n), sum = mine;
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        run.l0 += __shfl_xor_sync(0xFFFFFFFFu, run.l0, o);
-        run.l1 += __shfl_xor_sync(0xFFFFFFFFu, run.l1, o);
-    }
-    {
-        const uint32_t r = lane >> 2, j = lane & 3;
-        float *o0 = sm_o + (warp * 16 + r) * W + j * (W / 4), *o1 = o0 + 8 * W;
-#pragma unroll
-        for (int i = 0; i < W / 8; i++) {
-            o0[i] = run.o[i][0];
-            o0[W / 8 + i] = run.o[i][1];
-            o1[i] = run.o[i][2];
-            o1[W / 8 + i] = run.o[i][3];
-        }
-        if (j == 0) {
-            float *ml = sm_ml + (warp * 16 + r) * 2;
-            ml[0] = run.m0;
-            ml[1] = run.l0;
-            ml[16] = run.m1;
-            ml[17] = run.l1;
-        }
-    }
-    __syncthreads();
-    const uint32_t live = it.tokens * it.part;
-    for (uint32_t i = threadIdx.x; i < live * W; i += kThreads) {
-        const uint32_t m = i / W, d = i % W;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) top = fmaxf(top, sm_ml[(w * 16 + m) * 2]);
-        const float z = top == -INFINITY ? 0.0f : top;
-        float l = 0.0f, o = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            const float f = exp2_approx(sm_ml[(w * 16 + m) * 2] - z);
-            l = fmaf(sm_ml[(w * 16 + m) * 2 + 1], f, l);
-            o = fmaf(sm_o[(w * 16 + m) * W + d], f, o);
-        }
-        const size_t head = (size_t)(it.row + m / it.part) * p.heads + it.head0 + m % it.part;
-        if (p.chunks == 1) {
-            p.out[head * W + d] = l == 0.0f ? (uint16_t)0 : bf16_bits(o / l);
-        } else {
-            const size_t at = head * p.chunks + it.chunk;
-            p.part_o[at * W + d] = o;
-            if (d == 0) {
-                p.part_ml[at * 2] = top;
-                p.part_ml[at * 2 + 1] = l;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const uint64_t other = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+                        if (lane >= (uint32_t)o) sum += other;
+                    }
+                    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + sum > at);
+                    if (hit) {
+                        const int l = __ffs(hit) - 1;
+                        row = base + l;
+                        before += __shfl_sync(0xFFFFFFFFu, sum - mine, l);
+                        break;
+                    }
+                    before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+                }
+            }
+            bool begun = false;  // whether the run has had a tile already
+            while (at < end && row < p.rows && ring.ok) {
+                Tile tile;
+                if (!tile_of<W, LIST>(p, row, &tile)) {
+                    row++;
+                    continue;
+                }
+                const uint32_t n = padded ? (tile.steps + kPiece - 1) / kPiece * kPiece : tile.steps;
+                while (at < end && at < before + (uint64_t)n * per_row && ring.ok) {
+                    const uint32_t h = (uint32_t)((at - before) / n), s0 = (uint32_t)((at - before) % n);
+                    const uint64_t start = at - s0;
+                    const uint32_t s1 = (uint32_t)min((uint64_t)n, end - start);
+                    const uint32_t kvh = h / p.parts, hp = h % p.parts;
+                    const uint32_t head0 = kvh * p.group + hp * p.part, part = min(p.part, p.group - hp * p.part);
+                    const uint32_t w0 = (uint32_t)(start / run), w1 = (uint32_t)((start + tile.steps - 1) / run);
+                    if (s0 == 0 && p.merged && lane < tile.tokens)
+                        p.places[(size_t)(row + lane) * per_row + h] = make_uint4(w0, w1, start % run != 0, lane * part);
+                    const Target to = {w0 != w1, (size_t)worker * 2 + begun};
+                    const uint32_t stop = min(s1, tile.steps);
+                    if (tile.tokens * part <= 8)
+                        attend_steps<W, 1, LIST>(p, &map_k, &map_v, tile, kvh, head0, part, s0, stop, to, ring, status, lane);
+                    else
+                        attend_steps<W, 2, LIST>(p, &map_k, &map_v, tile, kvh, head0, part, s0, stop, to, ring, status, lane);
+                    begun = true;
+                    at = start + s1;
+                }
+                before += (uint64_t)n * per_row;
+                row++;
             }
         }
     }
     pdl_launch_dependents();
 }
 
-// One block per (row, head): folds the chunks in ascending order.
+// One block per (row, head): folds the partials of its tile in the order of their keys.
 template <int W>
 __global__ void __launch_bounds__(W) attend_q8_merge_kernel(const AttendParams p) {
     pdl_wait();
-    const size_t head = blockIdx.x, at = head * p.chunks;
-    float top = -INFINITY;
-    for (uint32_t c = 0; c < p.chunks; c++) top = fmaxf(top, p.part_ml[(at + c) * 2]);
-    const float z = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f, o = 0.0f;
-    for (uint32_t c = 0; c < p.chunks; c++) {
-        const float f = exp2_approx(p.part_ml[(at + c) * 2] - z);
-        l = fmaf(p.part_ml[(at + c) * 2 + 1], f, l);
-        o = fmaf(p.part_o[(at + c) * W + threadIdx.x], f, o);
+    const uint32_t row = blockIdx.x / p.heads, head = blockIdx.x % p.heads, d = threadIdx.x;
+    const uint32_t kvh = head / p.group, in = head % p.group, hp = in / p.part;
+    const uint4 place = p.places[((size_t)row * p.kv_heads + kvh) * p.parts + hp];
+    const uint32_t m = place.w + in % p.part;
+    if (place.x < place.y && place.y < p.workers && place.z < 2 && m < p.most) {  // else its one worker wrote it (or gave up)
+        auto slot = [&](uint32_t w) { return ((size_t)w * 2 + (w == place.x ? place.z : 0)) * p.most + m; };
+        float top = -INFINITY;
+        for (uint32_t w = place.x; w <= place.y; w++) top = fmaxf(top, p.part_ml[slot(w) * 2]);
+        const float z = top == -INFINITY ? 0.0f : top;
+        float l = 0.0f, o = 0.0f;
+        for (uint32_t w = place.x; w <= place.y; w++) {
+            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + slot(w) * 2);
+            const float f = exp2_approx(ml.x - z);
+            l = fmaf(ml.y, f, l);
+            o = fmaf(p.part_o[slot(w) * W + d], f, o);
+        }
+        p.out[((size_t)row * p.heads + head) * W + d] = l == 0.0f ? (uint16_t)0 : bf16_bits(o / l);
     }
     pdl_launch_dependents();
-    p.out[head * W + threadIdx.x] = l == 0.0f ? (uint16_t)0 : bf16_bits(o / l);
 }
 
+__device__ int g_attend_status = 0;
+
 struct Plan {
-    uint32_t part, parts, tokens, chunk, chunks;
+    uint32_t part, parts, tokens, workers;
+    bool merged;
+    size_t o_bytes, ml_bytes, places_bytes;
+    size_t bytes() const { return merged ? o_bytes + ml_bytes + places_bytes : 0; }
 };
 
-Plan plan_of(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t back, uint32_t count, uint32_t block) {
+Plan plan_of(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width, uint32_t back, uint32_t count,
+             uint32_t block) {
     Plan s;
-    const uint32_t group = heads / kv_heads;
+    const uint32_t group = heads / kv_heads, step = kHalfStage / width;
     s.part = group < 16 ? group : 16;
     s.parts = ceil_div(group, s.part);
     s.tokens = count || s.parts > 1 ? 1 : 16 / s.part;
-    uint64_t span = keys;  // keys a tile may see, in 16-key steps below
+    uint64_t span = keys;  // keys a tile may see; the first of them is anywhere in its block of 64 at most
     if (!count && (uint64_t)back + s.tokens < span) span = (uint64_t)back + s.tokens;
-    const uint64_t steps = count ? (uint64_t)count * (block / 16) : (span + 15) / 16 + 1;
-    const uint64_t tiles = (uint64_t)rows * kv_heads * s.parts;
-    const uint64_t want = ((uint64_t)sm_count() * 4 + tiles - 1) / tiles;
-    uint64_t chunk = (steps + want - 1) / want;
-    if (chunk < 16) chunk = 16;
-    if (chunk > steps) chunk = steps;
-    s.chunk = (uint32_t)(chunk ? chunk : 1);
-    s.chunks = (uint32_t)((steps + s.chunk - 1) / s.chunk);
-    if (s.chunks == 0) s.chunks = 1;
+    const uint64_t steps = count ? ((uint64_t)count * block + step - 1) / step : (span + 63 + step - 1) / step;
+    const uint64_t most = (uint64_t)sm_count() * (width == 256 ? Shape<256>::CTAS : Shape<128>::CTAS) * kWarps;
+    const uint64_t pieces = (uint64_t)rows * kv_heads * s.parts * ((steps + kPiece - 1) / kPiece);
+    s.workers = (uint32_t)(pieces < most ? pieces : most);
+    // Without a second kernel only where no tile can be cut: each fits one piece and there is a worker for every piece.
+    s.merged = steps > kPiece || pieces > most;
+    s.o_bytes = (size_t)s.workers * 2 * s.tokens * s.part * width * sizeof(float);
+    s.ml_bytes = align_up((size_t)s.workers * 2 * s.tokens * s.part * 2 * sizeof(float), 16);
+    s.places_bytes = (size_t)rows * kv_heads * s.parts * sizeof(uint4);
     return s;
 }
 
-template <int W>
-int launch_attend(const AttendParams &p, uint32_t items, cudaStream_t stream) {
-    const size_t smem = (size_t)kWarps * 16 * (W + 2) * sizeof(float);
+template <int W, bool LIST>
+int launch_attend(const AttendParams &p, cudaStream_t stream) {
+    constexpr size_t smem = kWarps * Shape<W>::STAGES * kStage;
     static OncePerDevice configured;
     if (configured.needs()) {
-        TS_CUDA(cudaFuncSetAttribute(attend_q8_kernel<W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        TS_CUDA(cudaFuncSetAttribute(attend_q8_kernel<W, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         configured.done();
     }
-    cudaError_t e = launch(attend_q8_kernel<W>, dim3(items), dim3(kThreads), smem, stream, pdl_enabled(), p);
-    if (e == cudaSuccess && p.chunks > 1)
-        e = launch(attend_q8_merge_kernel<W>, dim3(p.rows * p.heads), dim3(W), 0, stream, pdl_enabled(), p);
+    int *status = nullptr;
+    TS_CUDA(cudaGetSymbolAddress((void **)&status, g_attend_status));
+    // Codes as rows of `width` bytes; a copy takes up to a block's rows of one kv head.
+    CUtensorMap map_k, map_v;
+    const uint64_t rows = ((uint64_t)p.kv.blocks * p.kv_heads) << p.kv.shift;
+    const uint32_t box = min(1u << p.kv.shift, (uint32_t)Step<W>::KEYS);
+    int rc = make_tensor_map_codes(&map_k, p.kv.k, rows, W, Step<W>::COLS, box);
+    if (rc == TS_OK) rc = make_tensor_map_codes(&map_v, p.kv.v, rows, W, Step<W>::COLS, box);
+    if (rc != TS_OK) return rc;
+    const uint32_t grid = min(p.workers, (uint32_t)sm_count() * Shape<W>::CTAS);
+    cudaError_t e = launch(attend_q8_kernel<W, LIST>, dim3(grid), dim3(kThreads), smem, stream, pdl_enabled(), map_k, map_v, p, status);
+    if (e == cudaSuccess && p.merged)  // always as a dependent launch: it waits for the partials itself
+        e = launch(attend_q8_merge_kernel<W>, dim3(p.rows * p.heads), dim3(W), 0, stream, true, p);
     if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of attend (q8) failed: %s", cudaGetErrorString(e));
     return TS_OK;
 }
 
 }  // namespace
 
+int attend_q8_take_status() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_attend_status, sizeof(int)) != cudaSuccess) return TS_ERR_CUDA;
+    if (v != 0) cudaMemcpyToSymbol(g_attend_status, &zero, sizeof(int));
+    return v;
+}
+
 size_t attend_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width, uint32_t back,
                                  uint32_t count, uint32_t block) {
     if (rows == 0 || keys == 0 || heads == 0 || kv_heads == 0 || heads % kv_heads) return 0;
-    const Plan s = plan_of(rows, keys, heads, kv_heads, back, count, block);
-    return s.chunks > 1 ? (size_t)rows * heads * s.chunks * (width + 2) * sizeof(float) : 0;
+    if (width != 64 && width != 128 && width != 256) return 0;
+    return plan_of(rows, keys, heads, kv_heads, width, back, count, block).bytes();
 }
 
 int attend_q8(const void *q, const RowsQ8Dev &kv, const uint32_t *ids, void *out, const uint32_t *slots,
               const uint32_t *positions, uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,
               uint32_t back, uint32_t count, float scale, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
-    const Plan s = plan_of(rows, keys, heads, kv_heads, back, count, 1u << kv.shift);
-    const size_t need = s.chunks > 1 ? (size_t)rows * heads * s.chunks * (width + 2) * sizeof(float) : 0;
+    const Plan s = plan_of(rows, keys, heads, kv_heads, width, back, count, 1u << kv.shift);
+    const size_t need = s.bytes();
     TS_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace != nullptr && aligned16(workspace))),
                "attend (q8): workspace of %zu bytes is smaller than the %zu needed, or not 16-byte aligned", workspace_bytes, need);
-    const uint64_t items = (uint64_t)rows * kv_heads * s.parts * s.chunks;
-    TS_REQUIRE(items < 0x7FFFFFFFull && (uint64_t)rows * heads < 0x7FFFFFFFull, "attend (q8): %u rows are too many for one launch", rows);
+    TS_REQUIRE((uint64_t)rows * heads < 0x7FFFFFFFull, "attend (q8): %u rows are too many for one launch", rows);
+    TS_REQUIRE((((uint64_t)kv.blocks * kv_heads) << kv.shift) < 0x7FFFFFFFull, "attend (q8): a pool of %u blocks is too large", kv.blocks);
     AttendParams p = {};
     p.q = (const uint16_t *)q;
     p.kv = kv;
@@ -441,14 +718,18 @@ int attend_q8(const void *q, const RowsQ8Dev &kv, const uint32_t *ids, void *out
     p.part = s.part;
     p.parts = s.parts;
     p.tokens = s.tokens;
-    p.chunk = s.chunk;
-    p.chunks = s.chunks;
+    p.most = s.tokens * s.part;
+    p.workers = s.workers;
+    p.merged = s.merged;
     p.scale = scale;
-    p.part_o = (float *)workspace;
-    p.part_ml = p.part_o ? p.part_o + (size_t)rows * heads * s.chunks * width : nullptr;
-    return width == 64    ? launch_attend<64>(p, (uint32_t)items, stream)
-           : width == 128 ? launch_attend<128>(p, (uint32_t)items, stream)
-                          : launch_attend<256>(p, (uint32_t)items, stream);
+    if (s.merged) {
+        p.part_o = (float *)workspace;
+        p.part_ml = (float *)((uint8_t *)workspace + s.o_bytes);
+        p.places = (uint4 *)((uint8_t *)workspace + s.o_bytes + s.ml_bytes);
+    }
+    return width == 64    ? (ids ? launch_attend<64, true>(p, stream) : launch_attend<64, false>(p, stream))
+           : width == 128 ? (ids ? launch_attend<128, true>(p, stream) : launch_attend<128, false>(p, stream))
+                          : (ids ? launch_attend<256, true>(p, stream) : launch_attend<256, false>(p, stream));
 }
 
 }  // namespace ts

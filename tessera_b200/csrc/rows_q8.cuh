@@ -47,6 +47,7 @@ int unpack_q8(const RowsQ8Dev &kv, const uint32_t *slots, const uint32_t *positi
 // ids NULL: rows [max(0, pos - back), min(pos + 1, keys)) of the slot; else the `count` listed blocks per row and kv head.
 size_t attend_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width, uint32_t back,
                                  uint32_t count, uint32_t block);
+int attend_q8_take_status();
 int attend_q8(const void *q, const RowsQ8Dev &kv, const uint32_t *ids, void *out, const uint32_t *slots,
               const uint32_t *positions, uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,
               uint32_t back, uint32_t count, float scale, void *workspace, size_t workspace_bytes, cudaStream_t stream);

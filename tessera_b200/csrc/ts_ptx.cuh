@@ -185,6 +185,14 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, u
         : "memory");
 }
 
+// The same with shared-memory addresses.
+__device__ __forceinline__ void copy_codes(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t x, int32_t y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int32_t x,
                                             int32_t y, int32_t z) {
     asm volatile(
@@ -434,6 +442,9 @@ int make_tensor_map_2d(CUtensorMap *map, const void *base, uint64_t rows, uint64
 // Same without swizzle: rows of the tile lie back to back in shared memory (box_cols <= 256).
 int make_tensor_map_2d_plain(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint64_t row_stride,
                              uint32_t box_rows, uint32_t box_cols);
+
+// 2-D map of bytes, rows back to back; tiles of box_rows x box_cols bytes (64 or 128) with the swizzle of that width.
+int make_tensor_map_codes(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint32_t box_cols, uint32_t box_rows);
 
 // 3-D: [outer, rows, cols] with element strides; tile 1 x box_rows x box_cols.
 int make_tensor_map_3d(CUtensorMap *map, const void *base, uint64_t outer, uint64_t rows, uint64_t cols,

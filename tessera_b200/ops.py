@@ -7,6 +7,7 @@ with tensors that are not on a CUDA device is refused; there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -236,118 +237,132 @@ def _refuse(message: str):
     raise _lib.TesseraError(_lib.TS_ERR_BAD_INPUT, message)
 
 
-def _q8_call(kv: RowsQ8, kept: Kept, **tensors) -> tuple:
-    """Checks what a call over 8-bit rows is given, name -> (tensor or None, dtype, shape or None), and returns the
-    stream it goes to (the current one of the rows' device) and the addresses in order."""
-    dev = kv.k.device
-    if dev.type != "cuda":
+# A step makes a few of these calls a layer, each a few microseconds of GPU time, so the checks below read every property
+# of a tensor once and build nothing that they do not need.
+
+def _q8_stream(kv: RowsQ8) -> tuple:
+    """(device ordinal, stream): the current stream of the rows' device, which has to be the current device."""
+    dev = kv.k.get_device()
+    if dev < 0:
         _refuse("tensors must live on a CUDA device (there is no CPU path)")
-    if dev.index != torch.cuda.current_device():
-        _refuse(f"the rows are on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+    if dev != torch.cuda.current_device():
+        _refuse(f"the rows are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+    return dev, torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _at(t, dtype, count, dev, name):
+    """The address of a contiguous tensor of `count` elements of `dtype` on device `dev`; None stays None."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.numel() != count or t.get_device() != dev or not t.is_contiguous():
+        _refuse(f"{name}: expected {count} contiguous elements of {dtype} on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _kept_q8(kept: Kept, dev) -> TsKept:
     if kept.table is not None:
-        tensors["page table"] = (kept.table, torch.int32, None)
-    at = []
-    for name, (t, dtype, shape) in tensors.items():
-        if t is None:
-            at.append(None)
-            continue
-        if t.dtype != dtype or t.device != dev or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
-            _refuse(f"{name}: expected contiguous {dtype}{'' if shape is None else ' ' + str(list(shape))} on {dev}, got "
-                    f"{t.dtype} {list(t.shape)} on {t.device}")
-        at.append(t.data_ptr())
-    return _stream(), at
+        _at(kept.table, torch.int32, kept.table.numel(), dev, "page table")
+    return kept.c()
 
 
-def _scratch(nbytes: int, device) -> torch.Tensor | None:
+@functools.lru_cache(maxsize=256)
+def _q8_workspace(which: str, *sizes) -> int:
+    return getattr(lib, which)(*sizes)
+
+
+def _scratch(nbytes: int, like) -> torch.Tensor | None:
     """Scratch of one call, from the caching allocator: eager calls reuse it in stream order, a captured call keeps its
     own in the graph's pool, so that two graphs never share it."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
 def qk_norm_rope_append_q8(qkv, q_norm, k_norm, inv_freq, slots, positions, kv: RowsQ8, kept: Kept, heads: int, *, eps: float,
                            out=None):
     """Per-head norm (gains f32 [width] or None) and rotation, q out in bf16 [rows, heads, width], k and v into their
     blocks: ts_qk_norm_rope_append_q8.  Rows that fall into the same block stand next to one another."""
-    rows = qkv.shape[0]
+    dev, stream = _q8_stream(kv)
+    rows = slots.numel()
     _, kv_heads, _, width = kv.k.shape
     if out is None:
         out = torch.empty((rows, heads, width), dtype=torch.bfloat16, device=qkv.device)
-    stream, (a_qkv, a_qn, a_kn, a_freq, a_slots, a_pos, a_out, *_) = _q8_call(
-        kv, kept, qkv=(qkv, torch.bfloat16, (rows, (heads + 2 * kv_heads) * width)), q_norm=(q_norm, torch.float32, (width,)),
-        k_norm=(k_norm, torch.float32, (width,)), inv_freq=(inv_freq, torch.float32, (width // 2,)),
-        slots=(slots, torch.int32, (rows,)), positions=(positions, torch.int32, (rows,)),
-        out=(out, torch.bfloat16, (rows, heads, width)))
+    args = (_at(qkv, torch.bfloat16, rows * (heads + 2 * kv_heads) * width, dev, "qkv"), _at(q_norm, torch.float32, width, dev, "q_norm"),
+            _at(k_norm, torch.float32, width, dev, "k_norm"), _at(inv_freq, torch.float32, width // 2, dev, "inv_freq"),
+            _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions"),
+            _at(out, torch.bfloat16, rows * heads * width, dev, "out"))
     if rows:
-        check(lib.ts_qk_norm_rope_append_q8(a_qkv, a_qn, a_kn, a_freq, a_slots, a_pos, a_out, kv.c(), kept.c(), rows, heads,
-                                            kv_heads, width, eps, stream))
+        check(lib.ts_qk_norm_rope_append_q8(*args, kv.c(), _kept_q8(kept, dev), rows, heads, kv_heads, width, eps, stream))
     return out
 
 
 def rows_unpack_q8(kv: RowsQ8, slots, positions, kept: Kept):
     """The kept rows at (slots[r], positions[r]) as bf16 [rows, kv_heads, width], keys and values: ts_rows_unpack_q8."""
+    dev, stream = _q8_stream(kv)
     rows = slots.numel()
     _, kv_heads, _, width = kv.k.shape
     k_out = torch.empty((rows, kv_heads, width), dtype=torch.bfloat16, device=kv.k.device)
     v_out = torch.empty_like(k_out)
-    stream, (a_slots, a_pos, *_) = _q8_call(kv, kept, slots=(slots, torch.int32, (rows,)), positions=(positions, torch.int32, (rows,)))
+    args = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
     if rows:
-        check(lib.ts_rows_unpack_q8(kv.c(), a_slots, a_pos, k_out.data_ptr(), v_out.data_ptr(), kept.c(), rows, kv_heads, width,
+        check(lib.ts_rows_unpack_q8(kv.c(), *args, k_out.data_ptr(), v_out.data_ptr(), _kept_q8(kept, dev), rows, kv_heads, width,
                                     stream))
     return k_out, v_out
 
 
 def _heads_of(q, kv: RowsQ8) -> tuple:
     _, kv_heads, block, width = kv.k.shape
-    if q.dim() != 3 or q.shape[2] != width or q.shape[1] % kv_heads:
-        _refuse(f"q {list(q.shape)} does not go with {kv_heads} kv heads of width {width}")
-    return q.shape[0], q.shape[1], kv_heads, block, width
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != width or shape[1] % kv_heads:
+        _refuse(f"q {list(shape)} does not go with {kv_heads} kv heads of width {width}")
+    return shape[0], shape[1], kv_heads, block, width
 
 
 def attend_rows_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, *, scale: float, back=0xFFFFFFFF, out=None):
     """Ragged causal attention over 8-bit kept rows, q and result bf16 [rows, heads, width]: ts_attend_rows_q8."""
+    dev, stream = _q8_stream(kv)
     rows, heads, kv_heads, _, width = _heads_of(q, kv)
     if out is None:
         out = torch.empty_like(q)
-    stream, (a_q, a_slots, a_pos, a_out, *_) = _q8_call(
-        kv, kept, q=(q, torch.bfloat16, None), slots=(slots, torch.int32, (rows,)), positions=(positions, torch.int32, (rows,)),
-        out=(out, torch.bfloat16, (rows, heads, width)))
-    nbytes = lib.ts_attend_rows_q8_workspace_bytes(rows, keys, heads, kv_heads, width, back)
-    ws = _scratch(nbytes, q.device)
+    a_q, a_out = (_at(t, torch.bfloat16, rows * heads * width, dev, n) for t, n in ((q, "q"), (out, "out")))
+    a_slots, a_pos = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
+    nbytes = _q8_workspace("ts_attend_rows_q8_workspace_bytes", rows, keys, heads, kv_heads, width, back)
+    ws = _scratch(nbytes, q)
     if rows:
-        check(lib.ts_attend_rows_q8(a_q, kv.c(), a_out, a_slots, a_pos, kept.c(), rows, keys, heads, kv_heads, width, back, scale,
-                                    ws.data_ptr() if nbytes else None, nbytes, stream))
+        check(lib.ts_attend_rows_q8(a_q, kv.c(), a_out, a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads, width, back,
+                                    scale, ws.data_ptr() if nbytes else None, nbytes, stream))
     return out
 
 
 def select_blocks_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, count: int, *, first: int = 1, recent: int = 1):
     """The `count` blocks of positions each row and kv head should read, ascending, int32 [rows, kv_heads, count] with -1
     (UINT32_MAX) in spare entries: ts_select_blocks_q8."""
+    dev, stream = _q8_stream(kv)
     rows, heads, kv_heads, block, width = _heads_of(q, kv)
-    stream, (a_q, a_slots, a_pos, *_) = _q8_call(
-        kv, kept, q=(q, torch.bfloat16, None), slots=(slots, torch.int32, (rows,)), positions=(positions, torch.int32, (rows,)))
+    a_q = _at(q, torch.bfloat16, rows * heads * width, dev, "q")
+    a_slots, a_pos = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
     ids = torch.empty((rows, kv_heads, max(count, 0)), dtype=torch.int32, device=q.device)
-    nbytes = lib.ts_select_blocks_q8_workspace_bytes(rows, keys, kv_heads, block, count)
-    ws = _scratch(nbytes, q.device)
+    nbytes = _q8_workspace("ts_select_blocks_q8_workspace_bytes", rows, keys, kv_heads, block, max(count, 0))
+    ws = _scratch(nbytes, q)
     if rows:
-        check(lib.ts_select_blocks_q8(a_q, kv.c(), ids.data_ptr(), a_slots, a_pos, kept.c(), rows, keys, heads, kv_heads, width,
-                                      count, first, recent, ws.data_ptr() if nbytes else None, nbytes, stream))
+        check(lib.ts_select_blocks_q8(a_q, kv.c(), ids.data_ptr(), a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads,
+                                      width, max(count, 0), first, recent, ws.data_ptr() if nbytes else None, nbytes, stream))
     return ids
 
 
 def attend_blocks_q8(q, kv: RowsQ8, ids, slots, positions, kept: Kept, keys: int, *, scale: float, out=None):
     """Causal attention over the listed blocks only (ids int32 [rows, kv_heads, count], -1 = none): ts_attend_blocks_q8."""
+    dev, stream = _q8_stream(kv)
     rows, heads, kv_heads, block, width = _heads_of(q, kv)
     count = ids.shape[-1]
     if out is None:
         out = torch.empty_like(q)
-    stream, (a_q, a_ids, a_slots, a_pos, a_out, *_) = _q8_call(
-        kv, kept, q=(q, torch.bfloat16, None), ids=(ids, torch.int32, (rows, kv_heads, count)), slots=(slots, torch.int32, (rows,)),
-        positions=(positions, torch.int32, (rows,)), out=(out, torch.bfloat16, (rows, heads, width)))
-    nbytes = lib.ts_attend_blocks_q8_workspace_bytes(rows, count, heads, kv_heads, width, block)
-    ws = _scratch(nbytes, q.device)
+    a_q, a_out = (_at(t, torch.bfloat16, rows * heads * width, dev, n) for t, n in ((q, "q"), (out, "out")))
+    a_ids = _at(ids, torch.int32, rows * kv_heads * count, dev, "ids")
+    a_slots, a_pos = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
+    nbytes = _q8_workspace("ts_attend_blocks_q8_workspace_bytes", rows, count, heads, kv_heads, width, block)
+    ws = _scratch(nbytes, q)
     if rows:
-        check(lib.ts_attend_blocks_q8(a_q, kv.c(), a_ids, a_out, a_slots, a_pos, kept.c(), rows, keys, heads, kv_heads, width,
-                                      count, scale, ws.data_ptr() if nbytes else None, nbytes, stream))
+        check(lib.ts_attend_blocks_q8(a_q, kv.c(), a_ids, a_out, a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads,
+                                      width, count, scale, ws.data_ptr() if nbytes else None, nbytes, stream))
     return out
 
 
