@@ -1,14 +1,19 @@
 // Ragged attention over kept rows in 8 bits, whole slots or listed blocks.
 //
 // A tile is up to 16 query rows, (token, head) pairs: the G heads of a kv head's group times up to T = 16 / G neighbouring
-// rows that are the next positions of one slot (drafted tokens, a part of a prompt).  Both products run on warp MMAs
-// (m16n8k16, f16 in, f32 out) with the keys, then the channels, as the 16 rows and the queries as the 8 columns:
-//     S^T[16 keys x 8 queries] = K Q^T,      O^T[16 channels x 8 queries] += V^T P^T
+// rows that are the next positions of one slot (drafted tokens, a part of a prompt).  Both products run on warp MMAs with
+// the keys, then the channels, as the 16 rows and the queries as the 8 columns:
+//     S^T[16 keys x 8 queries] = K Q^T        m16n8k32, s8 in, s32 out
+//     O^T[16 channels x 8 queries] += V^T P^T m16n8k16, f16 in, f32 out
 // so that a decode row of up to eight heads wastes nothing of the accumulators, and a second eight of queries shares the
-// converted K and V.  (With the queries as rows, half of every accumulator quad of a decode row is padding: 64 more
-// registers and twice the MMAs.)  A code is exact in f16: the bytes are set as the low bits of 1024 + (128 + code) and 1152
-// is subtracted; a query row is brought into f16's range by a power of two, which is exact for bf16 (values below 2^-24
-// of the row's largest lose digits that no sum would keep).
+// loaded K and the converted V.  (With the queries as rows, half of every accumulator quad of a decode row is padding.)
+//
+// K goes into its product as it lies, without a conversion: a query row becomes whole numbers of 15 bits and a sign,
+// Q = round(q * 32639 / max |q|), in two signed digits Q = 256 q1 + q0, each a product of its own; the sums are exact in 32
+// bits (256 * 32639 * 127 < 2^31) and rounded once.  What this costs is the rounding of q to 2^-16 of the row's largest,
+// below what the probabilities' f16 costs; what it saves is half of all instructions (two conversions for every pair of
+// codes).  V's codes become f16, which holds them exactly: the bytes are set as the low bits of 1024 + (128 + code) and
+// 1152 is subtracted.
 //
 // The scales leave the products alone.  With s = raw * scale * k_scale in powers of two and
 //     x = s + log2(v_scale),   M = max x,   P = 2^(x - M)  <= 1   (f16 operand of P V)
@@ -26,7 +31,7 @@
 // may be as uneven as they like.  A run has at most one tile that began before it and one that goes on after it, so a
 // worker leaves at most two partial results (M, sum, output) in the workspace; tiles that lie within a run go straight
 // to the output.  A second kernel folds the partials of a tile in the order of their keys: no atomics, the same bits on
-// every run.  With little work every tile is cut into pieces of four steps instead.
+// every run.
 #include <cmath>
 
 #include "rows_q8.cuh"
@@ -37,16 +42,14 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kHalfStage = 4096, kStage = 2 * kHalfStage;  // K codes, then V codes
-constexpr int kPiece = 4;                                  // steps of a worker's run at least
+__device__ constexpr uint32_t kRuns[6] = {1, 2, 3, 4, 6, 8};
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kScaleFloor = 8.673617379884035e-19f;  // 2^-60
 
-// Blocks an SM holds and stages a warp has.  Twelve warps keep the issue slots busy where registers allow it (width
-// 256 needs up to 255 of them).
-template <int W>
-struct Shape {
-    static constexpr int CTAS = W == 256 ? 2 : 3, STAGES = W == 256 ? 3 : 2;
-};
+// Eight warps with three stages each fill an SM's shared memory (two blocks of 96 KB).  Twelve warps with two stages were
+// slower everywhere (64 rows x 8192 positions: 156 us against 145): they leave 168 registers a thread, which spills, and
+// a second tile behind every wait.  Six warps with four stages: 149.
+constexpr int kBlocks = 2, kStages = 3;
 
 struct AttendParams {
     const uint16_t *q;
@@ -108,7 +111,12 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(v) : "r"(a));
     return v;
 }
-// Two of the four biased codes (code + 128) as f16: bytes 0, 1 (0x4140), 2, 3 (0x4342), 0, 2 (0x4240) or 1, 3 (0x4341).
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// Two of the four biased codes (code + 128) as f16: bytes 0, 2 (0x4240) or 1, 3 (0x4341).
 __device__ __forceinline__ uint32_t codes_f16(uint32_t biased, uint32_t sel) {
     return sub_f16x2(__byte_perm(biased, 0x64646464u, sel), 0x64806480u);  // 1152 = 0x6480
 }
@@ -133,76 +141,141 @@ __device__ __forceinline__ void seen(const AttendParams &p, uint32_t pos, uint32
     *hi = pos < p.keys ? pos + 1 : p.keys;
 }
 
-// The tile that begins at `row`; false if the row lies in a tile that begins before it.
+// Consecutive rows, one a lane, and the tiles that begin at them.  A lane whose row lies in a tile that begins before it
+// has steps = 0.  `width` rows are looked at together, a multiple of the rows a tile may hold, so that no tile lies
+// across: tiles begin at multiples of `tokens` and where a row is not the next position of the slot before it (or the
+// same again).
+struct RowGroup {
+    uint32_t slot, tokens, from, to, steps;
+};
+
+__device__ __forceinline__ uint32_t rows_together(const AttendParams &p) { return 32 - 32 % p.tokens; }
+
+struct RawRow {
+    uint32_t slot, pos;
+};
+
+__device__ __forceinline__ RawRow row_at(const AttendParams &p, uint32_t first, uint32_t lane) {
+    RawRow raw = {0, 0};
+    if (lane < rows_together(p) && first + lane < p.rows) raw = {p.slots[first + lane], p.positions[first + lane]};
+    return raw;
+}
+
 template <int W, bool LIST>
-__device__ __forceinline__ bool tile_of(const AttendParams &p, uint32_t row, Tile *t) {
-    t->row = row;
-    t->tokens = 1;
-    t->slot = p.slots[row];
+__device__ __forceinline__ RowGroup rows_from(const AttendParams &p, const RawRow &raw, uint32_t first, uint32_t lane) {
+    RowGroup g = {raw.slot, 1, 0, 0, 0};
+    const uint32_t row = first + lane, pos = raw.pos;
+    const bool here = lane < rows_together(p) && row < p.rows;
+    uint32_t last = pos;
+    bool begins = here;
     if (!LIST && p.tokens > 1) {
-        // Tiles begin at multiples of `tokens` and where a row is not the next position of the slot before it (or the same
-        // again).
-        auto follows = [&](uint32_t r) {
-            if (r % p.tokens == 0 || p.slots[r] != p.slots[r - 1]) return false;  // also: row 0 has none before it
-            const uint32_t was = p.positions[r - 1], is = p.positions[r];
-            return is >= was && is - was <= 1u;
-        };
-        if (follows(row)) return false;
-        while (row + t->tokens < p.rows && follows(row + t->tokens)) t->tokens++;
+        const uint32_t slot0 = __shfl_up_sync(0xFFFFFFFFu, g.slot, 1), pos0 = __shfl_up_sync(0xFFFFFFFFu, pos, 1);
+        const bool follows = here && row % p.tokens != 0 && g.slot == slot0 && pos >= pos0 && pos - pos0 <= 1u;
+        const uint32_t mask = __ballot_sync(0xFFFFFFFFu, follows);
+        begins = here && !follows;
+        g.tokens = lane == 31 ? 1 : __ffs(~(mask >> (lane + 1)));  // this row and those that follow without a break
+        last = __shfl_sync(0xFFFFFFFFu, pos, min(lane + g.tokens - 1, 31u));
     }
-    // positions ascend within a tile: the first row sees the earliest key, the last one the latest
-    uint32_t a, b;
-    seen(p, p.positions[row], &t->from, &b);
-    seen(p, p.positions[row + t->tokens - 1], &a, &t->to);
-    if (t->from >= t->to) t->from = t->to = 0;
-    if (LIST) {
-        t->base = 0;
-        t->entries = p.count;
-        t->steps = ((p.count << (p.kv.shift - 4)) + Step<W>::UNITS - 1) / Step<W>::UNITS;
-    } else {
-        t->base = t->from >> p.kv.shift;
-        t->entries = t->from < t->to ? ((t->to - 1) >> p.kv.shift) + 1 - t->base : 0;
-        t->steps = t->from < t->to ? (t->to - 1 - (t->base << p.kv.shift)) / Step<W>::KEYS + 1 : 1;
+    // positions ascend within a tile: its first row sees the earliest key, its last one the latest
+    uint32_t x;
+    seen(p, pos, &g.from, &x);
+    seen(p, last, &x, &g.to);
+    if (g.from >= g.to) g.from = g.to = 0;
+    if (begins) {
+        if (LIST) g.steps = ((p.count << (p.kv.shift - 4)) + Step<W>::UNITS - 1) / Step<W>::UNITS;
+        else g.steps = g.from < g.to ? (g.to - 1 - (g.from >> p.kv.shift << p.kv.shift)) / Step<W>::KEYS + 1 : 1;
     }
-    return true;
+    return g;
+}
+
+template <bool LIST>
+__device__ __forceinline__ Tile tile_at(const AttendParams &p, const RowGroup &g, uint32_t first, uint32_t l) {
+    Tile t;
+    t.row = first + l;
+    t.tokens = __shfl_sync(0xFFFFFFFFu, g.tokens, l);
+    t.slot = __shfl_sync(0xFFFFFFFFu, g.slot, l);
+    t.from = __shfl_sync(0xFFFFFFFFu, g.from, l);
+    t.to = __shfl_sync(0xFFFFFFFFu, g.to, l);
+    t.steps = __shfl_sync(0xFFFFFFFFu, g.steps, l);
+    t.base = LIST ? 0 : t.from >> p.kv.shift;
+    t.entries = LIST ? p.count : t.from < t.to ? ((t.to - 1) >> p.kv.shift) + 1 - t.base : 0;
+    return t;
 }
 
 __device__ __forceinline__ uint32_t warp_total(uint32_t v) { return __reduce_add_sync(0xFFFFFFFFu, v); }
 
 // ---- the query operand: column r of eight is tile row 8 t + r; thread j of its four has channels 16 s + 4 j + 0..3 ----
+constexpr float kQueryMost = 32639.0f;  // 127 * 256 + 127
+
 template <int W, int NT>
 struct Queries {
-    uint32_t b[NT][W / 16][2];
-    float f[NT][2];            // raw score -> power-of-two exponent, without the key scale, for columns 2 j, 2 j + 1
+    uint32_t b[NT][W / 32][2][2];   // step of 32 channels; digit 256s, digit ones; channels 0-15 and 16-31 of the step
+    float f[NT][2];                 // raw score -> power-of-two exponent, without the key scale, for columns 2 j, 2 j + 1
     uint32_t lo[NT][2], hi[NT][2];  // keys those columns see
 };
 
+// As they lie in memory, asked for early.
 template <int W, int NT>
-__device__ __forceinline__ void load_queries(const AttendParams &p, const Tile &tile, uint32_t head0, uint32_t part, uint32_t lane,
-                                             Queries<W, NT> &qs) {
-    const uint32_t r = lane >> 2, j = lane & 3;
+struct RawQueries {
+    uint2 v[NT][W / 16];
+};
+
+template <int W, int NT>
+__device__ __forceinline__ RawQueries<W, NT> fetch_queries(const AttendParams &p, const Tile &tile, uint32_t head0, uint32_t part, uint32_t lane) {
+    RawQueries<W, NT> raw;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        const uint32_t m = 8 * t + r, token = m / part, head = m - token * part;
-        uint2 v[W / 16];
-        float most = 0.0f;
+        const uint32_t m = 8 * t + (lane >> 2), token = m / part, head = m - token * part;
+        const uint16_t *q = p.q + ((size_t)(tile.row + token) * p.heads + head0 + head) * W + 4 * (lane & 3);
 #pragma unroll
         for (int s = 0; s < W / 16; s++) {
-            v[s] = make_uint2(0, 0);
-            if (token < tile.tokens) v[s] = *reinterpret_cast<const uint2 *>(p.q + ((size_t)(tile.row + token) * p.heads + head0 + head) * W + 16 * s + 4 * j);
+            raw.v[t][s] = make_uint2(0, 0);
+            if (token < tile.tokens) raw.v[t][s] = *reinterpret_cast<const uint2 *>(q + 16 * s);
+        }
+    }
+    return raw;
+}
+
+template <int W, int NT>
+__device__ __forceinline__ void load_queries(const AttendParams &p, const Tile &tile, const RawQueries<W, NT> &raw, uint32_t part,
+                                             uint32_t lane, Queries<W, NT> &qs) {
+    const uint32_t j = lane & 3;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const uint2 (&v)[W / 16] = raw.v[t];
+        float most = 0.0f, bad = 0.0f;  // bad: NaN once an element is infinite or NaN
+#pragma unroll
+        for (int s = 0; s < W / 16; s++) {
+            const float x[4] = {bf16_lo(v[s].x), bf16_hi(v[s].x), bf16_lo(v[s].y), bf16_hi(v[s].y)};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                most = fmaxf(most, fabsf(x[i]));
+                bad = fmaf(x[i], 0.0f, bad);
+            }
         }
 #pragma unroll
-        for (int s = 0; s < W / 16; s++)
-            most = fmaxf(most, fmaxf(fmaxf(fabsf(bf16_lo(v[s].x)), fabsf(bf16_hi(v[s].x))), fmaxf(fabsf(bf16_lo(v[s].y)), fabsf(bf16_hi(v[s].y)))));
-        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-        uint32_t e = __float_as_uint(most) >> 23;  // the largest magnitude's exponent; 255: infinity
+        for (int o = 1; o < 4; o <<= 1) {
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+            bad += __shfl_xor_sync(0xFFFFFFFFu, bad, o);
+        }
+        // 2^-e first, so that neither the smallest nor the largest magnitudes leave f32 on the way
+        uint32_t e = __float_as_uint(most) >> 23;
         e = e < 1 ? 1 : e > 253 ? 253 : e;
-        const float down = __uint_as_float((254 - e) << 23), f = __uint_as_float(e << 23) * (p.scale * kLog2e);
+        const float down = __uint_as_float((254 - e) << 23), unit = most * down / kQueryMost;
+        const float inv = most > 0.0f ? kQueryMost / (most * down) : 0.0f;
+        const float f = __uint_as_float(e << 23) * unit * (p.scale * kLog2e) + bad;
 #pragma unroll
         for (int s = 0; s < W / 16; s++) {
-            qs.b[t][s][0] = pack_f16(bf16_lo(v[s].x) * down, bf16_hi(v[s].x) * down);
-            qs.b[t][s][1] = pack_f16(bf16_lo(v[s].y) * down, bf16_hi(v[s].y) * down);
+            const float x[4] = {bf16_lo(v[s].x), bf16_hi(v[s].x), bf16_lo(v[s].y), bf16_hi(v[s].y)};
+            uint32_t high = 0, low = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int q = __float2int_rn(x[i] * down * inv), q1 = (q + 128) >> 8;
+                high |= (uint32_t)(q1 & 255) << (8 * i);
+                low |= (uint32_t)((q - (q1 << 8)) & 255) << (8 * i);
+            }
+            qs.b[t][s / 2][0][s % 2] = high;
+            qs.b[t][s / 2][1][s % 2] = low;
         }
 #pragma unroll
         for (int e2 = 0; e2 < 2; e2++) {
@@ -232,31 +305,29 @@ __device__ __forceinline__ uint32_t piece_at(uint32_t tile, int u, int c, uint32
     else return tile + (c >> 3) * (Step<W>::KEYS * 128) + key * 128 + ((((c & 7) + side) ^ (key & 7)) << 4);
 }
 
-// One step.  EDGE: some key of it is not seen by some row.  A unit without keys has key0 past every row's.
+// A step's scores in powers of two with the value scale's exponent.  EDGE: some key of the step is not seen by some row.  A
+// unit without keys has key0 past every row's.
 template <int W, int NT, bool EDGE>
-__device__ __forceinline__ void step(const Queries<W, NT> &qs, Running<W, NT> &run, uint32_t tile, const float (&ks)[Step<W>::UNITS],
-                                     const float (&vs)[Step<W>::UNITS], const uint32_t (&key0)[Step<W>::UNITS], uint32_t lane) {
+__device__ __forceinline__ void score_step(const Queries<W, NT> &qs, uint32_t tile, const float (&ks)[Step<W>::UNITS],
+                                           const float (&vs)[Step<W>::UNITS], const uint32_t (&key0)[Step<W>::UNITS],
+                                           float (&x)[Step<W>::UNITS][NT][4], uint32_t lane) {
     constexpr int U = Step<W>::UNITS;
     const uint32_t r = lane >> 2;
-    float x[U][NT][4], most[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; t++) most[t][0] = most[t][1] = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; u++) {
+        int high[NT][4], low[NT][4];
 #pragma unroll
-        for (int t = 0; t < NT; t++) x[u][t][0] = x[u][t][1] = x[u][t][2] = x[u][t][3] = 0.0f;
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) high[t][i] = low[t][i] = 0;
 #pragma unroll
         for (int c = 0; c < W / 16; c += 2) {
-            uint32_t w[4];
-            ldsm_x4(piece_at<W>(tile, u, c, lane), w);
+            uint32_t a[4];
+            ldsm_x4(piece_at<W>(tile, u, c, lane), a);
 #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] ^= 0x80808080u;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint32_t a0 = codes_f16(w[2 * i], 0x4140), a1 = codes_f16(w[2 * i + 1], 0x4140), a2 = codes_f16(w[2 * i], 0x4342),
-                               a3 = codes_f16(w[2 * i + 1], 0x4342);
-#pragma unroll
-                for (int t = 0; t < NT; t++) mma_f16(x[u][t], a0, a1, a2, a3, qs.b[t][c + i]);
+            for (int t = 0; t < NT; t++) {
+                mma_s8(high[t], a, qs.b[t][c / 2][0]);
+                mma_s8(low[t], a, qs.b[t][c / 2][1]);
             }
         }
         const float lv = log2_approx(fmaxf(vs[u], kScaleFloor));
@@ -267,25 +338,35 @@ __device__ __forceinline__ void step(const Queries<W, NT> &qs, Running<W, NT> &r
                 const float f = qs.f[t][e] * ks[u];
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    float &y = x[u][t][2 * k + e];
-                    y = fmaf(y, f, lv);
+                    float y = fmaf(__int2float_rn(high[t][2 * k + e] * 256 + low[t][2 * k + e]), f, lv);
                     if (EDGE) {
                         const uint32_t key = key0[u] + 8 * k + r;
                         if (key < qs.lo[t][e] || key >= qs.hi[t][e]) y = -INFINITY;
                     }
-                    most[t][e] = fmaxf(most[t][e], y);
+                    x[u][t][2 * k + e] = y;
                 }
             }
     }
+}
+
+// The running maximum and sum over a step's scores, the output brought to the new maximum; b: the probabilities as the
+// second product's operand.
+template <int W, int NT>
+__device__ __forceinline__ void soften(Running<W, NT> &run, const float (&x)[Step<W>::UNITS][NT][4], const float (&vs)[Step<W>::UNITS],
+                                       uint32_t (&b)[Step<W>::UNITS][NT][2]) {
+    constexpr int U = Step<W>::UNITS;
     float scale[NT][2], top[NT][2];
     bool same = true;
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
+            float most = -INFINITY;
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) most[t][e] = fmaxf(most[t][e], __shfl_xor_sync(0xFFFFFFFFu, most[t][e], o));
-            const float now = fmaxf(run.m[t][e], most[t][e]);
+            for (int u = 0; u < U; u++) most = fmaxf(most, fmaxf(x[u][t][e], x[u][t][2 + e]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+            const float now = fmaxf(run.m[t][e], most);
             top[t][e] = now == -INFINITY ? 0.0f : now;  // nothing seen yet: 2^(-inf - 0) = 0
             scale[t][e] = exp2_approx(run.m[t][e] - top[t][e]);
             same = same && scale[t][e] == 1.0f;
@@ -306,7 +387,6 @@ __device__ __forceinline__ void step(const Queries<W, NT> &qs, Running<W, NT> &r
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const float inv = __fdividef(1.0f, fmaxf(vs[u], kScaleFloor));
-        uint32_t b[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             float p[4];
@@ -316,13 +396,20 @@ __device__ __forceinline__ void step(const Queries<W, NT> &qs, Running<W, NT> &r
                 p[2 + e] = exp2_approx(x[u][t][2 + e] - top[t][e]);
                 run.l[t][e] = fmaf(p[e] + p[2 + e], inv, run.l[t][e]);
             }
-            b[t][0] = transpose_8x8(pack_f16(p[0], p[1]));
-            b[t][1] = transpose_8x8(pack_f16(p[2], p[3]));
+            b[u][t][0] = transpose_8x8(pack_f16(p[0], p[1]));
+            b[u][t][1] = transpose_8x8(pack_f16(p[2], p[3]));
         }
+    }
+}
+
+template <int W, int NT>
+__device__ __forceinline__ void value_step(Running<W, NT> &run, uint32_t tile, const uint32_t (&b)[Step<W>::UNITS][NT][2], uint32_t lane) {
+#pragma unroll
+    for (int u = 0; u < Step<W>::UNITS; u++)
 #pragma unroll
         for (int c = 0; c < W / 16; c += 2) {
             uint32_t w[4];
-            ldsm_x4_trans(piece_at<W>(tile + kHalfStage, u, c, lane), w);
+            ldsm_x4_trans(piece_at<W>(tile, u, c, lane), w);
 #pragma unroll
             for (int i = 0; i < 4; i++) w[i] ^= 0x80808080u;
 #pragma unroll
@@ -330,10 +417,9 @@ __device__ __forceinline__ void step(const Queries<W, NT> &qs, Running<W, NT> &r
                 const uint32_t a0 = codes_f16(w[2 * i], 0x4240), a1 = codes_f16(w[2 * i], 0x4341), a2 = codes_f16(w[2 * i + 1], 0x4240),
                                a3 = codes_f16(w[2 * i + 1], 0x4341);
 #pragma unroll
-                for (int t = 0; t < NT; t++) mma_f16(run.o[c + i][t], a0, a1, a2, a3, b[t]);
+                for (int t = 0; t < NT; t++) mma_f16(run.o[c + i][t], a0, a1, a2, a3, b[u][t]);
             }
         }
-    }
 }
 
 // 32 blocks' places in the pool and scales, one a lane: entry `first` + lane of the tile's blocks.
@@ -358,10 +444,11 @@ __device__ __forceinline__ Group group_of(const AttendParams &p, const Tile &t, 
     return g;
 }
 
-// A warp's ring: the next stage to complete and the parity each completes with.
+// A warp's ring: the next stage to complete and the parity each completes with.  K and V of a stage complete, and are
+// asked for again, each by itself: while one is computed on, the other and the other stages are under way.
 struct Ring {
     uint32_t tiles;  // shared-memory address
-    uint64_t *full;
+    uint64_t *full;  // K of every stage, then V of every stage
     uint32_t stage, parity;
     bool ok;  // false: a wait ran out, nothing is copied or computed any more
 };
@@ -377,7 +464,7 @@ __device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtens
                                              uint32_t kvh, uint32_t head0, uint32_t part, uint32_t begin, uint32_t end, Target to,
                                              Ring &ring, int *status, uint32_t lane) {
     using namespace ptx;
-    constexpr int KEYS = Step<W>::KEYS, U = Step<W>::UNITS, HALVES = Step<W>::HALVES, COLS = Step<W>::COLS, STAGES = Shape<W>::STAGES;
+    constexpr int KEYS = Step<W>::KEYS, U = Step<W>::UNITS, HALVES = Step<W>::HALVES, COLS = Step<W>::COLS, STAGES = kStages;
     const uint32_t in_block = p.kv.shift - 4;  // log2 of a block's 16-key units
     Running<W, NT> run;
 #pragma unroll
@@ -389,38 +476,48 @@ __device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtens
     }
     if (tile.from < tile.to) {
         uint32_t first = (begin * U) >> in_block;  // entry of lane 0 of the current group
+        const RawQueries<W, NT> raw = fetch_queries<W, NT>(p, tile, head0, part, lane);
         Group now = group_of<LIST>(p, tile, kvh, first, lane);
-        Group next = group_of<LIST>(p, tile, kvh, first + 32, lane);
-        // Copies of step s into stage `at`; the current or the next group has its blocks.
-        auto copy = [&](uint32_t s, uint32_t at) {
-            const uint32_t dst = ring.tiles + at * kStage, bar = smem_addr(&ring.full[at]);
-            uint32_t blk[U], bytes = 0;
-            const uint32_t per = 1u << in_block, span = per < (uint32_t)U ? per : U;  // units of one copy
+        Group next = now;  // the first copies lie in the current group
+        const uint32_t per = 1u << in_block, span = per < (uint32_t)U ? per : U;  // units of one copy
+        // Where step s's units lie in the pool; the current or the next group has its blocks.
+        auto find = [&](uint32_t s, uint32_t (&blk)[U]) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const uint32_t e = ((s * U + u) >> in_block) - first;
                 const uint32_t a = __shfl_sync(0xFFFFFFFFu, now.blk, e & 31), b = __shfl_sync(0xFFFFFFFFu, next.blk, e & 31);
                 blk[u] = e < 32 ? a : b;
-                if ((u & (span - 1)) == 0 && blk[u] != kNoBlock) bytes += span * 16 * W * 2;
             }
+        };
+        // Copies of step s's K (values = 0) or V (1) into stage `at`.
+        auto copy = [&](uint32_t s, uint32_t at, const uint32_t (&blk)[U], const CUtensorMap *map, int values) {
             if (lane == 0) {
-                mbar_expect_tx(&ring.full[at], bytes);
+                uint64_t *bar = &ring.full[values * STAGES + at];
+                const uint32_t dst = ring.tiles + at * kStage + values * kHalfStage;
+                uint32_t bytes = 0;
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if ((u & (span - 1)) == 0 && blk[u] != kNoBlock) bytes += span * 16 * W;
+                mbar_expect_tx(bar, bytes);
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     if ((u & (span - 1)) != 0 || blk[u] == kNoBlock) continue;
                     const int32_t y = (int32_t)(((blk[u] * p.kv_heads + kvh) << p.kv.shift) + (((s * U + u) & (per - 1)) << 4));
 #pragma unroll
-                    for (int h = 0; h < HALVES; h++) {
-                        copy_codes(dst + (h * KEYS + 16 * u) * COLS, map_k, bar, h * COLS, y);
-                        copy_codes(dst + kHalfStage + (h * KEYS + 16 * u) * COLS, map_v, bar, h * COLS, y);
-                    }
+                    for (int h = 0; h < HALVES; h++) copy_codes(dst + (h * KEYS + 16 * u) * COLS, map, smem_addr(bar), h * COLS, y);
                 }
             }
         };
-        uint32_t ahead = begin;
-        for (; ahead < end && ahead < begin + STAGES; ahead++) copy(ahead, (ring.stage + (ahead - begin)) % STAGES);
+        uint32_t ahead = begin, blk[U];  // the next step to ask for, and where it lies
+        for (; ahead < end && ahead < begin + STAGES; ahead++) {
+            const uint32_t at = (ring.stage + (ahead - begin)) % STAGES;
+            find(ahead, blk);
+            copy(ahead, at, blk, map_k, 0);
+            copy(ahead, at, blk, map_v, 1);
+        }
+        next = group_of<LIST>(p, tile, kvh, first + 32, lane);
         Queries<W, NT> qs;
-        load_queries<W, NT>(p, tile, head0, part, lane, qs);
+        load_queries<W, NT>(p, tile, raw, part, lane, qs);
         uint32_t all_lo = 0, all_hi = 0;  // keys that every row of the tile sees
         {
             uint32_t x;
@@ -445,23 +542,43 @@ __device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtens
                 key0[u] = blk == kNoBlock ? 0xFFFFFFF0u : (id << p.kv.shift) + ((unit & ((1u << in_block) - 1)) << 4);
                 edge = edge || key0[u] < all_lo || key0[u] + 16 > all_hi || blk == kNoBlock;
             }
-            ring.ok = mbar_wait(&ring.full[ring.stage], ring.parity >> ring.stage & 1);
+            const uint32_t at = ring.tiles + ring.stage * kStage, odd = ring.parity >> ring.stage & 1;
             ring.parity ^= 1u << ring.stage;
-            if (!__all_sync(0xFFFFFFFFu, ring.ok)) {
-                ring.ok = false;  // the other copies are waited for, as long, before the block may end
+            // A wait that runs out ends the warp's work once the copies still under way have been waited for, as long:
+            // V of this step and both of the steps from s + 1 up to `ahead`.
+            auto give_up = [&](bool k_too) {
+                ring.ok = false;
+                if (!k_too) mbar_wait(&ring.full[STAGES + ring.stage], odd);
                 for (uint32_t i = s + 1; i < ahead; i++) {
-                    ring.stage = (ring.stage + 1) % STAGES;
-                    mbar_wait(&ring.full[ring.stage], ring.parity >> ring.stage & 1);
+                    const uint32_t stage = (ring.stage + (i - s)) % STAGES;
+                    mbar_wait(&ring.full[stage], ring.parity >> stage & 1);
+                    mbar_wait(&ring.full[STAGES + stage], ring.parity >> stage & 1);
                 }
+                if (k_too && ahead < end) mbar_wait(&ring.full[ring.stage], odd ^ 1);
                 if (lane == 0) atomicExch(status, TS_ERR_TIMEOUT);
+            };
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&ring.full[ring.stage], odd))) {
+                give_up(false);
                 return;
             }
-            const uint32_t at = ring.tiles + ring.stage * kStage;
-            if (edge) step<W, NT, true>(qs, run, at, ks, vs, key0, lane);
-            else step<W, NT, false>(qs, run, at, ks, vs, key0, lane);
+            float x[U][NT][4];
+            if (edge) score_step<W, NT, true>(qs, at, ks, vs, key0, x, lane);
+            else score_step<W, NT, false>(qs, at, ks, vs, key0, x, lane);
             __syncwarp();
             if (ahead < end) {
-                copy(ahead, ring.stage);
+                find(ahead, blk);
+                copy(ahead, ring.stage, blk, map_k, 0);
+            }
+            uint32_t b[U][NT][2];
+            soften<W, NT>(run, x, vs, b);
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&ring.full[STAGES + ring.stage], odd))) {
+                give_up(true);
+                return;
+            }
+            value_step<W, NT>(run, at + kHalfStage, b, lane);
+            __syncwarp();
+            if (ahead < end) {
+                copy(ahead, ring.stage, blk, map_v, 1);
                 ahead++;
             }
             ring.stage = (ring.stage + 1) % STAGES;
@@ -495,128 +612,209 @@ __device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtens
 }
 
 template <int W, bool LIST>
-__global__ void __launch_bounds__(kThreads, Shape<W>::CTAS)
+__global__ void __launch_bounds__(kThreads, kBlocks)
 attend_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttendParams p, int *status) {
     using namespace ptx;
-    constexpr int STAGES = Shape<W>::STAGES;
+    constexpr int STAGES = kStages;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint64_t bars[kWarps][STAGES];
+    __shared__ uint64_t bars[kWarps][2 * STAGES];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t worker = warp * gridDim.x + blockIdx.x;  // few workers spread over the SMs
     Ring ring = {smem_addr(smem) + warp * (STAGES * kStage), bars[warp], 0, 0, true};
     if (lane == 0) {
-        for (int s = 0; s < STAGES; s++) mbar_init(&ring.full[s], 1);
+        for (int s = 0; s < 2 * STAGES; s++) mbar_init(&ring.full[s], 1);
         fence_barrier_init();
+        if (warp == 0) {
+            prefetch_tensormap(&map_k);
+            prefetch_tensormap(&map_v);
+        }
     }
     __syncwarp();
     pdl_wait();
     if (worker < p.workers) {
         // ---- the steps of all tiles, and this worker's run of them ----
-        const uint32_t per_row = p.kv_heads * p.parts;
-        auto steps_of = [&](uint32_t row) {
-            Tile t;
-            return row < p.rows && tile_of<W, LIST>(p, row, &t) ? t.steps : 0u;
-        };
-        uint64_t steps = 0, pieces = 0;
+        const uint32_t per_row = p.kv_heads * p.parts, width = rows_together(p);
+        uint32_t first = 0, total = 0;
+        // Pieces if every tile is cut by itself into pieces of 1, 2, 3, 4, 6 or 8 steps.
+        uint32_t pieces[6] = {};
+        RawRow raw = row_at(p, 0, lane);
+        RowGroup rows;
         if (LIST) {
-            const uint32_t n = steps_of(0);
-            steps = (uint64_t)n * p.rows;
-            pieces = (uint64_t)((n + kPiece - 1) / kPiece) * p.rows;
+            rows = rows_from<W, LIST>(p, raw, 0, lane);
+            total = __shfl_sync(0xFFFFFFFFu, rows.steps, 0);
+#pragma unroll
+            for (int i = 0; i < 6; i++) pieces[i] = (total + kRuns[i] - 1) / kRuns[i] * p.rows;
+            total *= p.rows;
         } else {
-            for (uint32_t base = 0; base < p.rows; base += 32) {
-                const uint32_t n = steps_of(base + lane);
-                steps += warp_total(n);
-                pieces += warp_total((n + kPiece - 1) / kPiece);
+            for (uint32_t f = 0; f < p.rows; f += width) {
+                const RawRow next = row_at(p, f + width, lane);  // on its way during the sums
+                const RowGroup g = rows_from<W, LIST>(p, raw, f, lane);
+                total += warp_total(g.steps);
+#pragma unroll
+                for (int i = 1; i < 6; i++) pieces[i] += warp_total((g.steps + kRuns[i] - 1) / kRuns[i]);
+                if (f == 0) rows = g;
+                raw = next;
             }
+            pieces[0] = total;
         }
-        const bool padded = pieces * per_row <= p.workers;  // every tile in pieces of its own
-        const uint64_t total = (padded ? pieces * kPiece : steps) * per_row;
-        const uint32_t run = padded ? kPiece : (uint32_t)((total + p.workers - 1) / p.workers);
-        uint64_t at = (uint64_t)worker * run;
-        const uint64_t end = at + run < total ? at + run : total;
-        // the row in whose steps the run begins
-        uint64_t before = 0;  // steps of earlier rows, all kv heads
-        uint32_t row = 0;
+        total *= per_row;
+        // A worker's run: an equal share of the steps laid end to end, or, where that is eight steps at most, the shortest
+        // piece for which there are workers enough (a run that ends one tile and begins the next pays for two starts).
+        uint32_t run = max(1u, (total + p.workers - 1) / p.workers), by = 1;  // by: tiles take multiples of it
+        if (run <= 8) {
+#pragma unroll
+            for (int i = 5; i >= 0; i--)
+                if (pieces[i] * per_row <= p.workers) by = run = kRuns[i];
+        }
+        auto taken = [&](uint32_t steps) { return (steps + by - 1) / by * by; };
+        if (by > 1) {
+#pragma unroll
+            for (int i = 1; i < 6; i++)
+                if (by == kRuns[i]) total = pieces[i] * kRuns[i] * per_row;
+        }
+        uint32_t at = worker * run;
+        const uint32_t end = min(total, at + run);
         if (at < end) {
-            auto taken = [&](uint32_t n) { return (uint64_t)(padded ? (n + kPiece - 1) / kPiece * kPiece : n) * per_row; };
+            uint32_t before = 0, l = 0;  // steps of earlier rows, all kv heads; the lane whose row holds `at`
             if (LIST) {
-                const uint64_t each = taken(steps_of(0));
-                row = (uint32_t)(at / each);
+                const uint32_t each = total / p.rows, row = at / each;
                 before = row * each;
+                first = row;
+                rows = rows_from<W, LIST>(p, row_at(p, first, lane), first, lane);
             } else {
-                for (uint32_t base = 0; base < p.rows; base += 32) {
-                    const uint32_t n = steps_of(base + lane);
-                    uint64_t mine = taken(n), sum = mine;
+                for (;;) {
+                    uint32_t sum = taken(rows.steps) * per_row;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
-                        const uint64_t other = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+                        const uint32_t other = __shfl_up_sync(0xFFFFFFFFu, sum, o);
                         if (lane >= (uint32_t)o) sum += other;
                     }
                     const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + sum > at);
                     if (hit) {
-                        const int l = __ffs(hit) - 1;
-                        row = base + l;
-                        before += __shfl_sync(0xFFFFFFFFu, sum - mine, l);
+                        l = __ffs(hit) - 1;
+                        before += __shfl_sync(0xFFFFFFFFu, sum - taken(rows.steps) * per_row, l);
                         break;
                     }
                     before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+                    first += width;
+                    if (first >= p.rows) return;  // not reached: at < total
+                    rows = rows_from<W, LIST>(p, row_at(p, first, lane), first, lane);
                 }
             }
             bool begun = false;  // whether the run has had a tile already
-            while (at < end && row < p.rows && ring.ok) {
-                Tile tile;
-                if (!tile_of<W, LIST>(p, row, &tile)) {
-                    row++;
-                    continue;
-                }
-                const uint32_t n = padded ? (tile.steps + kPiece - 1) / kPiece * kPiece : tile.steps;
-                while (at < end && at < before + (uint64_t)n * per_row && ring.ok) {
-                    const uint32_t h = (uint32_t)((at - before) / n), s0 = (uint32_t)((at - before) % n);
-                    const uint64_t start = at - s0;
-                    const uint32_t s1 = (uint32_t)min((uint64_t)n, end - start);
-                    const uint32_t kvh = h / p.parts, hp = h % p.parts;
+            while (ring.ok) {
+                const Tile tile = tile_at<LIST>(p, rows, first, l);
+                const uint32_t n = taken(tile.steps);
+                uint32_t h = (at - before) / n;
+                uint32_t start = before + h * n;
+                for (; h < per_row && at < end && ring.ok; h++) {
+                    const uint32_t kvh = p.parts == 1 ? h : h / p.parts, hp = h - kvh * p.parts;
                     const uint32_t head0 = kvh * p.group + hp * p.part, part = min(p.part, p.group - hp * p.part);
-                    const uint32_t w0 = (uint32_t)(start / run), w1 = (uint32_t)((start + tile.steps - 1) / run);
-                    if (s0 == 0 && p.merged && lane < tile.tokens)
-                        p.places[(size_t)(row + lane) * per_row + h] = make_uint4(w0, w1, start % run != 0, lane * part);
-                    const Target to = {w0 != w1, (size_t)worker * 2 + begun};
-                    const uint32_t stop = min(s1, tile.steps);
+                    const uint32_t from = at - start, stop = min(tile.steps, end - start);
+                    const Target to = {from > 0 || stop < tile.steps, (size_t)worker * 2 + begun};
                     if (tile.tokens * part <= 8)
-                        attend_steps<W, 1, LIST>(p, &map_k, &map_v, tile, kvh, head0, part, s0, stop, to, ring, status, lane);
+                        attend_steps<W, 1, LIST>(p, &map_k, &map_v, tile, kvh, head0, part, from, stop, to, ring, status, lane);
                     else
-                        attend_steps<W, 2, LIST>(p, &map_k, &map_v, tile, kvh, head0, part, s0, stop, to, ring, status, lane);
+                        attend_steps<W, 2, LIST>(p, &map_k, &map_v, tile, kvh, head0, part, from, stop, to, ring, status, lane);
+                    // who has the tile's first step says where its partials are
+                    if (from == 0 && p.merged && lane < tile.tokens)
+                        p.places[(size_t)(tile.row + lane) * per_row + h] = make_uint4(worker, (start + tile.steps - 1) / run, begun, lane * part);
                     begun = true;
-                    at = start + s1;
+                    start += n;
+                    at = start;
                 }
-                before += (uint64_t)n * per_row;
-                row++;
+                if (at >= end) break;
+                before += n * per_row;
+                const uint32_t later = __ballot_sync(0xFFFFFFFFu, rows.steps != 0 && lane > l);
+                if (later) {
+                    l = __ffs(later) - 1;
+                } else {
+                    first += width;
+                    if (first >= p.rows) break;
+                    rows = rows_from<W, LIST>(p, row_at(p, first, lane), first, lane);
+                    l = 0;
+                }
             }
         }
     }
     pdl_launch_dependents();
 }
 
-// One block per (row, head): folds the partials of its tile in the order of their keys.
+// One block per (row, head): folds the partials of its tile in the order of their keys.  Threads take partials side by
+// side for their weights, then W / 4 threads read a partial's output and 1024 / W partials are under way at once.
+constexpr int kMergeThreads = 256;
+
 template <int W>
-__global__ void __launch_bounds__(W) attend_q8_merge_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(kMergeThreads) attend_q8_merge_kernel(const AttendParams p) {
+    constexpr uint32_t COLS = W / 4, SETS = kMergeThreads / COLS;
+    extern __shared__ float weight[];  // [partials]
+    __shared__ float sm_top[kMergeThreads / 32], sm_l[kMergeThreads / 32];
+    __shared__ float4 sm_o[SETS][COLS];
     pdl_wait();
-    const uint32_t row = blockIdx.x / p.heads, head = blockIdx.x % p.heads, d = threadIdx.x;
+    const uint32_t row = blockIdx.x / p.heads, head = blockIdx.x % p.heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t kvh = head / p.group, in = head % p.group, hp = in / p.part;
     const uint4 place = p.places[((size_t)row * p.kv_heads + kvh) * p.parts + hp];
     const uint32_t m = place.w + in % p.part;
-    if (place.x < place.y && place.y < p.workers && place.z < 2 && m < p.most) {  // else its one worker wrote it (or gave up)
-        auto slot = [&](uint32_t w) { return ((size_t)w * 2 + (w == place.x ? place.z : 0)) * p.most + m; };
+    // else its one worker wrote it (or gave up)
+    if (place.x < place.y && place.y < p.workers && place.z < 2 && m < p.most) {
+        const uint32_t n = place.y - place.x + 1;
+        auto slot = [&](uint32_t i) { return ((size_t)(place.x + i) * 2 + (i == 0 ? place.z : 0)) * p.most + m; };
+        // the first outputs are asked for before their weights are known
+        constexpr int EARLY = 4;
+        const uint32_t set = threadIdx.x / COLS, col = threadIdx.x % COLS;
+        float4 early[EARLY];
+#pragma unroll
+        for (int k = 0; k < EARLY; k++)
+            if (set + k * SETS < n) early[k] = *reinterpret_cast<const float4 *>(p.part_o + slot(set + k * SETS) * W + col * 4);
         float top = -INFINITY;
-        for (uint32_t w = place.x; w <= place.y; w++) top = fmaxf(top, p.part_ml[slot(w) * 2]);
-        const float z = top == -INFINITY ? 0.0f : top;
-        float l = 0.0f, o = 0.0f;
-        for (uint32_t w = place.x; w <= place.y; w++) {
-            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + slot(w) * 2);
-            const float f = exp2_approx(ml.x - z);
-            l = fmaf(ml.y, f, l);
-            o = fmaf(p.part_o[slot(w) * W + d], f, o);
+        for (uint32_t i = threadIdx.x; i < n; i += kMergeThreads) {
+            weight[i] = p.part_ml[slot(i) * 2];
+            top = fmaxf(top, weight[i]);
         }
-        p.out[((size_t)row * p.heads + head) * W + d] = l == 0.0f ? (uint16_t)0 : bf16_bits(o / l);
+        top = warp_max(top);
+        if (lane == 0) sm_top[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kMergeThreads / 32; w++) top = fmaxf(top, sm_top[w]);
+        if (top == -INFINITY) top = 0.0f;
+        float l = 0.0f;
+        for (uint32_t i = threadIdx.x; i < n; i += kMergeThreads) {
+            const float f = exp2_approx(weight[i] - top);
+            weight[i] = f;
+            l = fmaf(p.part_ml[slot(i) * 2 + 1], f, l);
+        }
+        l = warp_sum(l);
+        if (lane == 0) sm_l[warp] = l;
+        __syncthreads();
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        auto add = [&](const float4 &v, float f) {
+            o.x = fmaf(v.x, f, o.x);
+            o.y = fmaf(v.y, f, o.y);
+            o.z = fmaf(v.z, f, o.z);
+            o.w = fmaf(v.w, f, o.w);
+        };
+#pragma unroll
+        for (int k = 0; k < EARLY; k++)
+            if (set + k * SETS < n) add(early[k], weight[set + k * SETS]);
+#pragma unroll 4
+        for (uint32_t i = set + EARLY * SETS; i < n; i += SETS)
+            add(*reinterpret_cast<const float4 *>(p.part_o + slot(i) * W + col * 4), weight[i]);
+        sm_o[set][col] = o;
+        __syncthreads();
+        if (threadIdx.x < COLS) {
+            float4 sum = sm_o[0][threadIdx.x];
+            l = sm_l[0];
+#pragma unroll
+            for (int i = 1; i < (int)SETS; i++) {
+                const float4 v = sm_o[i][threadIdx.x];
+                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+            }
+#pragma unroll
+            for (int w = 1; w < kMergeThreads / 32; w++) l += sm_l[w];
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            *reinterpret_cast<uint2 *>(p.out + ((size_t)row * p.heads + head) * W + threadIdx.x * 4) =
+                make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+        }
     }
     pdl_launch_dependents();
 }
@@ -624,7 +822,7 @@ __global__ void __launch_bounds__(W) attend_q8_merge_kernel(const AttendParams p
 __device__ int g_attend_status = 0;
 
 struct Plan {
-    uint32_t part, parts, tokens, workers;
+    uint32_t part, parts, tokens, workers, together;
     bool merged;
     size_t o_bytes, ml_bytes, places_bytes;
     size_t bytes() const { return merged ? o_bytes + ml_bytes + places_bytes : 0; }
@@ -640,11 +838,13 @@ Plan plan_of(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, ui
     uint64_t span = keys;  // keys a tile may see; the first of them is anywhere in its block of 64 at most
     if (!count && (uint64_t)back + s.tokens < span) span = (uint64_t)back + s.tokens;
     const uint64_t steps = count ? ((uint64_t)count * block + step - 1) / step : (span + 63 + step - 1) / step;
-    const uint64_t most = (uint64_t)sm_count() * (width == 256 ? Shape<256>::CTAS : Shape<128>::CTAS) * kWarps;
-    const uint64_t pieces = (uint64_t)rows * kv_heads * s.parts * ((steps + kPiece - 1) / kPiece);
-    s.workers = (uint32_t)(pieces < most ? pieces : most);
-    // Without a second kernel only where no tile can be cut: each fits one piece and there is a worker for every piece.
-    s.merged = steps > kPiece || pieces > most;
+    const uint64_t most = (uint64_t)sm_count() * kBlocks * kWarps;
+    const uint64_t each = (uint64_t)kv_heads * s.parts * steps;  // steps of a row at most
+    // The kernel counts steps in 32 bits: more rows than that allows go in several launches, whole tiles each.
+    uint64_t together = 0x7FFFFFFFull / each / s.tokens * s.tokens;
+    s.together = (uint32_t)(rows < together ? rows : together);
+    s.workers = (uint32_t)(s.together * each < most ? s.together * each : most);
+    s.merged = s.together * each > 1;  // else the one step there is belongs to one worker
     s.o_bytes = (size_t)s.workers * 2 * s.tokens * s.part * width * sizeof(float);
     s.ml_bytes = align_up((size_t)s.workers * 2 * s.tokens * s.part * 2 * sizeof(float), 16);
     s.places_bytes = (size_t)rows * kv_heads * s.parts * sizeof(uint4);
@@ -653,7 +853,7 @@ Plan plan_of(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, ui
 
 template <int W, bool LIST>
 int launch_attend(const AttendParams &p, cudaStream_t stream) {
-    constexpr size_t smem = kWarps * Shape<W>::STAGES * kStage;
+    constexpr size_t smem = kWarps * kStages * kStage;
     static OncePerDevice configured;
     if (configured.needs()) {
         TS_CUDA(cudaFuncSetAttribute(attend_q8_kernel<W, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -668,10 +868,11 @@ int launch_attend(const AttendParams &p, cudaStream_t stream) {
     int rc = make_tensor_map_codes(&map_k, p.kv.k, rows, W, Step<W>::COLS, box);
     if (rc == TS_OK) rc = make_tensor_map_codes(&map_v, p.kv.v, rows, W, Step<W>::COLS, box);
     if (rc != TS_OK) return rc;
-    const uint32_t grid = min(p.workers, (uint32_t)sm_count() * Shape<W>::CTAS);
+    const uint32_t grid = min(p.workers, (uint32_t)sm_count() * kBlocks);
     cudaError_t e = launch(attend_q8_kernel<W, LIST>, dim3(grid), dim3(kThreads), smem, stream, pdl_enabled(), map_k, map_v, p, status);
     if (e == cudaSuccess && p.merged)  // always as a dependent launch: it waits for the partials itself
-        e = launch(attend_q8_merge_kernel<W>, dim3(p.rows * p.heads), dim3(W), 0, stream, true, p);
+        e = launch(attend_q8_merge_kernel<W>, dim3(p.rows * p.heads), dim3(kMergeThreads),
+                   p.workers * sizeof(float), stream, true, p);
     if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of attend (q8) failed: %s", cudaGetErrorString(e));
     return TS_OK;
 }
@@ -695,12 +896,16 @@ size_t attend_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t heads, u
 int attend_q8(const void *q, const RowsQ8Dev &kv, const uint32_t *ids, void *out, const uint32_t *slots,
               const uint32_t *positions, uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,
               uint32_t back, uint32_t count, float scale, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+    // A slot has no keys past what its stride or its pages hold (and fewer keys never ask for a larger workspace).
+    const uint64_t room = (uint64_t)kv.scalar << (kv.per_shift + kv.shift);
+    if (room < keys) keys = (uint32_t)room;
     const Plan s = plan_of(rows, keys, heads, kv_heads, width, back, count, 1u << kv.shift);
     const size_t need = s.bytes();
     TS_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace != nullptr && aligned16(workspace))),
                "attend (q8): workspace of %zu bytes is smaller than the %zu needed, or not 16-byte aligned", workspace_bytes, need);
     TS_REQUIRE((uint64_t)rows * heads < 0x7FFFFFFFull, "attend (q8): %u rows are too many for one launch", rows);
     TS_REQUIRE((((uint64_t)kv.blocks * kv_heads) << kv.shift) < 0x7FFFFFFFull, "attend (q8): a pool of %u blocks is too large", kv.blocks);
+    TS_REQUIRE(s.together > 0, "attend (q8): %u keys of %u kv heads are too many for one launch", keys, kv_heads);
     AttendParams p = {};
     p.q = (const uint16_t *)q;
     p.kv = kv;
@@ -727,9 +932,19 @@ int attend_q8(const void *q, const RowsQ8Dev &kv, const uint32_t *ids, void *out
         p.part_ml = (float *)((uint8_t *)workspace + s.o_bytes);
         p.places = (uint4 *)((uint8_t *)workspace + s.o_bytes + s.ml_bytes);
     }
-    return width == 64    ? (ids ? launch_attend<64, true>(p, stream) : launch_attend<64, false>(p, stream))
-           : width == 128 ? (ids ? launch_attend<128, true>(p, stream) : launch_attend<128, false>(p, stream))
-                          : (ids ? launch_attend<256, true>(p, stream) : launch_attend<256, false>(p, stream));
+    for (uint32_t row = 0; row < rows; row += s.together) {
+        p.q = (const uint16_t *)q + (size_t)row * heads * width;
+        p.out = (uint16_t *)out + (size_t)row * heads * width;
+        p.ids = ids ? ids + (size_t)row * kv_heads * count : nullptr;
+        p.slots = slots + row;
+        p.positions = positions + row;
+        p.rows = min(s.together, rows - row);
+        const int rc = width == 64    ? (ids ? launch_attend<64, true>(p, stream) : launch_attend<64, false>(p, stream))
+                       : width == 128 ? (ids ? launch_attend<128, true>(p, stream) : launch_attend<128, false>(p, stream))
+                                      : (ids ? launch_attend<256, true>(p, stream) : launch_attend<256, false>(p, stream));
+        if (rc != TS_OK) return rc;
+    }
+    return TS_OK;
 }
 
 }  // namespace ts
