@@ -1,11 +1,15 @@
 // Kept rows in 8 bits: append (norm, rotation, block scales, key bounds) and reading rows back.
 //
 // Append.  A block of B positions has one scale per kv head, so the rows of a call that fall into one block are one
-// unit of work: run = the neighbouring rows of a (slot, block).  One thread block per (run, kv head, k or v): its four
-// warps take the block's positions in turn, keep the prepared values of their B / 4 positions in registers, agree on the
-// largest magnitude through shared memory, and write codes once, so that every value is read once and rounded once.
-// Held codes are read and rewritten only when the scale grows (a new largest value: for values without a trend once in
-// i rows at the block's i-th row).  Query heads go to warps of their own.
+// unit of work: run = the neighbouring rows of a (slot, block).  A long run (a prompt's) belongs to a thread block for each
+// kv head's keys and values: its eight warps take the block's positions in turn and agree on the largest magnitude
+// through shared memory.  A short run (a step's row) belongs to one warp.  Either way the prepared values stay in registers
+// until the scale is known, so that every value is read once and rounded once.  Held codes are read and rewritten only when
+// the scale grows (a new largest value: for values without a trend once in i rows at the block's i-th row).  Query
+// heads go to warps of their own, eight heads of a row each when there are many.
+//
+// W / 8 lanes hold a head: lane i of them the four pairs 4 i .. 4 i + 3, elements 4 i + e and W / 2 + 4 i + e, so that
+// loads are 8 bytes and stores of codes 4 a lane.
 #include <cmath>
 
 #include "rows_q8.cuh"
@@ -58,62 +62,75 @@ namespace {
 constexpr float kScaleFloor = 8.673617379884035e-19f;  // 2^-60
 constexpr float kLargest = 3.3895313892515355e38f;    // the largest finite bf16
 
-// Cosine and sine of pos * f, the product and its reduction to [-pi, pi] in 64 bits: in 32 bits position 100000 would
-// leave an error of 100000 * 2^-24 = 0.006 radians.  Two constants: 2 pi and what its 64-bit form leaves out.
-__device__ __forceinline__ void turn_of(uint32_t pos, float f, float *s, float *c) {
-    double a = (double)pos * (double)f;
-    const double n = rint(a * 0.15915494309189535);
-    a = fma(n, -6.283185307179586, a);
-    a = fma(n, -2.4492935982947064e-16, a);
-    sincosf((float)a, s, c);
+// Cosine and sine of pos * f.  In 32 bits the product would be off by 0.006 radians at position 100000, so the angle is
+// kept in turns as a 64-bit fraction: pos * round(2^64 f / 2 pi) modulo 2^64, whose rounding is below 1e-7 turns at any
+// position.  The upper 32 bits, less whole quarters, are an angle within pi / 4, where the series of sine to the ninth
+// and of cosine to the eighth power are off by 2e-9 and 3e-8.
+__device__ __forceinline__ uint64_t turns_of(float f) {
+    const double v = (double)f * 0.15915494309189535;  // 1 / 2 pi
+    return __double2ull_rn((v - floor(v)) * 18446744073709551616.0);
 }
 
-// A head's row on a warp: lane l owns the pairs j = l * PER + e (e < PER = W / 64): x[e] is element j, x[PER + e]
-// element j + W / 2.
-template <int W>
-__device__ __forceinline__ void load_head(const uint16_t *src, uint32_t lane, uint32_t (&raw)[W / 64]) {
-    constexpr int PER = W / 64;
-    if constexpr (PER == 1) {
-        raw[0] = (uint32_t)src[lane] | ((uint32_t)src[lane + W / 2] << 16);  // low half: element j, high half: j + W / 2
-    } else if constexpr (PER == 2) {
-        raw[0] = *reinterpret_cast<const uint32_t *>(src + lane * 2);
-        raw[1] = *reinterpret_cast<const uint32_t *>(src + W / 2 + lane * 2);
-    } else {
-        const uint2 a = *reinterpret_cast<const uint2 *>(src + lane * 4), b = *reinterpret_cast<const uint2 *>(src + W / 2 + lane * 4);
-        raw[0] = a.x; raw[1] = a.y; raw[2] = b.x; raw[3] = b.y;
-    }
+__device__ __forceinline__ void sine_cosine(uint32_t pos, uint64_t turns, float *s, float *c) {
+    const uint32_t t = (uint32_t)((pos * turns) >> 32);
+    const uint32_t quarter = (t + (1u << 29)) >> 30;
+    const float x = (float)(int32_t)(t - (quarter << 30)) * 1.4629180792671596e-9f, x2 = x * x;  // 2 pi / 2^32
+    const float sine = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 2.7557319e-6f, -1.9841270e-4f), 8.3333333e-3f), -1.6666667e-1f), x);
+    const float cosine = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 2.4801587e-5f, -1.3888889e-3f), 4.1666667e-2f), -0.5f), 1.0f);
+    const bool swap = quarter & 1;
+    const float a = swap ? cosine : sine, b = swap ? sine : cosine;
+    *s = quarter & 2 ? -a : a;
+    *c = (quarter + 1) & 2 ? -b : b;
 }
 
-// The head's values in raw order (widened): x[i], i < W / 32, elements lane * PER + i, then W / 2 + lane * PER + i - PER.
+// What a lane holds of a head: lane i of the W / 8.
 template <int W>
-__device__ __forceinline__ void widen(const uint32_t (&raw)[W / 64], float (&x)[W / 32]) {
-#pragma unroll
-    for (int i = 0; i < W / 64; i++) {
-        x[2 * i] = bf16_lo(raw[i]);
-        x[2 * i + 1] = bf16_hi(raw[i]);
-    }
-}
+struct Lanes {
+    static constexpr int PER_HEAD = W / 8, TOGETHER = 32 / PER_HEAD;  // lanes of a head; heads a warp holds at once
+};
+
+struct Raw {
+    uint2 a, b;  // bf16 elements 4 i .. 4 i + 3 and W / 2 + 4 i ..
+};
 
 template <int W>
-__device__ __forceinline__ void norm_turn(float (&x)[W / 32], const float *gain, const float (&sn)[W / 64],
-                                          const float (&cs)[W / 64], float eps, uint32_t lane) {
-    constexpr int PER = W / 64;
-    if (gain) {
+__device__ __forceinline__ Raw load_head(const uint16_t *src, uint32_t i) {
+    return {*reinterpret_cast<const uint2 *>(src + 4 * i), *reinterpret_cast<const uint2 *>(src + W / 2 + 4 * i)};
+}
+
+__device__ __forceinline__ void widen(const Raw &raw, float (&x)[8]) {
+    x[0] = bf16_lo(raw.a.x); x[1] = bf16_hi(raw.a.x); x[2] = bf16_lo(raw.a.y); x[3] = bf16_hi(raw.a.y);
+    x[4] = bf16_lo(raw.b.x); x[5] = bf16_hi(raw.b.x); x[6] = bf16_lo(raw.b.y); x[7] = bf16_hi(raw.b.y);
+}
+
+// Norm (g: the lane's gains) and rotation, in 32 bits.
+template <int W>
+__device__ __forceinline__ void norm_turn(float (&x)[8], bool normed, const float (&g)[8], const float (&sn)[4], const float (&cs)[4],
+                                          float eps) {
+    if (normed) {
         float ss = 0.0f;
 #pragma unroll
-        for (int i = 0; i < W / 32; i++) ss = fmaf(x[i], x[i], ss);
-        const float inv = 1.0f / sqrtf(warp_sum(ss) / (float)W + eps);
+        for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-        for (int e = 0; e < PER; e++) {
-            x[e] *= inv * gain[lane * PER + e];
-            x[PER + e] *= inv * gain[lane * PER + e + W / 2];
-        }
+        for (int o = 1; o < Lanes<W>::PER_HEAD; o <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+        const float inv = 1.0f / sqrtf(ss / (float)W + eps);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] *= inv * g[i];
     }
 #pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const float a = x[e], b = x[PER + e];
+    for (int e = 0; e < 4; e++) {
+        const float a = x[e], b = x[4 + e];
         x[e] = a * cs[e] - b * sn[e];
-        x[PER + e] = a * sn[e] + b * cs[e];
+        x[4 + e] = a * sn[e] + b * cs[e];
+    }
+}
+
+template <int W>
+__device__ __forceinline__ void load_gains(const float *gain, uint32_t i, float (&g)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        g[e] = gain ? gain[4 * i + e] : 1.0f;
+        g[4 + e] = gain ? gain[W / 2 + 4 * i + e] : 1.0f;
     }
 }
 
@@ -130,42 +147,137 @@ struct AppendParams {
     uint32_t per_warp;  // query heads a warp takes
 };
 
-__device__ __forceinline__ int to_code(float x) {  // NaN converts to 0, infinities to the ends of the integer range
-    return max(-127, min(127, __float2int_rn(x)));
+__device__ __forceinline__ float min_nan(float a, float b) {  // NaN if either is
+    float v;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float v;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
+    return v;
+}
+// What is kept of an infinity and of NaN.
+__device__ __forceinline__ float tame(float x) { return x != x ? 0.0f : fminf(fmaxf(x, -kLargest), kLargest); }
+
+// round(x * inv) for |x * inv| < 2^22 in the low bits: the sum's last place is one.
+__device__ __forceinline__ uint32_t code_bits(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.0f)); }
+__device__ __forceinline__ uint32_t pack_bits(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+__device__ __forceinline__ float code_at(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
+
+// A block's scale before and after, and how its codes follow.
+struct Scales {
+    float inv, ratio, now;
+    bool fresh;
+};
+
+__device__ __forceinline__ Scales grow(const float *scale, bool fresh, float most) {
+    const float old = fresh ? 0.0f : *scale;
+    Scales s;
+    s.now = fmaxf(old, fmaxf(most / 127.0f, kScaleFloor));
+    s.inv = 1.0f / s.now;
+    s.ratio = fresh ? 1.0f : old / s.now;  // within [0, 1] for every scale that append writes
+    s.fresh = fresh;
+    return s;
 }
 
-template <int W, int B>
-__global__ void __launch_bounds__(128) append_q8_kernel(const AppendParams p) {
-    constexpr int PER = W / 64, N = W / 32, MINE = B / 4;  // positions of a block per warp
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// |x| <= most, so that no code passes 127.
+template <int W>
+__device__ __forceinline__ void write_row(int8_t *row, uint32_t i, const float (&x)[8], float inv) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        *reinterpret_cast<uint32_t *>(row + h * (W / 2) + 4 * i) =
+            pack_bits(code_bits(x[4 * h], inv), code_bits(x[4 * h + 1], inv), code_bits(x[4 * h + 2], inv), code_bits(x[4 * h + 3], inv));
+}
+
+// A held row's codes follow the scale (a code of -128, which append never writes, becomes -127 at most).
+__device__ __forceinline__ uint32_t follow(uint32_t w, float ratio) {
+    uint32_t c[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) c[e] = code_bits(fmaxf(code_at(w, e), -127.0f), ratio);
+    return pack_bits(c[0], c[1], c[2], c[3]);
+}
+
+template <int W>
+__device__ __forceinline__ void follow_row(int8_t *row, uint32_t i, float ratio) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        uint32_t *at = reinterpret_cast<uint32_t *>(row + h * (W / 2) + 4 * i);
+        *at = follow(*at, ratio);
+    }
+}
+
+// Bounds of four channels from the least and the largest new value (rounding keeps their order), joined with those the
+// block had unless it is fresh.
+template <int W>
+__device__ __forceinline__ void write_bounds(int8_t *bounds, uint32_t first, const float *low, const float *high, const Scales &sc) {
+    uint32_t *lo = reinterpret_cast<uint32_t *>(bounds + first), *hi = reinterpret_cast<uint32_t *>(bounds + W + first);
+    const uint32_t was_lo = sc.fresh ? 0 : follow(*lo, sc.ratio), was_hi = sc.fresh ? 0 : follow(*hi, sc.ratio);
+    uint32_t a[4], b[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        int l = (int8_t)code_bits(low[e], sc.inv), h = (int8_t)code_bits(high[e], sc.inv);
+        if (!sc.fresh) {
+            l = min(l, (int)(int8_t)(was_lo >> (8 * e)));
+            h = max(h, (int)(int8_t)(was_hi >> (8 * e)));
+        }
+        a[e] = (uint32_t)l;
+        b[e] = (uint32_t)h;
+    }
+    *lo = pack_bits(a[0], a[1], a[2], a[3]);
+    *hi = pack_bits(b[0], b[1], b[2], b[3]);
+}
+
+constexpr uint32_t kShort = 4;  // rows of a run that one warp takes
+constexpr int kAppendWarps = 4, kAppendThreads = kAppendWarps * 32;
+
+// Parts of an append in one kernel: blocks [0, kv_ctas) keys and values, the others queries.
+enum Role { kAll, kKeysValues, kQueries };
+
+template <int W, int B, Role ROLE>
+__global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQueries ? 8 : 6) append_q8_kernel(const AppendParams p) {
+    constexpr int L = Lanes<W>::PER_HEAD, T = Lanes<W>::TOGETHER;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, li = lane % L, which = lane / L;
     const uint32_t per_row = p.heads + 2 * p.kv_heads;
+    __shared__ uint64_t sm_turns[W / 2];  // each pair's, computed once: its 64-bit arithmetic is slow
     pdl_wait();
-    if (blockIdx.x >= p.kv_ctas) {
-        // ---- queries: a warp takes `per_warp` heads of a row, the row's angles are computed once ----
+    if (threadIdx.x < W / 2) sm_turns[threadIdx.x] = turns_of(p.inv_freq[threadIdx.x]);
+    __syncthreads();
+    uint64_t turns[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) turns[e] = sm_turns[4 * li + e];
+    if (ROLE == kQueries || (ROLE == kAll && blockIdx.x >= p.kv_ctas)) {
+        // ---- queries: a warp takes up to `per_warp` heads of a row, T of them side by side ----
         const uint32_t parts = (p.heads + p.per_warp - 1) / p.per_warp;
-        const uint64_t unit = (uint64_t)(blockIdx.x - p.kv_ctas) * 4 + warp;
+        const uint64_t unit = (uint64_t)(blockIdx.x - (ROLE == kAll ? p.kv_ctas : 0)) * kAppendWarps + warp;
         if (unit < (uint64_t)p.rows * parts) {
             const uint32_t r = unit / parts, h0 = unit % parts * p.per_warp, h1 = min(p.heads, h0 + p.per_warp);
             const uint32_t pos = p.positions[r];
-            float sn[PER], cs[PER];
+            float sn[4], cs[4], g[8];
+            constexpr int PASSES = 8 / T;
+            Raw raw[PASSES];
 #pragma unroll
-            for (int e = 0; e < PER; e++) turn_of(pos, p.inv_freq[lane * PER + e], &sn[e], &cs[e]);
-            for (uint32_t h = h0; h < h1; h++) {
-                uint32_t raw[PER];
-                load_head<W>(p.qkv + ((size_t)r * per_row + h) * W, lane, raw);
-                float x[N];
-                widen<W>(raw, x);
-                norm_turn<W>(x, p.q_norm, sn, cs, p.eps, lane);
-                uint16_t *dst = p.q_out + ((size_t)r * p.heads + h) * W;
-                if constexpr (PER == 1) {
-                    dst[lane] = bf16_bits(x[0]);
-                    dst[lane + W / 2] = bf16_bits(x[1]);
-                } else {
+            for (int k = 0; k < PASSES; k++) {
+                const uint32_t h = h0 + k * T + which;
+                raw[k] = {make_uint2(0, 0), make_uint2(0, 0)};
+                if (h < h1) raw[k] = load_head<W>(p.qkv + ((size_t)r * per_row + h) * W, li);
+            }
+            load_gains<W>(p.q_norm, li, g);
 #pragma unroll
-                    for (int e = 0; e < PER; e += 2) {
-                        *reinterpret_cast<uint32_t *>(dst + lane * PER + e) = pack_bf16(x[e], x[e + 1]);
-                        *reinterpret_cast<uint32_t *>(dst + W / 2 + lane * PER + e) = pack_bf16(x[PER + e], x[PER + e + 1]);
-                    }
+            for (int e = 0; e < 4; e++) sine_cosine(pos, turns[e], &sn[e], &cs[e]);
+#pragma unroll
+            for (int k = 0; k < PASSES; k++) {
+                if (h0 + k * T >= h1) break;
+                const uint32_t h = h0 + k * T + which;
+                float x[8];
+                widen(raw[k], x);
+                norm_turn<W>(x, p.q_norm != nullptr, g, sn, cs, p.eps);
+                if (h < h1) {
+                    uint16_t *dst = p.q_out + ((size_t)r * p.heads + h) * W + 4 * li;
+                    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+                    *reinterpret_cast<uint2 *>(dst + W / 2) = make_uint2(pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
                 }
             }
         }
@@ -173,173 +285,343 @@ __global__ void __launch_bounds__(128) append_q8_kernel(const AppendParams p) {
         return;
     }
 
-    __shared__ int src[B];          // the row that writes each position of the block, or -1
+    __shared__ int src[B];  // long runs: the row that writes each position of the block, or -1
     __shared__ uint32_t stop;
-    __shared__ float sm_max[4];
-    __shared__ int8_t sm_low[4][W], sm_high[4][W];
+    __shared__ float sm_max[kAppendWarps];
+    // Long runs: a thread's prepared values wait here for the scale (in registers they would leave room for 12 warps an SM,
+    // 54 us for 8165 rows), then the block's bounds are put together in the same place.
+    extern __shared__ __align__(16) float4 kept[];  // [passes][2][threads]
     const uint32_t units = 2 * p.kv_heads, unit = blockIdx.x % units;
     const bool is_v = unit >= p.kv_heads;
     const uint32_t h = is_v ? unit - p.kv_heads : unit;
+    const uint16_t *heads = p.qkv + (size_t)(p.heads + unit) * W;  // this unit's head of row 0
+    const bool bounded = !is_v && p.kv.bounds != nullptr, normed = !is_v && p.k_norm != nullptr;
     const uint32_t r0 = blockIdx.x / units * p.window, r1 = min(p.rows, r0 + p.window);
-    for (uint32_t r = r0; r < r1; r++) {
-        const uint32_t slot = p.slots[r], b = p.positions[r] >> p.kv.shift;
-        if (r > 0 && p.slots[r - 1] == slot && (p.positions[r - 1] >> p.kv.shift) == b) continue;  // not a run's first row
-        const uint32_t blk = block_of(p.kv, slot, b);
+    // ---- the runs that begin among rows [r0, r1), at most 32 of them, one a lane ----
+    uint32_t slot = 0, blk_pos = 0xFFFFFFFFu;
+    if (r0 + lane < r1) {
+        slot = p.slots[r0 + lane];
+        blk_pos = p.positions[r0 + lane] >> p.kv.shift;
+    }
+    uint32_t slot_was = __shfl_up_sync(0xFFFFFFFFu, slot, 1), pos_was = __shfl_up_sync(0xFFFFFFFFu, blk_pos, 1);
+    if (lane == 0 && r0 > 0) {
+        slot_was = p.slots[r0 - 1];
+        pos_was = p.positions[r0 - 1] >> p.kv.shift;
+    }
+    const bool begins = r0 + lane < r1 && ((r0 == 0 && lane == 0) || slot != slot_was || blk_pos != pos_was);
+    uint32_t starts = __ballot_sync(0xFFFFFFFFu, begins);
+    float g[8];
+    if (starts) load_gains<W>(normed ? p.k_norm : nullptr, li, g);
+    for (uint32_t turn = 0; starts; turn++) {
+        const uint32_t first = __ffs(starts) - 1;
+        starts &= starts - 1;
+        const uint32_t s = r0 + first, run_slot = __shfl_sync(0xFFFFFFFFu, slot, first), b = __shfl_sync(0xFFFFFFFFu, blk_pos, first);
+        const uint32_t blk = block_of(p.kv, run_slot, b);
+        auto same = [&](uint32_t i) { return i < p.rows && p.slots[i] == run_slot && (p.positions[i] >> p.kv.shift) == b; };
+        // rows of the run, as far as kShort + 1: the next run's start tells, or the rows past this block's do
+        uint32_t n = starts ? __ffs(starts) - 1 - first : r1 - s;
+        if (!starts && n <= kShort) {
+            const uint32_t out = ~__ballot_sync(0xFFFFFFFFu, lane < n || (lane <= kShort && same(s + lane)));
+            n = __ffs(out) - 1;
+        }
         if (blk == kNoBlock) continue;
-        // ---- the run: which row writes which position ----
+        const size_t at = (size_t)blk * p.kv_heads + h;
+        float *scale = (is_v ? p.kv.v_scale : p.kv.k_scale) + at;
+        int8_t *codes = (is_v ? p.kv.v : p.kv.k) + at * B * W;
+        int8_t *bounds = p.kv.bounds + at * 2 * W;
+        if (n <= kShort) {
+            // ---- a warp's run ----
+            if (turn % kAppendWarps != warp) continue;
+            constexpr int PASSES = kShort / T > 0 ? kShort / T : 1;
+            uint64_t written = 0;
+            for (uint32_t k = 0; k < n; k++) written |= 1ull << (p.positions[s + k] & (B - 1));
+            float x[PASSES][8], low[8], high[8];
+            int8_t *row[PASSES];
+#pragma unroll
+            for (int e = 0; e < 8; e++) low[e] = INFINITY, high[e] = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < PASSES; k++) {
+                const uint32_t j = k * T + which;
+                uint32_t pos = 0;
+                bool live = j < n;
+                Raw raw = {make_uint2(0, 0), make_uint2(0, 0)};
+                if (live) {
+                    raw = load_head<W>(heads + (size_t)(s + j) * per_row * W, li);
+                    pos = p.positions[s + j];
+                    for (uint32_t later = j + 1; later < n; later++) live = live && p.positions[s + later] != pos;
+                }
+                widen(raw, x[k]);
+                if (!is_v && k * T < n) {
+                    float sn[4], cs[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sine_cosine(pos, turns[e], &sn[e], &cs[e]);
+                    norm_turn<W>(x[k], normed, g, sn, cs, p.eps);
+                }
+                row[k] = live ? codes + (pos & (B - 1)) * W : nullptr;
+                if (live) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[k][e] = tame(x[k][e]);
+                        low[e] = fminf(low[e], x[k][e]);
+                        high[e] = fmaxf(high[e], x[k][e]);
+                    }
+                }
+            }
+            float most = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (high[e] >= low[e]) most = fmaxf(most, fmaxf(fabsf(low[e]), fabsf(high[e])));
+            most = warp_max(most);
+            const Scales sc = grow(scale, written & 1, most);
+#pragma unroll
+            for (int k = 0; k < PASSES; k++)
+                if (row[k]) write_row<W>(row[k], li, x[k], sc.inv);
+            if (sc.ratio < 1.0f)
+                for (uint32_t i = which; i < (uint32_t)B; i += T)
+                    if (!(written >> i & 1)) follow_row<W>(codes + i * W, li, sc.ratio);
+            if (bounded) {
+#pragma unroll
+                for (int o = L; o < 32; o <<= 1)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        low[e] = fminf(low[e], __shfl_xor_sync(0xFFFFFFFFu, low[e], o));
+                        high[e] = fmaxf(high[e], __shfl_xor_sync(0xFFFFFFFFu, high[e], o));
+                    }
+                if (which == 0) {
+                    write_bounds<W>(bounds, 4 * li, low, high, sc);
+                    write_bounds<W>(bounds, W / 2 + 4 * li, low + 4, high + 4, sc);
+                }
+            }
+            __syncwarp();  // every lane has read the old scale
+            if (lane == 0) *scale = sc.now;
+            continue;
+        }
+        // ---- a thread block's run: which row writes which position ----
+        constexpr int STEP = kAppendWarps * T, PASSES = B > STEP ? B / STEP : 1;  // positions warp * T + which + STEP u
+        const uint32_t mine = warp * T + which;
         __syncthreads();
         if (threadIdx.x < B) src[threadIdx.x] = -1;
         if (threadIdx.x == 0) stop = p.rows;
         __syncthreads();
-        for (uint32_t base = r; base < p.rows; base += 128) {
+        for (uint32_t base = s; base < p.rows; base += kAppendThreads) {
             const uint32_t i = base + threadIdx.x;
-            const uint32_t pos = i < p.rows ? p.positions[i] : 0;
-            const bool in = i < p.rows && p.slots[i] == slot && (pos >> p.kv.shift) == b;
+            const bool in = same(i);
             if (!in && i < p.rows) atomicMin(&stop, i);
             __syncthreads();
-            const uint32_t end = stop;
-            if (in && i < end) atomicMax(&src[pos & (B - 1)], (int)i);
-            if (end < base + 128) break;
+            const uint32_t end = stop;  // later passes only bring it down to rows past this one's
+            if (in && i < end) atomicMax(&src[p.positions[i] & (B - 1)], (int)i);
+            if (end < base + kAppendThreads) break;
         }
         __syncthreads();
-        const bool fresh = src[0] >= 0;
-        // ---- this warp's positions: warp, warp + 4, ... ----
-        uint32_t raw[MINE][PER];
+        auto row_of = [&](int u) { return mine + STEP * u < B ? src[mine + STEP * u] : -1; };
+        // Least and largest of each of the lane's channels; NaN stays, so that one comparison finds what is to be tamed.
+        float low[8], high[8];
 #pragma unroll
-        for (int u = 0; u < MINE; u++) {
-            const int row = src[warp + 4 * u];
+        for (int e = 0; e < 8; e++) low[e] = INFINITY, high[e] = -INFINITY;
+        float sn[4], cs[4], step_s[4], step_c[4];
+        if (!is_v) {
 #pragma unroll
-            for (int e = 0; e < PER; e++) raw[u][e] = 0;
-            if (row >= 0) load_head<W>(p.qkv + ((size_t)row * per_row + p.heads + unit) * W, lane, raw[u]);
+            for (int e = 0; e < 4; e++) {
+                sine_cosine((b << p.kv.shift) + mine, turns[e], &sn[e], &cs[e]);
+                sine_cosine(STEP, turns[e], &step_s[e], &step_c[e]);
+            }
         }
-        float x[MINE][N];
+        bool any = false;
+        constexpr int GROUP = PASSES < 4 ? PASSES : 4;  // passes whose loads are under way together
+        for (int u0 = 0; u0 < PASSES; u0 += GROUP) {
+            Raw raw[GROUP];
+#pragma unroll
+            for (int k = 0; k < GROUP; k++) {
+                const int row = row_of(u0 + k);
+                raw[k] = {make_uint2(0, 0), make_uint2(0, 0)};
+                if (row >= 0) raw[k] = load_head<W>(heads + (size_t)row * per_row * W, li);
+            }
+#pragma unroll
+            for (int k = 0; k < GROUP; k++) {
+                float x[8];
+                widen(raw[k], x);
+                if (!is_v) {
+                    norm_turn<W>(x, normed, g, sn, cs, p.eps);
+                    // the next pass is STEP positions on: a turn by a fixed angle (at most 15 of them, 2^-24 each)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float s0 = sn[e], c0 = cs[e];
+                        cs[e] = c0 * step_c[e] - s0 * step_s[e];
+                        sn[e] = s0 * step_c[e] + c0 * step_s[e];
+                    }
+                }
+                if (row_of(u0 + k) >= 0) {
+                    any = true;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        low[e] = min_nan(low[e], x[e]);
+                        high[e] = max_nan(high[e], x[e]);
+                    }
+                }
+                kept[(2 * (u0 + k)) * kAppendThreads + threadIdx.x] = make_float4(x[0], x[1], x[2], x[3]);
+                kept[(2 * (u0 + k) + 1) * kAppendThreads + threadIdx.x] = make_float4(x[4], x[5], x[6], x[7]);
+            }
+        }
         float most = 0.0f;
 #pragma unroll
-        for (int u = 0; u < MINE; u++) {
-            widen<W>(raw[u], x[u]);
-            if (!is_v && src[warp + 4 * u] >= 0) {
-                float sn[PER], cs[PER];
+        for (int e = 0; e < 8; e++) most = max_nan(most, max_nan(fabsf(low[e]), fabsf(high[e])));
+        if (any && !(most <= kLargest)) {  // an infinity or NaN among them
+            most = 0.0f;
 #pragma unroll
-                for (int e = 0; e < PER; e++)
-                    turn_of((b << p.kv.shift) + warp + 4 * u, p.inv_freq[lane * PER + e], &sn[e], &cs[e]);
-                norm_turn<W>(x[u], p.k_norm, sn, cs, p.eps, lane);
-            }
+            for (int e = 0; e < 8; e++) low[e] = INFINITY, high[e] = -INFINITY;
+            for (int u = 0; u < PASSES; u++)
 #pragma unroll
-            for (int i = 0; i < N; i++) most = fmaxf(most, fabsf(x[u][i]));  // fmaxf passes over NaN
+                for (int half = 0; half < 2; half++) {
+                    float4 &v = kept[(2 * u + half) * kAppendThreads + threadIdx.x];
+                    float x[4] = {tame(v.x), tame(v.y), tame(v.z), tame(v.w)};
+                    v = make_float4(x[0], x[1], x[2], x[3]);
+                    if (row_of(u) < 0) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        low[4 * half + e] = fminf(low[4 * half + e], x[e]);
+                        high[4 * half + e] = fmaxf(high[4 * half + e], x[e]);
+                        most = fmaxf(most, fabsf(x[e]));
+                    }
+                }
         }
-        most = warp_max(most);
+        most = warp_max(any ? most : 0.0f);
         if (lane == 0) sm_max[warp] = most;
         __syncthreads();
-        most = fminf(fmaxf(fmaxf(sm_max[0], sm_max[1]), fmaxf(sm_max[2], sm_max[3])), kLargest);
-        const size_t at = (size_t)blk * p.kv_heads + h;
-        float *scale = (is_v ? p.kv.v_scale : p.kv.k_scale) + at;
-        const float s_old = fresh ? 0.0f : *scale;
-        const float s_new = fmaxf(s_old, fmaxf(most / 127.0f, kScaleFloor));
-        const float inv = 1.0f / s_new, ratio = fresh ? 1.0f : s_old / s_new;
-        int8_t *codes = (is_v ? p.kv.v : p.kv.k) + at * B * W;
-        int low[N], high[N];
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            low[i] = 127;
-            high[i] = -127;
+        most = fmaxf(fmaxf(sm_max[0], sm_max[1]), fmaxf(sm_max[2], sm_max[3]));
+        const Scales sc = grow(scale, src[0] >= 0, most);
+#pragma unroll 2
+        for (int u = 0; u < PASSES; u++) {
+            const uint32_t i = mine + STEP * u;
+            if (row_of(u) >= 0) {
+                const float4 v = kept[(2 * u) * kAppendThreads + threadIdx.x], w = kept[(2 * u + 1) * kAppendThreads + threadIdx.x];
+                const float x[8] = {v.x, v.y, v.z, v.w, w.x, w.y, w.z, w.w};
+                write_row<W>(codes + i * W, li, x, sc.inv);
+            } else if (i < B && sc.ratio < 1.0f) {
+                follow_row<W>(codes + i * W, li, sc.ratio);
+            }
         }
+        __syncthreads();  // every thread has read the old scale and its kept values
+        if (threadIdx.x == 0) *scale = sc.now;
+        if (bounded) {
+            // lanes that hold the same channels meet in shared memory: [kAppendWarps * T][low, high][W]
+            float *sm = reinterpret_cast<float *>(kept) + mine * 2 * W;
 #pragma unroll
-        for (int u = 0; u < MINE; u++) {
-            int8_t *row = codes + (warp + 4 * u) * W;
-            const bool written = src[warp + 4 * u] >= 0;
-            if (!written && !(ratio < 1.0f)) continue;
-            int c[N];
-            if (written) {
+            for (int half = 0; half < 2; half++) {
+                const uint32_t d = half * (W / 2) + 4 * li;
+                *reinterpret_cast<float4 *>(sm + d) = make_float4(low[4 * half], low[4 * half + 1], low[4 * half + 2], low[4 * half + 3]);
+                *reinterpret_cast<float4 *>(sm + W + d) = make_float4(high[4 * half], high[4 * half + 1], high[4 * half + 2], high[4 * half + 3]);
+            }
+            __syncthreads();
+            if (threadIdx.x < W / 4) {
+                const float *all = reinterpret_cast<const float *>(kept) + 4 * threadIdx.x;
+                float lo[4], hi[4];
 #pragma unroll
-                for (int i = 0; i < N; i++) {
-                    c[i] = to_code(x[u][i] * inv);
-                    low[i] = min(low[i], c[i]);
-                    high[i] = max(high[i], c[i]);
+                for (int e = 0; e < 4; e++) lo[e] = INFINITY, hi[e] = -INFINITY;
+#pragma unroll 4
+                for (int k = 0; k < STEP; k++) {
+                    const float4 l = *reinterpret_cast<const float4 *>(all + k * 2 * W), m = *reinterpret_cast<const float4 *>(all + k * 2 * W + W);
+                    lo[0] = fminf(lo[0], l.x); lo[1] = fminf(lo[1], l.y); lo[2] = fminf(lo[2], l.z); lo[3] = fminf(lo[3], l.w);
+                    hi[0] = fmaxf(hi[0], m.x); hi[1] = fmaxf(hi[1], m.y); hi[2] = fmaxf(hi[2], m.z); hi[3] = fmaxf(hi[3], m.w);
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; i++)
-                    c[i] = to_code((float)row[(i < PER ? 0 : W / 2 - PER) + lane * PER + i] * ratio);
-            }
-            if constexpr (PER == 1) {
-                row[lane] = (int8_t)c[0];
-                row[W / 2 + lane] = (int8_t)c[1];
-            } else if constexpr (PER == 2) {
-                *reinterpret_cast<uint16_t *>(row + lane * 2) = (uint16_t)((c[0] & 255) | (c[1] & 255) << 8);
-                *reinterpret_cast<uint16_t *>(row + W / 2 + lane * 2) = (uint16_t)((c[2] & 255) | (c[3] & 255) << 8);
-            } else {
-                *reinterpret_cast<uint32_t *>(row + lane * 4) =
-                    (c[0] & 255) | (c[1] & 255) << 8 | (c[2] & 255) << 16 | (uint32_t)(c[3] & 255) << 24;
-                *reinterpret_cast<uint32_t *>(row + W / 2 + lane * 4) =
-                    (c[4] & 255) | (c[5] & 255) << 8 | (c[6] & 255) << 16 | (uint32_t)(c[7] & 255) << 24;
+                write_bounds<W>(bounds, 4 * threadIdx.x, lo, hi, sc);
             }
         }
-        if (!is_v && p.kv.bounds) {
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int d = (i < PER ? 0 : W / 2 - PER) + lane * PER + i;
-                sm_low[warp][d] = (int8_t)low[i];
-                sm_high[warp][d] = (int8_t)high[i];
-            }
-        }
-        __syncthreads();  // also: every thread has read the old scale
-        if (!is_v && p.kv.bounds) {
-            int8_t *bounds = p.kv.bounds + at * 2 * W;
-            for (uint32_t d = threadIdx.x; d < W; d += 128) {
-                int lo = min(min(sm_low[0][d], sm_low[1][d]), min(sm_low[2][d], sm_low[3][d]));
-                int hi = max(max(sm_high[0][d], sm_high[1][d]), max(sm_high[2][d], sm_high[3][d]));
-                if (!fresh) {
-                    lo = min(lo, to_code((float)bounds[d] * ratio));
-                    hi = max(hi, to_code((float)bounds[W + d] * ratio));
-                }
-                bounds[d] = (int8_t)lo;
-                bounds[W + d] = (int8_t)hi;
-            }
-        }
-        if (threadIdx.x == 0) *scale = s_new;
     }
     pdl_launch_dependents();
 }
 
-// One thread per 16 codes; a row's K and V pieces lie side by side in the grid.
+// A thread has its 16 channels of a kv head's keys or values and goes over rows: `pieces` threads hold a row (all of K, then
+// V), `together` rows lie side by side in a block, and a thread asks for four of its rows before it writes the first.
+constexpr int kUnpackRows = 4;
+
 template <int W>
-__global__ void __launch_bounds__(256) unpack_q8_kernel(const RowsQ8Dev kv, const uint32_t *slots, const uint32_t *positions,
-                                                        uint4 *k_out, uint4 *v_out, uint32_t rows, uint32_t kv_heads) {
+__global__ void __launch_bounds__(1024) unpack_q8_kernel(const RowsQ8Dev kv, const uint32_t *slots, const uint32_t *positions,
+                                                         uint4 *k_out, uint4 *v_out, uint32_t rows, uint32_t kv_heads, uint32_t pieces,
+                                                         uint32_t together) {
     constexpr uint32_t PIECES = W / 16;
     pdl_wait();
-    const uint32_t per_row = 2 * kv_heads * PIECES;
-    const uint64_t total = (uint64_t)rows * per_row;
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
-        const uint32_t r = i / per_row, rest = i % per_row;
+    const uint32_t sub = threadIdx.x / pieces, rest = blockIdx.y * pieces + threadIdx.x % pieces;
+    if (rest < 2 * kv_heads * PIECES) {
         const bool is_v = rest >= kv_heads * PIECES;
         const uint32_t at = is_v ? rest - kv_heads * PIECES : rest, h = at / PIECES, piece = at % PIECES;
-        const uint32_t pos = positions[r];
-        const uint32_t blk = block_of(kv, slots[r], pos >> kv.shift);
-        uint32_t out[8] = {};
-        if (blk != kNoBlock) {
-            const size_t head = (size_t)blk * kv_heads + h;
-            const float s = (is_v ? kv.v_scale : kv.k_scale)[head];
-            const int8_t *from = (is_v ? kv.v : kv.k) + ((head << kv.shift) + (pos & ((1u << kv.shift) - 1u))) * W + piece * 16;
-            const int4 c = *reinterpret_cast<const int4 *>(from);
-            const int w[4] = {c.x, c.y, c.z, c.w};
+        const int8_t *codes = (is_v ? kv.v : kv.k) + piece * 16;
+        const float *scales = is_v ? kv.v_scale : kv.k_scale;
+        uint4 *to = (is_v ? v_out : k_out) + (size_t)at * 2;
+        const uint32_t r0 = blockIdx.x * together * kUnpackRows + sub;
+        uint32_t slot[kUnpackRows], pos[kUnpackRows];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                out[2 * j] = pack_bf16((float)(int8_t)w[j] * s, (float)(int8_t)(w[j] >> 8) * s);
-                out[2 * j + 1] = pack_bf16((float)(int8_t)(w[j] >> 16) * s, (float)(int8_t)(w[j] >> 24) * s);
+        for (int u = 0; u < kUnpackRows; u++) {
+            const uint32_t r = r0 + u * together;
+            slot[u] = r < rows ? slots[r] : 0;
+            pos[u] = r < rows ? positions[r] : 0;
+        }
+        int4 c[kUnpackRows];
+        float s[kUnpackRows];
+#pragma unroll
+        for (int u = 0; u < kUnpackRows; u++) {
+            const uint32_t blk = r0 + u * together < rows ? block_of(kv, slot[u], pos[u] >> kv.shift) : kNoBlock;
+            c[u] = make_int4(0, 0, 0, 0);
+            s[u] = 0.0f;
+            if (blk != kNoBlock) {
+                const size_t head = (size_t)blk * kv_heads + h;
+                s[u] = scales[head];
+                c[u] = *reinterpret_cast<const int4 *>(codes + ((head << kv.shift) + (pos[u] & ((1u << kv.shift) - 1u))) * W);
             }
         }
-        uint4 *to = (is_v ? v_out : k_out) + ((size_t)r * kv_heads * PIECES + at) * 2;
-        to[0] = make_uint4(out[0], out[1], out[2], out[3]);
-        to[1] = make_uint4(out[4], out[5], out[6], out[7]);
+#pragma unroll
+        for (int u = 0; u < kUnpackRows; u++) {
+            const uint32_t r = r0 + u * together;
+            if (r >= rows) break;
+            const int w[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
+            uint32_t out[8];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                out[2 * j] = pack_bf16((float)(int8_t)w[j] * s[u], (float)(int8_t)(w[j] >> 8) * s[u]);
+                out[2 * j + 1] = pack_bf16((float)(int8_t)(w[j] >> 16) * s[u], (float)(int8_t)(w[j] >> 24) * s[u]);
+            }
+            uint4 *dst = to + (size_t)r * kv_heads * PIECES * 2;
+            dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
+            dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+        }
     }
     pdl_launch_dependents();
 }
 
+// Shared memory of a block of positions: its values in f32, or what the bounds need, whichever is more.
+template <int W, int B>
+constexpr size_t append_smem() {
+    constexpr size_t values = (size_t)B * W * sizeof(float), bounds = (size_t)kAppendWarps * Lanes<W>::TOGETHER * 2 * W * sizeof(float);
+    constexpr size_t least = 2 * kAppendThreads * sizeof(float4);  // one pass
+    return values > bounds ? (values > least ? values : least) : (bounds > least ? bounds : least);
+}
+
+template <int W, int B, Role ROLE>
+cudaError_t launch_append_block(const AppendParams &p, uint32_t grid, bool dependent, cudaStream_t stream) {
+    constexpr size_t smem = ROLE == kQueries ? 0 : append_smem<W, B>();
+    static OncePerDevice configured;
+    if (smem > 48 * 1024 && configured.needs()) {
+        const cudaError_t e = cudaFuncSetAttribute(append_q8_kernel<W, B, ROLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        configured.done();
+    }
+    return launch(append_q8_kernel<W, B, ROLE>, dim3(grid), dim3(kAppendThreads), smem, stream, dependent, p);
+}
+
+template <int W, Role ROLE>
+cudaError_t launch_append(const AppendParams &p, uint32_t block, uint32_t grid, bool dependent, cudaStream_t stream) {
+    return block == 16   ? launch_append_block<W, 16, ROLE>(p, grid, dependent, stream)
+           : block == 32 ? launch_append_block<W, 32, ROLE>(p, grid, dependent, stream)
+                         : launch_append_block<W, 64, ROLE>(p, grid, dependent, stream);
+}
+
+// Many rows: keys and values, which need registers, apart from queries, which need warps; the second launch waits for the
+// first by itself.
 template <int W>
-cudaError_t launch_append(const AppendParams &p, uint32_t block, uint32_t grid, cudaStream_t stream) {
-    return block == 16   ? launch(append_q8_kernel<W, 16>, dim3(grid), dim3(128), 0, stream, pdl_enabled(), p)
-           : block == 32 ? launch(append_q8_kernel<W, 32>, dim3(grid), dim3(128), 0, stream, pdl_enabled(), p)
-                         : launch(append_q8_kernel<W, 64>, dim3(grid), dim3(128), 0, stream, pdl_enabled(), p);
+cudaError_t launch_append(const AppendParams &p, uint32_t kv_ctas, uint32_t q_ctas, cudaStream_t stream) {
+    const uint32_t block = 1u << p.kv.shift;
+    if (p.window < 32) return launch_append<W, kAll>(p, block, kv_ctas + q_ctas, pdl_enabled(), stream);
+    const cudaError_t e = launch_append<W, kKeysValues>(p, block, kv_ctas, pdl_enabled(), stream);
+    return e != cudaSuccess ? e : launch_append_block<W, 16, kQueries>(p, q_ctas, true, stream);
 }
 
 }  // namespace
@@ -360,32 +642,35 @@ int append_q8(const void *qkv, const float *q_norm, const float *k_norm, const f
     p.heads = heads;
     p.kv_heads = kv_heads;
     p.eps = eps;
-    // A step's rows each have a run of their own: a thread block for each.  A prompt's rows come in runs of up to a
-    // block: looking at eight rows saves seven of eight thread blocks that would find no run to start.
-    p.window = rows <= 256 ? 1 : 8;
-    p.per_warp = (uint64_t)rows * heads > 8192 ? 4 : 1;
+    // A step's rows each have a run of their own: eight of them keep the warps of a thread block busy.  A prompt's
+    // rows come in runs of up to a block: looking at 32 rows leaves few thread blocks without a run to start.
+    p.window = rows <= 1024 ? kAppendWarps : 32;
+    // Eight heads a warp compute a row's angles once and have their loads under way together; a step's few heads go to
+    // as many warps as there are.
+    p.per_warp = (uint64_t)rows * heads > 8192 ? 8 : 32 / (width / 8);
     const uint64_t kv_ctas = (uint64_t)ceil_div(rows, p.window) * 2 * kv_heads;
-    const uint64_t q_ctas = ((uint64_t)rows * ceil_div(heads, p.per_warp) + 3) / 4;
+    const uint64_t q_ctas = ((uint64_t)rows * ceil_div(heads, p.per_warp) + kAppendWarps - 1) / kAppendWarps;
     TS_REQUIRE(kv_ctas + q_ctas < 0x7FFFFFFFull, "append (q8): %u rows of %u heads are too many for one launch", rows, heads);
     p.kv_ctas = (uint32_t)kv_ctas;
-    const uint32_t grid = (uint32_t)(kv_ctas + q_ctas), block = 1u << kv.shift;
-    const cudaError_t e = width == 64    ? launch_append<64>(p, block, grid, stream)
-                          : width == 128 ? launch_append<128>(p, block, grid, stream)
-                                         : launch_append<256>(p, block, grid, stream);
+    const cudaError_t e = width == 64    ? launch_append<64>(p, (uint32_t)kv_ctas, (uint32_t)q_ctas, stream)
+                          : width == 128 ? launch_append<128>(p, (uint32_t)kv_ctas, (uint32_t)q_ctas, stream)
+                                         : launch_append<256>(p, (uint32_t)kv_ctas, (uint32_t)q_ctas, stream);
     if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of append (q8) failed: %s", cudaGetErrorString(e));
     return TS_OK;
 }
 
 int unpack_q8(const RowsQ8Dev &kv, const uint32_t *slots, const uint32_t *positions, void *k_out, void *v_out, uint32_t rows,
               uint32_t kv_heads, uint32_t width, cudaStream_t stream) {
-    const uint64_t threads = (uint64_t)rows * 2 * kv_heads * (width / 16);
-    const uint64_t most = (uint64_t)sm_count() * 8 * 4;
-    const uint64_t want = (threads + 255) / 256;
-    const dim3 grid((uint32_t)(want < most ? want : most));
-    const cudaError_t e =
-        width == 64    ? launch(unpack_q8_kernel<64>, grid, dim3(256), 0, stream, pdl_enabled(), kv, slots, positions, (uint4 *)k_out, (uint4 *)v_out, rows, kv_heads)
-        : width == 128 ? launch(unpack_q8_kernel<128>, grid, dim3(256), 0, stream, pdl_enabled(), kv, slots, positions, (uint4 *)k_out, (uint4 *)v_out, rows, kv_heads)
-                       : launch(unpack_q8_kernel<256>, grid, dim3(256), 0, stream, pdl_enabled(), kv, slots, positions, (uint4 *)k_out, (uint4 *)v_out, rows, kv_heads);
+    const uint32_t all = 2 * kv_heads * (width / 16);
+    const uint32_t pieces = min(all, 512u), together = pieces < 256 ? 256 / pieces : 1;
+    const dim3 grid((uint32_t)(((uint64_t)rows + (uint64_t)together * kUnpackRows - 1) / (together * kUnpackRows)), ceil_div(all, pieces));
+    const dim3 block(pieces * together);
+    TS_REQUIRE(grid.y <= 65535, "rows_unpack (q8): %u kv heads are too many", kv_heads);
+    auto go = [&](auto kernel) {
+        return launch(kernel, grid, block, 0, stream, pdl_enabled(), kv, slots, positions, (uint4 *)k_out, (uint4 *)v_out, rows, kv_heads,
+                      pieces, together);
+    };
+    const cudaError_t e = width == 64 ? go(unpack_q8_kernel<64>) : width == 128 ? go(unpack_q8_kernel<128>) : go(unpack_q8_kernel<256>);
     if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of unpack (q8) failed: %s", cudaGetErrorString(e));
     return TS_OK;
 }
