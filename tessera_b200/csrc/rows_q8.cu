@@ -113,7 +113,7 @@ __device__ __forceinline__ void norm_turn(float (&x)[8], bool normed, const floa
         for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
         for (int o = 1; o < Lanes<W>::PER_HEAD; o <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-        const float inv = 1.0f / sqrtf(ss / (float)W + eps);
+        const float inv = rsqrtf(fmaf(ss, 1.0f / (float)W, eps));
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] *= inv * g[i];
     }
@@ -144,7 +144,7 @@ struct AppendParams {
     float eps;
     uint32_t window;    // rows whose runs one thread block looks after
     uint32_t kv_ctas;   // thread blocks [0, kv_ctas) do keys and values, the others queries
-    uint32_t per_warp;  // query heads a warp takes
+    uint32_t per_warp, q_rows;  // query heads, and rows, that a warp takes
 };
 
 __device__ __forceinline__ float min_nan(float a, float b) {  // NaN if either is
@@ -165,7 +165,12 @@ __device__ __forceinline__ uint32_t code_bits(float x, float inv) { return __flo
 __device__ __forceinline__ uint32_t pack_bits(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-__device__ __forceinline__ float code_at(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
+// Code i of four: sign extension by a byte permutation (a conversion straight from a byte runs at a quarter of the rate).
+__device__ __forceinline__ float code_at(uint32_t w, int i) {
+    int v;
+    asm("prmt.b32 %0, %1, 0, %2;" : "=r"(v) : "r"(w), "r"(i | (i | 8) * 0x1110));  // bit 3 of a selector: the sign
+    return __int2float_rn(v);
+}
 
 // A block's scale before and after, and how its codes follow.
 struct Scales {
@@ -173,8 +178,8 @@ struct Scales {
     bool fresh;
 };
 
-__device__ __forceinline__ Scales grow(const float *scale, bool fresh, float most) {
-    const float old = fresh ? 0.0f : *scale;
+__device__ __forceinline__ Scales grow(float was, bool fresh, float most) {
+    const float old = fresh ? 0.0f : was;
     Scales s;
     s.now = fmaxf(old, fmaxf(most / 127.0f, kScaleFloor));
     s.inv = 1.0f / s.now;
@@ -212,9 +217,11 @@ __device__ __forceinline__ void follow_row(int8_t *row, uint32_t i, float ratio)
 // Bounds of four channels from the least and the largest new value (rounding keeps their order), joined with those the
 // block had unless it is fresh.
 template <int W>
-__device__ __forceinline__ void write_bounds(int8_t *bounds, uint32_t first, const float *low, const float *high, const Scales &sc) {
+__device__ __forceinline__ void write_bounds(int8_t *bounds, uint32_t first, uint32_t was_lo, uint32_t was_hi, const float *low,
+                                             const float *high, const Scales &sc) {
     uint32_t *lo = reinterpret_cast<uint32_t *>(bounds + first), *hi = reinterpret_cast<uint32_t *>(bounds + W + first);
-    const uint32_t was_lo = sc.fresh ? 0 : follow(*lo, sc.ratio), was_hi = sc.fresh ? 0 : follow(*hi, sc.ratio);
+    was_lo = follow(was_lo, sc.ratio);
+    was_hi = follow(was_hi, sc.ratio);
     uint32_t a[4], b[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -243,41 +250,64 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
     const uint32_t per_row = p.heads + 2 * p.kv_heads;
     __shared__ uint64_t sm_turns[W / 2];  // each pair's, computed once: its 64-bit arithmetic is slow
     pdl_wait();
+    const bool queries = ROLE == kQueries || (ROLE == kAll && blockIdx.x >= p.kv_ctas);
+    // ---- keys, values: the runs that begin among this block's rows, at most 32 of them, one a lane ----
+    const uint32_t units = 2 * p.kv_heads, unit = blockIdx.x % units;
+    const uint32_t r0 = blockIdx.x / units * p.window, r1 = min(p.rows, r0 + p.window);
+    uint32_t slot = 0, blk_pos = 0xFFFFFFFFu, starts = 0;
+    if (!queries) {
+        if (r0 + lane < r1) {
+            slot = p.slots[r0 + lane];
+            blk_pos = p.positions[r0 + lane] >> p.kv.shift;
+        }
+        uint32_t slot_was = __shfl_up_sync(0xFFFFFFFFu, slot, 1), pos_was = __shfl_up_sync(0xFFFFFFFFu, blk_pos, 1);
+        if (lane == 0 && r0 > 0) {
+            slot_was = p.slots[r0 - 1];
+            pos_was = p.positions[r0 - 1] >> p.kv.shift;
+        }
+        const bool begins = r0 + lane < r1 && ((r0 == 0 && lane == 0) || slot != slot_was || blk_pos != pos_was);
+        starts = __ballot_sync(0xFFFFFFFFu, begins);
+        if (starts == 0) {
+            pdl_launch_dependents();
+            return;
+        }
+    }
     if (threadIdx.x < W / 2) sm_turns[threadIdx.x] = turns_of(p.inv_freq[threadIdx.x]);
     __syncthreads();
     uint64_t turns[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) turns[e] = sm_turns[4 * li + e];
-    if (ROLE == kQueries || (ROLE == kAll && blockIdx.x >= p.kv_ctas)) {
-        // ---- queries: a warp takes up to `per_warp` heads of a row, T of them side by side ----
+    if (queries) {
+        // ---- queries: a warp takes up to `per_warp` heads of `q_rows` rows, T of them side by side ----
         const uint32_t parts = (p.heads + p.per_warp - 1) / p.per_warp;
-        const uint64_t unit = (uint64_t)(blockIdx.x - (ROLE == kAll ? p.kv_ctas : 0)) * kAppendWarps + warp;
-        if (unit < (uint64_t)p.rows * parts) {
-            const uint32_t r = unit / parts, h0 = unit % parts * p.per_warp, h1 = min(p.heads, h0 + p.per_warp);
+        const uint32_t job = (blockIdx.x - (ROLE == kAll ? p.kv_ctas : 0)) * kAppendWarps + warp;
+        const uint32_t h0 = job % parts * p.per_warp, h1 = min(p.heads, h0 + p.per_warp);
+        const uint32_t first = job / parts * p.q_rows;
+        float g[8];
+        load_gains<W>(p.q_norm, li, g);
+        for (uint32_t r = first; r < min(first + p.q_rows, p.rows); r++) {
             const uint32_t pos = p.positions[r];
-            float sn[4], cs[4], g[8];
             constexpr int PASSES = 8 / T;
+            const uint16_t *from = p.qkv + ((size_t)r * per_row + h0 + which) * W;
+            uint16_t *to = p.q_out + ((size_t)r * p.heads + h0 + which) * W + 4 * li;
             Raw raw[PASSES];
 #pragma unroll
             for (int k = 0; k < PASSES; k++) {
-                const uint32_t h = h0 + k * T + which;
                 raw[k] = {make_uint2(0, 0), make_uint2(0, 0)};
-                if (h < h1) raw[k] = load_head<W>(p.qkv + ((size_t)r * per_row + h) * W, li);
+                if (h0 + k * T + which < h1) raw[k] = load_head<W>(from + k * T * W, li);
             }
-            load_gains<W>(p.q_norm, li, g);
+            float sn[4], cs[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) sine_cosine(pos, turns[e], &sn[e], &cs[e]);
 #pragma unroll
             for (int k = 0; k < PASSES; k++) {
                 if (h0 + k * T >= h1) break;
-                const uint32_t h = h0 + k * T + which;
                 float x[8];
                 widen(raw[k], x);
                 norm_turn<W>(x, p.q_norm != nullptr, g, sn, cs, p.eps);
-                if (h < h1) {
-                    uint16_t *dst = p.q_out + ((size_t)r * p.heads + h) * W + 4 * li;
-                    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-                    *reinterpret_cast<uint2 *>(dst + W / 2) = make_uint2(pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+                if (h0 + k * T + which < h1) {
+                    *reinterpret_cast<uint2 *>(to + k * T * W) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+                    *reinterpret_cast<uint2 *>(to + k * T * W + W / 2) = make_uint2(pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
                 }
             }
         }
@@ -285,33 +315,32 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
         return;
     }
 
-    __shared__ int src[B];  // long runs: the row that writes each position of the block, or -1
-    __shared__ uint32_t stop;
-    __shared__ float sm_max[kAppendWarps];
+    // Long runs belong to a team of warps: all four for 64 positions, else two.
+    constexpr int TEAM = B == 64 ? 4 : 2, TEAMS = kAppendWarps / TEAM, STEP = TEAM * T, PASSES = B > STEP ? B / STEP : 1;
+    const uint32_t team = warp / TEAM, tid = threadIdx.x - team * TEAM * 32;  // the thread's number in its team
+    const uint32_t mine = tid / L;                                            // it has positions mine + STEP u
+    auto team_sync = [&] {
+        if (TEAMS == 1) __syncthreads();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(TEAM * 32) : "memory");
+    };
+    __shared__ int all_src[TEAMS][B];  // the row that writes each position of the block, or -1
+    __shared__ uint32_t all_stop[TEAMS];
+    __shared__ uint32_t sm_max[kAppendWarps];
+    __shared__ float2 sm_step[W / 2];  // sine and cosine of STEP positions
+    int *src = all_src[team];
+    uint32_t &stop = all_stop[team];
     // Long runs: a thread's prepared values wait here for the scale (in registers they would leave room for 12 warps an SM,
     // 54 us for 8165 rows), then the block's bounds are put together in the same place.
-    extern __shared__ __align__(16) float4 kept[];  // [passes][2][threads]
-    const uint32_t units = 2 * p.kv_heads, unit = blockIdx.x % units;
+    extern __shared__ __align__(16) float4 all_kept[];  // [teams][passes][2][threads]
+    float4 *kept = all_kept + team * (PASSES * 2 * TEAM * 32);
     const bool is_v = unit >= p.kv_heads;
     const uint32_t h = is_v ? unit - p.kv_heads : unit;
     const uint16_t *heads = p.qkv + (size_t)(p.heads + unit) * W;  // this unit's head of row 0
     const bool bounded = !is_v && p.kv.bounds != nullptr, normed = !is_v && p.k_norm != nullptr;
-    const uint32_t r0 = blockIdx.x / units * p.window, r1 = min(p.rows, r0 + p.window);
-    // ---- the runs that begin among rows [r0, r1), at most 32 of them, one a lane ----
-    uint32_t slot = 0, blk_pos = 0xFFFFFFFFu;
-    if (r0 + lane < r1) {
-        slot = p.slots[r0 + lane];
-        blk_pos = p.positions[r0 + lane] >> p.kv.shift;
-    }
-    uint32_t slot_was = __shfl_up_sync(0xFFFFFFFFu, slot, 1), pos_was = __shfl_up_sync(0xFFFFFFFFu, blk_pos, 1);
-    if (lane == 0 && r0 > 0) {
-        slot_was = p.slots[r0 - 1];
-        pos_was = p.positions[r0 - 1] >> p.kv.shift;
-    }
-    const bool begins = r0 + lane < r1 && ((r0 == 0 && lane == 0) || slot != slot_was || blk_pos != pos_was);
-    uint32_t starts = __ballot_sync(0xFFFFFFFFu, begins);
     float g[8];
-    if (starts) load_gains<W>(normed ? p.k_norm : nullptr, li, g);
+    load_gains<W>(normed ? p.k_norm : nullptr, li, g);
+    if (!is_v && threadIdx.x < W / 2) sine_cosine(STEP, sm_turns[threadIdx.x], &sm_step[threadIdx.x].x, &sm_step[threadIdx.x].y);
+    __syncthreads();
     for (uint32_t turn = 0; starts; turn++) {
         const uint32_t first = __ffs(starts) - 1;
         starts &= starts - 1;
@@ -329,10 +358,16 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
         float *scale = (is_v ? p.kv.v_scale : p.kv.k_scale) + at;
         int8_t *codes = (is_v ? p.kv.v : p.kv.k) + at * B * W;
         int8_t *bounds = p.kv.bounds + at * 2 * W;
+        const float was = *scale;  // asked for before it is needed
         if (n <= kShort) {
             // ---- a warp's run ----
             if (turn % kAppendWarps != warp) continue;
             constexpr int PASSES = kShort / T > 0 ? kShort / T : 1;
+            uint32_t held[4] = {};  // the bounds of this lane's channels
+            if (bounded && which == 0) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) held[i] = *reinterpret_cast<const uint32_t *>(bounds + (i & 1) * W + (i >> 1) * (W / 2) + 4 * li);
+            }
             uint64_t written = 0;
             for (uint32_t k = 0; k < n; k++) written |= 1ull << (p.positions[s + k] & (B - 1));
             float x[PASSES][8], low[8], high[8];
@@ -372,7 +407,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
             for (int e = 0; e < 8; e++)
                 if (high[e] >= low[e]) most = fmaxf(most, fmaxf(fabsf(low[e]), fabsf(high[e])));
             most = warp_max(most);
-            const Scales sc = grow(scale, written & 1, most);
+            const Scales sc = grow(was, written & 1, most);
 #pragma unroll
             for (int k = 0; k < PASSES; k++)
                 if (row[k]) write_row<W>(row[k], li, x[k], sc.inv);
@@ -388,44 +423,103 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
                         high[e] = fmaxf(high[e], __shfl_xor_sync(0xFFFFFFFFu, high[e], o));
                     }
                 if (which == 0) {
-                    write_bounds<W>(bounds, 4 * li, low, high, sc);
-                    write_bounds<W>(bounds, W / 2 + 4 * li, low + 4, high + 4, sc);
+                    write_bounds<W>(bounds, 4 * li, held[0], held[1], low, high, sc);
+                    write_bounds<W>(bounds, W / 2 + 4 * li, held[2], held[3], low + 4, high + 4, sc);
                 }
             }
             __syncwarp();  // every lane has read the old scale
             if (lane == 0) *scale = sc.now;
             continue;
         }
-        // ---- a thread block's run: which row writes which position ----
-        constexpr int STEP = kAppendWarps * T, PASSES = B > STEP ? B / STEP : 1;  // positions warp * T + which + STEP u
-        const uint32_t mine = warp * T + which;
-        __syncthreads();
-        if (threadIdx.x < B) src[threadIdx.x] = -1;
-        if (threadIdx.x == 0) stop = p.rows;
-        __syncthreads();
-        for (uint32_t base = s; base < p.rows; base += kAppendThreads) {
-            const uint32_t i = base + threadIdx.x;
+        // ---- a team's run: which row writes which position ----
+        if (turn % TEAMS != team) continue;
+        team_sync();
+        if (tid < B) src[tid] = -1;
+        if (tid == 0) stop = p.rows;
+        team_sync();
+        for (uint32_t base = s; base < p.rows; base += TEAM * 32) {
+            const uint32_t i = base + tid;
             const bool in = same(i);
             if (!in && i < p.rows) atomicMin(&stop, i);
-            __syncthreads();
+            team_sync();
             const uint32_t end = stop;  // later passes only bring it down to rows past this one's
             if (in && i < end) atomicMax(&src[p.positions[i] & (B - 1)], (int)i);
-            if (end < base + kAppendThreads) break;
+            if (end < base + TEAM * 32) break;
         }
-        __syncthreads();
+        team_sync();
         auto row_of = [&](int u) { return mine + STEP * u < B ? src[mine + STEP * u] : -1; };
+        if (is_v) {
+            // ---- values: bf16 as they come, kept as such; magnitudes compare as whole numbers ----
+            Raw raw[PASSES];
+            uint32_t top = 0;
+#pragma unroll
+            for (int u = 0; u < PASSES; u++) {
+                const int row = row_of(u);
+                raw[u] = {make_uint2(0, 0), make_uint2(0, 0)};
+                if (row >= 0) raw[u] = load_head<W>(heads + (size_t)row * per_row * W, li);
+            }
+#pragma unroll
+            for (int u = 0; u < PASSES; u++) {
+                top = __vmaxu2(top, __vmaxu2(raw[u].a.x & 0x7FFF7FFFu, raw[u].a.y & 0x7FFF7FFFu));
+                top = __vmaxu2(top, __vmaxu2(raw[u].b.x & 0x7FFF7FFFu, raw[u].b.y & 0x7FFF7FFFu));
+            }
+            top = __reduce_max_sync(0xFFFFFFFFu, max(top & 0xFFFFu, top >> 16));
+            if (lane == 0) sm_max[warp] = top;
+            team_sync();
+            top = sm_max[team * TEAM];
+#pragma unroll
+            for (int w = 1; w < TEAM; w++) top = max(top, sm_max[team * TEAM + w]);
+            const bool wild = top > 0x7F7Fu;  // an infinity or NaN among them: the largest of the others counts, see `tame`
+            float most = __uint_as_float(top << 16);
+            if (wild) {
+                most = 0.0f;
+#pragma unroll
+                for (int u = 0; u < PASSES; u++) {
+                    float x[8];
+                    widen(raw[u], x);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(tame(x[e])));
+                }
+                top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
+                team_sync();
+                if (lane == 0) sm_max[warp] = top;
+                team_sync();
+#pragma unroll
+                for (int w = 0; w < TEAM; w++) most = fmaxf(most, __uint_as_float(sm_max[team * TEAM + w]));
+            }
+            const Scales sc = grow(was, src[0] >= 0, most);
+#pragma unroll
+            for (int u = 0; u < PASSES; u++) {
+                const uint32_t i = mine + STEP * u;
+                if (row_of(u) >= 0) {
+                    float x[8];
+                    widen(raw[u], x);
+                    if (wild) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = tame(x[e]);
+                    }
+                    write_row<W>(codes + i * W, li, x, sc.inv);
+                } else if (i < B && sc.ratio < 1.0f) {
+                    follow_row<W>(codes + i * W, li, sc.ratio);
+                }
+            }
+            team_sync();  // every thread has read the old scale
+            if (tid == 0) *scale = sc.now;
+            continue;
+        }
+        // ---- keys ----
+        uint32_t held_lo = 0, held_hi = 0;  // the bounds of channels 4 tid ..
+        if (bounded && tid < W / 4) {
+            held_lo = *reinterpret_cast<const uint32_t *>(bounds + 4 * tid);
+            held_hi = *reinterpret_cast<const uint32_t *>(bounds + W + 4 * tid);
+        }
         // Least and largest of each of the lane's channels; NaN stays, so that one comparison finds what is to be tamed.
         float low[8], high[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) low[e] = INFINITY, high[e] = -INFINITY;
-        float sn[4], cs[4], step_s[4], step_c[4];
-        if (!is_v) {
+        float sn[4], cs[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                sine_cosine((b << p.kv.shift) + mine, turns[e], &sn[e], &cs[e]);
-                sine_cosine(STEP, turns[e], &step_s[e], &step_c[e]);
-            }
-        }
+        for (int e = 0; e < 4; e++) sine_cosine((b << p.kv.shift) + mine, turns[e], &sn[e], &cs[e]);
         bool any = false;
         constexpr int GROUP = PASSES < 4 ? PASSES : 4;  // passes whose loads are under way together
         for (int u0 = 0; u0 < PASSES; u0 += GROUP) {
@@ -440,15 +534,14 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
             for (int k = 0; k < GROUP; k++) {
                 float x[8];
                 widen(raw[k], x);
-                if (!is_v) {
-                    norm_turn<W>(x, normed, g, sn, cs, p.eps);
-                    // the next pass is STEP positions on: a turn by a fixed angle (at most 15 of them, 2^-24 each)
+                norm_turn<W>(x, normed, g, sn, cs, p.eps);
+                // the next pass is STEP positions on: a turn by a fixed angle (at most 15 of them, 2^-24 each)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float s0 = sn[e], c0 = cs[e];
-                        cs[e] = c0 * step_c[e] - s0 * step_s[e];
-                        sn[e] = s0 * step_c[e] + c0 * step_s[e];
-                    }
+                for (int e = 0; e < 4; e++) {
+                    const float2 by = sm_step[4 * li + e];
+                    const float s0 = sn[e], c0 = cs[e];
+                    cs[e] = c0 * by.y - s0 * by.x;
+                    sn[e] = s0 * by.y + c0 * by.x;
                 }
                 if (row_of(u0 + k) >= 0) {
                     any = true;
@@ -458,8 +551,8 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
                         high[e] = max_nan(high[e], x[e]);
                     }
                 }
-                kept[(2 * (u0 + k)) * kAppendThreads + threadIdx.x] = make_float4(x[0], x[1], x[2], x[3]);
-                kept[(2 * (u0 + k) + 1) * kAppendThreads + threadIdx.x] = make_float4(x[4], x[5], x[6], x[7]);
+                kept[(2 * (u0 + k)) * (TEAM * 32) + tid] = make_float4(x[0], x[1], x[2], x[3]);
+                kept[(2 * (u0 + k) + 1) * (TEAM * 32) + tid] = make_float4(x[4], x[5], x[6], x[7]);
             }
         }
         float most = 0.0f;
@@ -472,7 +565,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
             for (int u = 0; u < PASSES; u++)
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
-                    float4 &v = kept[(2 * u + half) * kAppendThreads + threadIdx.x];
+                    float4 &v = kept[(2 * u + half) * (TEAM * 32) + tid];
                     float x[4] = {tame(v.x), tame(v.y), tame(v.z), tame(v.w)};
                     v = make_float4(x[0], x[1], x[2], x[3]);
                     if (row_of(u) < 0) continue;
@@ -485,25 +578,26 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
                 }
         }
         most = warp_max(any ? most : 0.0f);
-        if (lane == 0) sm_max[warp] = most;
-        __syncthreads();
-        most = fmaxf(fmaxf(sm_max[0], sm_max[1]), fmaxf(sm_max[2], sm_max[3]));
-        const Scales sc = grow(scale, src[0] >= 0, most);
+        if (lane == 0) sm_max[warp] = __float_as_uint(most);
+        team_sync();
+#pragma unroll
+        for (int w = 0; w < TEAM; w++) most = fmaxf(most, __uint_as_float(sm_max[team * TEAM + w]));
+        const Scales sc = grow(was, src[0] >= 0, most);
 #pragma unroll 2
         for (int u = 0; u < PASSES; u++) {
             const uint32_t i = mine + STEP * u;
             if (row_of(u) >= 0) {
-                const float4 v = kept[(2 * u) * kAppendThreads + threadIdx.x], w = kept[(2 * u + 1) * kAppendThreads + threadIdx.x];
+                const float4 v = kept[(2 * u) * (TEAM * 32) + tid], w = kept[(2 * u + 1) * (TEAM * 32) + tid];
                 const float x[8] = {v.x, v.y, v.z, v.w, w.x, w.y, w.z, w.w};
                 write_row<W>(codes + i * W, li, x, sc.inv);
             } else if (i < B && sc.ratio < 1.0f) {
                 follow_row<W>(codes + i * W, li, sc.ratio);
             }
         }
-        __syncthreads();  // every thread has read the old scale and its kept values
-        if (threadIdx.x == 0) *scale = sc.now;
+        team_sync();  // every thread has read the old scale and its kept values
+        if (tid == 0) *scale = sc.now;
         if (bounded) {
-            // lanes that hold the same channels meet in shared memory: [kAppendWarps * T][low, high][W]
+            // lanes that hold the same channels meet in shared memory: [STEP][low, high][W]
             float *sm = reinterpret_cast<float *>(kept) + mine * 2 * W;
 #pragma unroll
             for (int half = 0; half < 2; half++) {
@@ -511,9 +605,9 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
                 *reinterpret_cast<float4 *>(sm + d) = make_float4(low[4 * half], low[4 * half + 1], low[4 * half + 2], low[4 * half + 3]);
                 *reinterpret_cast<float4 *>(sm + W + d) = make_float4(high[4 * half], high[4 * half + 1], high[4 * half + 2], high[4 * half + 3]);
             }
-            __syncthreads();
-            if (threadIdx.x < W / 4) {
-                const float *all = reinterpret_cast<const float *>(kept) + 4 * threadIdx.x;
+            team_sync();
+            if (tid < W / 4) {
+                const float *all = reinterpret_cast<const float *>(kept) + 4 * tid;
                 float lo[4], hi[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) lo[e] = INFINITY, hi[e] = -INFINITY;
@@ -523,76 +617,76 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
                     lo[0] = fminf(lo[0], l.x); lo[1] = fminf(lo[1], l.y); lo[2] = fminf(lo[2], l.z); lo[3] = fminf(lo[3], l.w);
                     hi[0] = fmaxf(hi[0], m.x); hi[1] = fmaxf(hi[1], m.y); hi[2] = fmaxf(hi[2], m.z); hi[3] = fmaxf(hi[3], m.w);
                 }
-                write_bounds<W>(bounds, 4 * threadIdx.x, lo, hi, sc);
+                write_bounds<W>(bounds, 4 * tid, held_lo, held_hi, lo, hi, sc);
             }
         }
     }
     pdl_launch_dependents();
 }
 
-// A thread has its 16 channels of a kv head's keys or values and goes over rows: `pieces` threads hold a row (all of K, then
-// V), `together` rows lie side by side in a block, and a thread asks for four of its rows before it writes the first.
-constexpr int kUnpackRows = 4;
-
-template <int W>
-__global__ void __launch_bounds__(1024) unpack_q8_kernel(const RowsQ8Dev kv, const uint32_t *slots, const uint32_t *positions,
-                                                         uint4 *k_out, uint4 *v_out, uint32_t rows, uint32_t kv_heads, uint32_t pieces,
-                                                         uint32_t together) {
-    constexpr uint32_t PIECES = W / 16;
+// A thread has its 8 channels of a kv head's keys or values (a warp's stores then fill whole lines) and goes over ROWS rows: `pieces` threads hold a row (all of K,
+// then V), `together` rows lie side by side. The block first looks all its rows up, then every thread asks for the codes
+// of all its rows before it writes the first.
+template <int W, int ROWS>
+__global__ void __launch_bounds__(512) unpack_q8_kernel(const RowsQ8Dev kv, const uint32_t *slots, const uint32_t *positions,
+                                                        uint4 *k_out, uint4 *v_out, uint32_t rows, uint32_t kv_heads, uint32_t pieces,
+                                                        uint32_t together) {
+    constexpr uint32_t PIECES = W / 8;
+    __shared__ uint2 place[256];  // block and position in it
     pdl_wait();
-    const uint32_t sub = threadIdx.x / pieces, rest = blockIdx.y * pieces + threadIdx.x % pieces;
+    const uint32_t first = blockIdx.x * together * ROWS;
+    for (uint32_t i = threadIdx.x; i < together * ROWS; i += blockDim.x) {
+        uint2 at = make_uint2(kNoBlock, 0);
+        if (first + i < rows) {
+            const uint32_t pos = positions[first + i];
+            at = make_uint2(block_of(kv, slots[first + i], pos >> kv.shift), pos & ((1u << kv.shift) - 1u));
+        }
+        place[i] = at;
+    }
+    __syncthreads();
+    const uint32_t sub = threadIdx.x / pieces, rest = blockIdx.y * pieces + threadIdx.x - sub * pieces;
     if (rest < 2 * kv_heads * PIECES) {
         const bool is_v = rest >= kv_heads * PIECES;
         const uint32_t at = is_v ? rest - kv_heads * PIECES : rest, h = at / PIECES, piece = at % PIECES;
-        const int8_t *codes = (is_v ? kv.v : kv.k) + piece * 16;
+        const int8_t *codes = (is_v ? kv.v : kv.k) + piece * 8;
         const float *scales = is_v ? kv.v_scale : kv.k_scale;
-        uint4 *to = (is_v ? v_out : k_out) + (size_t)at * 2;
-        const uint32_t r0 = blockIdx.x * together * kUnpackRows + sub;
-        uint32_t slot[kUnpackRows], pos[kUnpackRows];
+        uint4 *to = (is_v ? v_out : k_out) + ((size_t)(first + sub) * kv_heads * PIECES + at);
+        const size_t stride = (size_t)together * kv_heads * PIECES;
+        uint2 c[ROWS];
+        float s[ROWS];
 #pragma unroll
-        for (int u = 0; u < kUnpackRows; u++) {
-            const uint32_t r = r0 + u * together;
-            slot[u] = r < rows ? slots[r] : 0;
-            pos[u] = r < rows ? positions[r] : 0;
-        }
-        int4 c[kUnpackRows];
-        float s[kUnpackRows];
-#pragma unroll
-        for (int u = 0; u < kUnpackRows; u++) {
-            const uint32_t blk = r0 + u * together < rows ? block_of(kv, slot[u], pos[u] >> kv.shift) : kNoBlock;
-            c[u] = make_int4(0, 0, 0, 0);
+        for (int u = 0; u < ROWS; u++) {
+            const uint2 where = place[sub + u * together];
+            c[u] = make_uint2(0, 0);
             s[u] = 0.0f;
-            if (blk != kNoBlock) {
-                const size_t head = (size_t)blk * kv_heads + h;
+            if (where.x != kNoBlock) {
+                const size_t head = (size_t)where.x * kv_heads + h;
                 s[u] = scales[head];
-                c[u] = *reinterpret_cast<const int4 *>(codes + ((head << kv.shift) + (pos[u] & ((1u << kv.shift) - 1u))) * W);
+                c[u] = *reinterpret_cast<const uint2 *>(codes + ((head << kv.shift) + where.y) * W);
             }
         }
 #pragma unroll
-        for (int u = 0; u < kUnpackRows; u++) {
-            const uint32_t r = r0 + u * together;
-            if (r >= rows) break;
-            const int w[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
-            uint32_t out[8];
+        for (int u = 0; u < ROWS; u++) {
+            if (first + sub + u * together >= rows) break;
+            const uint32_t w[2] = {c[u].x, c[u].y};
+            uint32_t out[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                out[2 * j] = pack_bf16((float)(int8_t)w[j] * s[u], (float)(int8_t)(w[j] >> 8) * s[u]);
-                out[2 * j + 1] = pack_bf16((float)(int8_t)(w[j] >> 16) * s[u], (float)(int8_t)(w[j] >> 24) * s[u]);
+            for (int j = 0; j < 2; j++) {
+                out[2 * j] = pack_bf16(code_at(w[j], 0) * s[u], code_at(w[j], 1) * s[u]);
+                out[2 * j + 1] = pack_bf16(code_at(w[j], 2) * s[u], code_at(w[j], 3) * s[u]);
             }
-            uint4 *dst = to + (size_t)r * kv_heads * PIECES * 2;
-            dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
-            dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+            to[u * stride] = make_uint4(out[0], out[1], out[2], out[3]);
         }
     }
     pdl_launch_dependents();
 }
 
-// Shared memory of a block of positions: its values in f32, or what the bounds need, whichever is more.
+// Shared memory of the teams: a block of positions' values in f32 each, or what the bounds need, which is less.
 template <int W, int B>
 constexpr size_t append_smem() {
-    constexpr size_t values = (size_t)B * W * sizeof(float), bounds = (size_t)kAppendWarps * Lanes<W>::TOGETHER * 2 * W * sizeof(float);
-    constexpr size_t least = 2 * kAppendThreads * sizeof(float4);  // one pass
-    return values > bounds ? (values > least ? values : least) : (bounds > least ? bounds : least);
+    constexpr int team = B == 64 ? 4 : 2, step = team * Lanes<W>::TOGETHER, passes = B > step ? B / step : 1;
+    static_assert(passes * team * 32 * 8 >= step * 2 * W, "the bounds fit where the values were");
+    return (size_t)(kAppendWarps / team) * passes * 2 * team * 32 * sizeof(float4);
 }
 
 template <int W, int B, Role ROLE>
@@ -645,12 +739,14 @@ int append_q8(const void *qkv, const float *q_norm, const float *k_norm, const f
     // A step's rows each have a run of their own: eight of them keep the warps of a thread block busy.  A prompt's
     // rows come in runs of up to a block: looking at 32 rows leaves few thread blocks without a run to start.
     p.window = rows <= 1024 ? kAppendWarps : 32;
-    // Eight heads a warp compute a row's angles once and have their loads under way together; a step's few heads go to
-    // as many warps as there are.
-    p.per_warp = (uint64_t)rows * heads > 8192 ? 8 : 32 / (width / 8);
+    // Eight heads a warp compute a row's angles once and have their loads under way together, four rows share what a warp
+    // sets up; a step's few heads go to as many warps as there are.
+    const bool many = (uint64_t)rows * heads > 32768;
+    p.per_warp = many ? 8 : 32 / (width / 8);
+    p.q_rows = many ? 4 : 1;
     const uint64_t kv_ctas = (uint64_t)ceil_div(rows, p.window) * 2 * kv_heads;
-    const uint64_t q_ctas = ((uint64_t)rows * ceil_div(heads, p.per_warp) + kAppendWarps - 1) / kAppendWarps;
-    TS_REQUIRE(kv_ctas + q_ctas < 0x7FFFFFFFull, "append (q8): %u rows of %u heads are too many for one launch", rows, heads);
+    const uint64_t q_ctas = ((uint64_t)ceil_div(rows, p.q_rows) * ceil_div(heads, p.per_warp) + kAppendWarps - 1) / kAppendWarps;
+    TS_REQUIRE(kv_ctas + q_ctas < 0x1FFFFFFFull, "append (q8): %u rows of %u heads are too many for one launch", rows, heads);
     p.kv_ctas = (uint32_t)kv_ctas;
     const cudaError_t e = width == 64    ? launch_append<64>(p, (uint32_t)kv_ctas, (uint32_t)q_ctas, stream)
                           : width == 128 ? launch_append<128>(p, (uint32_t)kv_ctas, (uint32_t)q_ctas, stream)
@@ -661,16 +757,20 @@ int append_q8(const void *qkv, const float *q_norm, const float *k_norm, const f
 
 int unpack_q8(const RowsQ8Dev &kv, const uint32_t *slots, const uint32_t *positions, void *k_out, void *v_out, uint32_t rows,
               uint32_t kv_heads, uint32_t width, cudaStream_t stream) {
-    const uint32_t all = 2 * kv_heads * (width / 16);
+    const uint32_t all = 2 * kv_heads * (width / 8);
     const uint32_t pieces = min(all, 512u), together = pieces < 256 ? 256 / pieces : 1;
-    const dim3 grid((uint32_t)(((uint64_t)rows + (uint64_t)together * kUnpackRows - 1) / (together * kUnpackRows)), ceil_div(all, pieces));
-    const dim3 block(pieces * together);
+    // Eight rows a thread once that still leaves a block for every place on the GPU.
+    const bool many = (uint64_t)rows * all >= (uint64_t)sm_count() * 2048 * 8;
+    const uint32_t each = together * (many ? 8 : 2);
+    const dim3 grid((uint32_t)(((uint64_t)rows + each - 1) / each), ceil_div(all, pieces)), block(pieces * together);
     TS_REQUIRE(grid.y <= 65535, "rows_unpack (q8): %u kv heads are too many", kv_heads);
     auto go = [&](auto kernel) {
         return launch(kernel, grid, block, 0, stream, pdl_enabled(), kv, slots, positions, (uint4 *)k_out, (uint4 *)v_out, rows, kv_heads,
                       pieces, together);
     };
-    const cudaError_t e = width == 64 ? go(unpack_q8_kernel<64>) : width == 128 ? go(unpack_q8_kernel<128>) : go(unpack_q8_kernel<256>);
+    const cudaError_t e = width == 64    ? (many ? go(unpack_q8_kernel<64, 8>) : go(unpack_q8_kernel<64, 2>))
+                          : width == 128 ? (many ? go(unpack_q8_kernel<128, 8>) : go(unpack_q8_kernel<128, 2>))
+                                         : (many ? go(unpack_q8_kernel<256, 8>) : go(unpack_q8_kernel<256, 2>));
     if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of unpack (q8) failed: %s", cudaGetErrorString(e));
     return TS_OK;
 }

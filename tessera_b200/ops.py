@@ -260,8 +260,9 @@ def _at(t, dtype, count, dev, name):
 
 
 def _kept_q8(kept: Kept, dev) -> TsKept:
-    if kept.table is not None:
-        _at(kept.table, torch.int32, kept.table.numel(), dev, "page table")
+    t = kept.table
+    if t is not None and (t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous()):
+        _refuse(f"page table: expected contiguous {torch.int32} on cuda:{dev}, got {t.dtype} on {t.device}")
     return kept.c()
 
 
@@ -273,7 +274,7 @@ def _q8_workspace(which: str, *sizes) -> int:
 def _scratch(nbytes: int, like) -> torch.Tensor | None:
     """Scratch of one call, from the caching allocator: eager calls reuse it in stream order, a captured call keeps its
     own in the graph's pool, so that two graphs never share it."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def qk_norm_rope_append_q8(qkv, q_norm, k_norm, inv_freq, slots, positions, kv: RowsQ8, kept: Kept, heads: int, *, eps: float,
@@ -283,9 +284,10 @@ def qk_norm_rope_append_q8(qkv, q_norm, k_norm, inv_freq, slots, positions, kv: 
     dev, stream = _q8_stream(kv)
     rows = slots.numel()
     _, kv_heads, _, width = kv.k.shape
+    a_qkv = _at(qkv, torch.bfloat16, rows * (heads + 2 * kv_heads) * width, dev, "qkv")
     if out is None:
-        out = torch.empty((rows, heads, width), dtype=torch.bfloat16, device=qkv.device)
-    args = (_at(qkv, torch.bfloat16, rows * (heads + 2 * kv_heads) * width, dev, "qkv"), _at(q_norm, torch.float32, width, dev, "q_norm"),
+        out = qkv.new_empty((rows, heads, width))
+    args = (a_qkv, _at(q_norm, torch.float32, width, dev, "q_norm"),
             _at(k_norm, torch.float32, width, dev, "k_norm"), _at(inv_freq, torch.float32, width // 2, dev, "inv_freq"),
             _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions"),
             _at(out, torch.bfloat16, rows * heads * width, dev, "out"))
@@ -299,7 +301,7 @@ def rows_unpack_q8(kv: RowsQ8, slots, positions, kept: Kept):
     dev, stream = _q8_stream(kv)
     rows = slots.numel()
     _, kv_heads, _, width = kv.k.shape
-    k_out = torch.empty((rows, kv_heads, width), dtype=torch.bfloat16, device=kv.k.device)
+    k_out = kv.k.new_empty((rows, kv_heads, width), dtype=torch.bfloat16)
     v_out = torch.empty_like(k_out)
     args = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
     if rows:
@@ -320,9 +322,12 @@ def attend_rows_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, *, sc
     """Ragged causal attention over 8-bit kept rows, q and result bf16 [rows, heads, width]: ts_attend_rows_q8."""
     dev, stream = _q8_stream(kv)
     rows, heads, kv_heads, _, width = _heads_of(q, kv)
+    a_q = _at(q, torch.bfloat16, rows * heads * width, dev, "q")
     if out is None:
         out = torch.empty_like(q)
-    a_q, a_out = (_at(t, torch.bfloat16, rows * heads * width, dev, n) for t, n in ((q, "q"), (out, "out")))
+        a_out = out.data_ptr()
+    else:
+        a_out = _at(out, torch.bfloat16, rows * heads * width, dev, "out")
     a_slots, a_pos = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
     nbytes = _q8_workspace("ts_attend_rows_q8_workspace_bytes", rows, keys, heads, kv_heads, width, back)
     ws = _scratch(nbytes, q)
@@ -339,7 +344,7 @@ def select_blocks_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, cou
     rows, heads, kv_heads, block, width = _heads_of(q, kv)
     a_q = _at(q, torch.bfloat16, rows * heads * width, dev, "q")
     a_slots, a_pos = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
-    ids = torch.empty((rows, kv_heads, max(count, 0)), dtype=torch.int32, device=q.device)
+    ids = q.new_empty((rows, kv_heads, max(count, 0)), dtype=torch.int32)
     nbytes = _q8_workspace("ts_select_blocks_q8_workspace_bytes", rows, keys, kv_heads, block, max(count, 0))
     ws = _scratch(nbytes, q)
     if rows:
@@ -353,9 +358,12 @@ def attend_blocks_q8(q, kv: RowsQ8, ids, slots, positions, kept: Kept, keys: int
     dev, stream = _q8_stream(kv)
     rows, heads, kv_heads, block, width = _heads_of(q, kv)
     count = ids.shape[-1]
+    a_q = _at(q, torch.bfloat16, rows * heads * width, dev, "q")
     if out is None:
         out = torch.empty_like(q)
-    a_q, a_out = (_at(t, torch.bfloat16, rows * heads * width, dev, n) for t, n in ((q, "q"), (out, "out")))
+        a_out = out.data_ptr()
+    else:
+        a_out = _at(out, torch.bfloat16, rows * heads * width, dev, "out")
     a_ids = _at(ids, torch.int32, rows * kv_heads * count, dev, "ids")
     a_slots, a_pos = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
     nbytes = _q8_workspace("ts_attend_blocks_q8_workspace_bytes", rows, count, heads, kv_heads, width, block)
