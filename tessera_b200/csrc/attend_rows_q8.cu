@@ -63,6 +63,7 @@ struct AttendParams {
     uint32_t most;                // tile rows a partial has room for: tokens * part
     uint32_t workers;
     int merged;                   // whether the second kernel runs
+    uint32_t whole;               // without it: every tile counts as this many steps and is never cut
     float scale;
     float *part_o;    // [workers, 2, most, W]
     float *part_ml;   // [workers, 2, most, 2]
@@ -661,7 +662,9 @@ attend_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         // A worker's run: an equal share of the steps laid end to end, or, where that is eight steps at most, the shortest
         // piece for which there are workers enough (a run that ends one tile and begins the next pays for two starts).
         uint32_t run = max(1u, (total + p.workers - 1) / p.workers), by = 1;  // by: tiles take multiples of it
-        if (run <= 8) {
+        if (!p.merged) {
+            by = p.whole;
+        } else if (run <= 8) {
 #pragma unroll
             for (int i = 5; i >= 0; i--)
                 if (pieces[i] * per_row <= p.workers) by = run = kRuns[i];
@@ -672,6 +675,7 @@ attend_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             for (int i = 1; i < 6; i++)
                 if (by == kRuns[i]) total = pieces[i] * kRuns[i] * per_row;
         }
+        if (!p.merged) run = (total + p.workers * by - 1) / (p.workers * by) * by;
         uint32_t at = worker * run;
         const uint32_t end = min(total, at + run);
         if (at < end) {
@@ -822,7 +826,7 @@ __global__ void __launch_bounds__(kMergeThreads) attend_q8_merge_kernel(const At
 __device__ int g_attend_status = 0;
 
 struct Plan {
-    uint32_t part, parts, tokens, workers, together;
+    uint32_t part, parts, tokens, workers, together, whole;
     bool merged;
     size_t o_bytes, ml_bytes, places_bytes;
     size_t bytes() const { return merged ? o_bytes + ml_bytes + places_bytes : 0; }
@@ -837,14 +841,18 @@ Plan plan_of(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, ui
     s.tokens = count || s.parts > 1 ? 1 : 16 / s.part;
     uint64_t span = keys;  // keys a tile may see; the first of them is anywhere in its block of 64 at most
     if (!count && (uint64_t)back + s.tokens < span) span = (uint64_t)back + s.tokens;
-    const uint64_t steps = count ? ((uint64_t)count * block + step - 1) / step : (span + 63 + step - 1) / step;
+    const uint64_t offset = !count && span < keys ? 63 : 0;
+    const uint64_t steps = count ? ((uint64_t)count * block + step - 1) / step : (span + offset + step - 1) / step;
     const uint64_t most = (uint64_t)sm_count() * kBlocks * kWarps;
     const uint64_t each = (uint64_t)kv_heads * s.parts * steps;  // steps of a row at most
     // The kernel counts steps in 32 bits: more rows than that allows go in several launches, whole tiles each.
     uint64_t together = 0x7FFFFFFFull / each / s.tokens * s.tokens;
     s.together = (uint32_t)(rows < together ? rows : together);
-    s.workers = (uint32_t)(s.together * each < most ? s.together * each : most);
-    s.merged = s.together * each > 1;  // else the one step there is belongs to one worker
+    // A tile of up to four steps is not worth cutting: a worker does it in less time than a second kernel takes.
+    s.merged = steps > 4;
+    s.whole = steps <= 1 ? 1 : (uint32_t)(steps < 4 ? steps : 4);
+    const uint64_t jobs = s.merged ? s.together * each : s.together * (each / steps);
+    s.workers = (uint32_t)(jobs < most ? jobs : most);
     s.o_bytes = (size_t)s.workers * 2 * s.tokens * s.part * width * sizeof(float);
     s.ml_bytes = align_up((size_t)s.workers * 2 * s.tokens * s.part * 2 * sizeof(float), 16);
     s.places_bytes = (size_t)rows * kv_heads * s.parts * sizeof(uint4);
@@ -926,6 +934,7 @@ int attend_q8(const void *q, const RowsQ8Dev &kv, const uint32_t *ids, void *out
     p.most = s.tokens * s.part;
     p.workers = s.workers;
     p.merged = s.merged;
+    p.whole = s.whole;
     p.scale = scale;
     if (s.merged) {
         p.part_o = (float *)workspace;

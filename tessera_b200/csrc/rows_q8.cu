@@ -143,7 +143,7 @@ struct AppendParams {
     uint32_t rows, heads, kv_heads;
     float eps;
     uint32_t window;    // rows whose runs one thread block looks after
-    uint32_t kv_ctas;   // thread blocks [0, kv_ctas) do keys and values, the others queries
+    uint32_t q_ctas, stride;  // thread blocks for queries, one in every `stride`
     uint32_t per_warp, q_rows;  // query heads, and rows, that a warp takes
 };
 
@@ -240,20 +240,22 @@ __device__ __forceinline__ void write_bounds(int8_t *bounds, uint32_t first, uin
 constexpr uint32_t kShort = 4;  // rows of a run that one warp takes
 constexpr int kAppendWarps = 4, kAppendThreads = kAppendWarps * 32;
 
-// Parts of an append in one kernel: blocks [0, kv_ctas) keys and values, the others queries.
-enum Role { kAll, kKeysValues, kQueries };
-
-template <int W, int B, Role ROLE>
-__global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQueries ? 8 : 6) append_q8_kernel(const AppendParams p) {
+template <int W, int B>
+__global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_kernel(const AppendParams p) {
     constexpr int L = Lanes<W>::PER_HEAD, T = Lanes<W>::TOGETHER;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, li = lane % L, which = lane / L;
     const uint32_t per_row = p.heads + 2 * p.kv_heads;
     __shared__ uint64_t sm_turns[W / 2];  // each pair's, computed once: its 64-bit arithmetic is slow
     pdl_wait();
-    const bool queries = ROLE == kQueries || (ROLE == kAll && blockIdx.x >= p.kv_ctas);
+    // Query blocks are spread among the others (which wait for one load after another, while they are bound by their
+    // traffic): every p.stride-th block as long as there are any.
+    const uint32_t turn_q = blockIdx.x / p.stride;
+    const bool queries = blockIdx.x % p.stride == p.stride - 1 && turn_q < p.q_ctas;
+    const uint32_t kv_block = blockIdx.x - min(turn_q, p.q_ctas);
+    const float freq = threadIdx.x < W / 2 ? p.inv_freq[threadIdx.x] : 0.0f;
     // ---- keys, values: the runs that begin among this block's rows, at most 32 of them, one a lane ----
-    const uint32_t units = 2 * p.kv_heads, unit = blockIdx.x % units;
-    const uint32_t r0 = blockIdx.x / units * p.window, r1 = min(p.rows, r0 + p.window);
+    const uint32_t units = 2 * p.kv_heads, unit = kv_block % units;
+    const uint32_t r0 = kv_block / units * p.window, r1 = min(p.rows, r0 + p.window);
     uint32_t slot = 0, blk_pos = 0xFFFFFFFFu, starts = 0;
     if (!queries) {
         if (r0 + lane < r1) {
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
             return;
         }
     }
-    if (threadIdx.x < W / 2) sm_turns[threadIdx.x] = turns_of(p.inv_freq[threadIdx.x]);
+    if (threadIdx.x < W / 2) sm_turns[threadIdx.x] = turns_of(freq);
     __syncthreads();
     uint64_t turns[4];
 #pragma unroll
@@ -280,7 +282,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
     if (queries) {
         // ---- queries: a warp takes up to `per_warp` heads of `q_rows` rows, T of them side by side ----
         const uint32_t parts = (p.heads + p.per_warp - 1) / p.per_warp;
-        const uint32_t job = (blockIdx.x - (ROLE == kAll ? p.kv_ctas : 0)) * kAppendWarps + warp;
+        const uint32_t job = turn_q * kAppendWarps + warp;
         const uint32_t h0 = job % parts * p.per_warp, h1 = min(p.heads, h0 + p.per_warp);
         const uint32_t first = job / parts * p.q_rows;
         float g[8];
@@ -353,15 +355,14 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
             const uint32_t out = ~__ballot_sync(0xFFFFFFFFu, lane < n || (lane <= kShort && same(s + lane)));
             n = __ffs(out) - 1;
         }
-        if (blk == kNoBlock) continue;
-        const size_t at = (size_t)blk * p.kv_heads + h;
+        const size_t at = (size_t)(blk == kNoBlock ? 0 : blk) * p.kv_heads + h;
         float *scale = (is_v ? p.kv.v_scale : p.kv.k_scale) + at;
         int8_t *codes = (is_v ? p.kv.v : p.kv.k) + at * B * W;
         int8_t *bounds = p.kv.bounds + at * 2 * W;
         const float was = *scale;  // asked for before it is needed
         if (n <= kShort) {
             // ---- a warp's run ----
-            if (turn % kAppendWarps != warp) continue;
+            if (turn % kAppendWarps != warp || blk == kNoBlock) continue;
             constexpr int PASSES = kShort / T > 0 ? kShort / T : 1;
             uint32_t held[4] = {};  // the bounds of this lane's channels
             if (bounded && which == 0) {
@@ -447,6 +448,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : ROLE == kQuerie
             if (end < base + TEAM * 32) break;
         }
         team_sync();
+        if (blk == kNoBlock) continue;
         auto row_of = [&](int u) { return mine + STEP * u < B ? src[mine + STEP * u] : -1; };
         if (is_v) {
             // ---- values: bf16 as they come, kept as such; magnitudes compare as whole numbers ----
@@ -689,33 +691,23 @@ constexpr size_t append_smem() {
     return (size_t)(kAppendWarps / team) * passes * 2 * team * 32 * sizeof(float4);
 }
 
-template <int W, int B, Role ROLE>
-cudaError_t launch_append_block(const AppendParams &p, uint32_t grid, bool dependent, cudaStream_t stream) {
-    constexpr size_t smem = ROLE == kQueries ? 0 : append_smem<W, B>();
+template <int W, int B>
+cudaError_t launch_append(const AppendParams &p, uint32_t grid, cudaStream_t stream) {
+    constexpr size_t smem = append_smem<W, B>();
     static OncePerDevice configured;
     if (smem > 48 * 1024 && configured.needs()) {
-        const cudaError_t e = cudaFuncSetAttribute(append_q8_kernel<W, B, ROLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = cudaFuncSetAttribute(append_q8_kernel<W, B>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
         configured.done();
     }
-    return launch(append_q8_kernel<W, B, ROLE>, dim3(grid), dim3(kAppendThreads), smem, stream, dependent, p);
+    return launch(append_q8_kernel<W, B>, dim3(grid), dim3(kAppendThreads), smem, stream, pdl_enabled(), p);
 }
 
-template <int W, Role ROLE>
-cudaError_t launch_append(const AppendParams &p, uint32_t block, uint32_t grid, bool dependent, cudaStream_t stream) {
-    return block == 16   ? launch_append_block<W, 16, ROLE>(p, grid, dependent, stream)
-           : block == 32 ? launch_append_block<W, 32, ROLE>(p, grid, dependent, stream)
-                         : launch_append_block<W, 64, ROLE>(p, grid, dependent, stream);
-}
-
-// Many rows: keys and values, which need registers, apart from queries, which need warps; the second launch waits for the
-// first by itself.
 template <int W>
-cudaError_t launch_append(const AppendParams &p, uint32_t kv_ctas, uint32_t q_ctas, cudaStream_t stream) {
-    const uint32_t block = 1u << p.kv.shift;
-    if (p.window < 32) return launch_append<W, kAll>(p, block, kv_ctas + q_ctas, pdl_enabled(), stream);
-    const cudaError_t e = launch_append<W, kKeysValues>(p, block, kv_ctas, pdl_enabled(), stream);
-    return e != cudaSuccess ? e : launch_append_block<W, 16, kQueries>(p, q_ctas, true, stream);
+cudaError_t launch_append(const AppendParams &p, uint32_t grid, cudaStream_t stream) {
+    return p.kv.shift == 4   ? launch_append<W, 16>(p, grid, stream)
+           : p.kv.shift == 5 ? launch_append<W, 32>(p, grid, stream)
+                             : launch_append<W, 64>(p, grid, stream);
 }
 
 }  // namespace
@@ -747,10 +739,12 @@ int append_q8(const void *qkv, const float *q_norm, const float *k_norm, const f
     const uint64_t kv_ctas = (uint64_t)ceil_div(rows, p.window) * 2 * kv_heads;
     const uint64_t q_ctas = ((uint64_t)ceil_div(rows, p.q_rows) * ceil_div(heads, p.per_warp) + kAppendWarps - 1) / kAppendWarps;
     TS_REQUIRE(kv_ctas + q_ctas < 0x1FFFFFFFull, "append (q8): %u rows of %u heads are too many for one launch", rows, heads);
-    p.kv_ctas = (uint32_t)kv_ctas;
-    const cudaError_t e = width == 64    ? launch_append<64>(p, (uint32_t)kv_ctas, (uint32_t)q_ctas, stream)
-                          : width == 128 ? launch_append<128>(p, (uint32_t)kv_ctas, (uint32_t)q_ctas, stream)
-                                         : launch_append<256>(p, (uint32_t)kv_ctas, (uint32_t)q_ctas, stream);
+    const uint32_t grid = (uint32_t)(kv_ctas + q_ctas);
+    p.q_ctas = (uint32_t)q_ctas;
+    p.stride = grid / p.q_ctas;
+    const cudaError_t e = width == 64    ? launch_append<64>(p, grid, stream)
+                          : width == 128 ? launch_append<128>(p, grid, stream)
+                                         : launch_append<256>(p, grid, stream);
     if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of append (q8) failed: %s", cudaGetErrorString(e));
     return TS_OK;
 }

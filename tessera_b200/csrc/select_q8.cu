@@ -19,7 +19,6 @@ struct SelectParams {
     const uint32_t *slots, *positions;
     uint32_t rows, keys, heads, kv_heads, count, first, recent;
     uint32_t most;    // blocks a row may have: the scores' row length
-    uint32_t chunk;   // blocks a scoring thread block takes
     float *scores;    // [rows, kv_heads, most]
 };
 
@@ -34,6 +33,8 @@ __device__ __forceinline__ int dp2a_hi(int a, int b, int c) {
     return d;
 }
 
+constexpr int kScore = 128;  // threads of a scoring thread block, and the blocks it scores
+
 // Blocks that hold a position a row sees: 1 + min(pos, keys - 1) / B.
 __device__ __forceinline__ uint32_t blocks_of(const SelectParams &p, uint32_t row) {
     return (min(p.positions[row], p.keys - 1) >> p.kv.shift) + 1;
@@ -45,74 +46,83 @@ __device__ __forceinline__ uint32_t rank_of(float score) {
     return score != score ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// A warp scores 32 blocks: its lanes look them up side by side, W / 8 lanes then hold a block's 2 W bounds, 16 a lane, and
+// several blocks' bounds are under way before the weights are ready.
 template <int W>
-__global__ void __launch_bounds__(128) score_blocks_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(kScore) score_blocks_kernel(const SelectParams p) {
+    constexpr uint32_t LANES = W / 8, AT_ONCE = 32 / LANES, LOADS = 32 / AT_ONCE;  // loads for 32 blocks
+    constexpr uint32_t EARLY = LOADS < 8 ? LOADS : 8;
     __shared__ __align__(16) int16_t weight[2][W];  // for the lowest codes, for the highest
-    __shared__ float sm_max[4];
+    __shared__ float sm_max[kScore / 32];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();
-    const uint32_t row = blockIdx.z, h = blockIdx.y, n = blocks_of(p, row), b0 = blockIdx.x * p.chunk;
+    const uint32_t row = blockIdx.z, h = blockIdx.y, n = blocks_of(p, row), b0 = blockIdx.x * kScore;
     if (n <= p.count || b0 >= n) {
         pdl_launch_dependents();
         return;
     }
+    const uint32_t mine = b0 + warp * 32 + lane, part = lane % LANES, which = lane / LANES;
+    const uint32_t blk = mine < n ? block_of(p.kv, p.slots[row], mine) : kNoBlock;
     const uint32_t group = p.heads / p.kv_heads;
     const uint16_t *q = p.q + ((size_t)row * p.heads + h * group) * W;
+    // channels threadIdx.x, + kScore: the group's largest magnitude
     float most = 0.0f;
-    for (uint32_t i = threadIdx.x; i < group * W; i += 128) most = fmaxf(most, fabsf(bf16_lo(q[i])));
+    for (uint32_t i = threadIdx.x; i < group * W / 2; i += kScore) {
+        const uint32_t v = reinterpret_cast<const uint32_t *>(q)[i];
+        most = fmaxf(most, fmaxf(fabsf(bf16_lo(v)), fabsf(bf16_hi(v))));
+    }
+    int4 c[EARLY];
+    auto bounds_at = [&](uint32_t k) {  // of the block that load k has for this lane
+        const uint32_t b = __shfl_sync(0xFFFFFFFFu, blk, k * AT_ONCE + which);
+        return b == kNoBlock ? make_int4(0, 0, 0, 0) : *reinterpret_cast<const int4 *>(p.kv.bounds + ((size_t)b * p.kv_heads + h) * 2 * W + part * 16);
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < EARLY; k++) c[k] = bounds_at(k);
+    const float scale = blk == kNoBlock ? 0.0f : p.kv.k_scale[(size_t)blk * p.kv_heads + h];
     most = warp_max(most);
     if (lane == 0) sm_max[warp] = most;
     __syncthreads();
-    most = fmaxf(fmaxf(sm_max[0], sm_max[1]), fmaxf(sm_max[2], sm_max[3]));
-    for (uint32_t d = threadIdx.x; d < W; d += 128) {
+#pragma unroll
+    for (int w = 0; w < kScore / 32; w++) most = fmaxf(most, sm_max[w]);
+    for (uint32_t d = threadIdx.x; d < W; d += kScore) {
         int up = 0, down = 0;
         for (uint32_t g = 0; g < group; g++) {
             const float x = bf16_lo(q[g * W + d]);
             // NaN and infinity over infinity convert to 0
-            const int c = most > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(x * 127.0f, most)))) : 0;
-            up += max(c, 0);
-            down += min(c, 0);
+            const int code = most > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(x * 127.0f, most)))) : 0;
+            up += max(code, 0);
+            down += min(code, 0);
         }
         weight[0][d] = (int16_t)down;
         weight[1][d] = (int16_t)up;
     }
     __syncthreads();
-    // a lane holds 16 channels' weights; W / 8 lanes cover a block's 2 W bounds
-    constexpr uint32_t LANES = W / 8;
-    const uint32_t part = lane % LANES;
-    int w[8];
+    int w[8];  // of this lane's 16 channels
 #pragma unroll
     for (int i = 0; i < 8; i++) w[i] = reinterpret_cast<const int *>(&weight[0][0])[part * 8 + i];
-    const uint32_t slot = p.slots[row], end = min(n, b0 + p.chunk);
-    for (uint32_t b = b0 + warp * (32 / LANES); b < end; b += 4 * (32 / LANES)) {
-        const uint32_t mine = b + lane / LANES;
-        int sum = 0;
-        float scale = 0.0f;
-        bool there = false;
-        if (mine < end) {
-            const uint32_t blk = block_of(p.kv, slot, mine);
-            if (blk != kNoBlock) {
-                there = true;
-                const size_t at = (size_t)blk * p.kv_heads + h;
-                const int4 c = *reinterpret_cast<const int4 *>(p.kv.bounds + at * 2 * W + part * 16);
-                const int v[4] = {c.x, c.y, c.z, c.w};
+    int total = 0;  // of this lane's own block
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    sum = dp2a_lo(w[2 * i], v[i], sum);
-                    sum = dp2a_hi(w[2 * i + 1], v[i], sum);
-                }
-                scale = p.kv.k_scale[at];
-            }
+    for (uint32_t k = 0; k < LOADS; k++) {
+        const int4 v = k < EARLY ? c[k < EARLY ? k : 0] : bounds_at(k);
+        const int b[4] = {v.x, v.y, v.z, v.w};
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            sum = dp2a_lo(w[2 * i], b[i], sum);
+            sum = dp2a_hi(w[2 * i + 1], b[i], sum);
         }
 #pragma unroll
         for (uint32_t o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        if (part == 0 && mine < end)
-            p.scores[((size_t)row * p.kv_heads + h) * p.most + mine] = there ? __fmul_rn(__int2float_rn(sum), scale) : -INFINITY;
+        const int got = __shfl_sync(0xFFFFFFFFu, sum, (lane % AT_ONCE) * LANES);  // block k * AT_ONCE + lane % AT_ONCE
+        if (lane / AT_ONCE == k) total = got;
     }
+    if (mine < n)
+        p.scores[((size_t)row * p.kv_heads + h) * p.most + mine] = blk == kNoBlock ? -INFINITY : __fmul_rn(__int2float_rn(total), scale);
     pdl_launch_dependents();
 }
 
 constexpr int kPick = 256;
+constexpr uint32_t kHeld = 4;
 
 // One thread block per (row, kv head): the rank of the count-th best by four passes over 8-bit digits, then the blocks
 // above it, and the lowest of those at it, in ascending order.
@@ -128,15 +138,22 @@ __global__ void __launch_bounds__(kPick) pick_blocks_kernel(const SelectParams p
         return;
     }
     const float *scores = p.scores + ((size_t)row * p.kv_heads + h) * p.most;
-    auto rank = [&](uint32_t i) { return i < p.first || i >= n - p.recent ? 0xFFFFFFFFu : min(rank_of(scores[i]), 0xFFFFFFFEu); };
+    auto ranked = [&](uint32_t i) { return i < p.first || i >= n - p.recent ? 0xFFFFFFFFu : min(rank_of(scores[i]), 0xFFFFFFFEu); };
+    // the first kHeld of a thread's blocks stay in registers over the passes
+    uint32_t held[kHeld];
+#pragma unroll
+    for (uint32_t k = 0; k < kHeld; k++) held[k] = threadIdx.x + k * kPick < n ? ranked(threadIdx.x + k * kPick) : 0;
     uint32_t prefix = 0, left = p.count;  // the digits found so far; how many are still to come among those that share them
     for (int shift = 24; shift >= 0; shift -= 8) {
         hist[threadIdx.x] = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n; i += kPick) {
-            const uint32_t u = rank(i);
+        auto count = [&](uint32_t u) {
             if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255], 1u);
-        }
+        };
+#pragma unroll
+        for (uint32_t k = 0; k < kHeld; k++)
+            if (threadIdx.x + k * kPick < n) count(held[k]);
+        for (uint32_t i = threadIdx.x + kHeld * kPick; i < n; i += kPick) count(ranked(i));
         __syncthreads();
         if (warp == 0) {
             // lane l: digits 255 - 8 l downwards
@@ -163,7 +180,14 @@ __global__ void __launch_bounds__(kPick) pick_blocks_kernel(const SelectParams p
     uint32_t out = 0, equal = 0;  // taken so far, seen at the border so far
     for (uint32_t base = 0; base < n && out < p.count; base += kPick) {
         const uint32_t i = base + threadIdx.x;
-        const uint32_t u = i < n ? rank(i) : 0;
+        uint32_t u = 0;
+        if (base < kHeld * kPick) {
+#pragma unroll
+            for (uint32_t k = 0; k < kHeld; k++)
+                if (base == k * kPick) u = held[k];
+        } else if (i < n) {
+            u = ranked(i);
+        }
         const bool gt = i < n && u > prefix, eq = i < n && u == prefix;
         const uint32_t m_gt = __ballot_sync(0xFFFFFFFFu, gt), m_eq = __ballot_sync(0xFFFFFFFFu, eq);
         __syncthreads();
@@ -216,7 +240,6 @@ int select_q8(const void *q, const RowsQ8Dev &kv, uint32_t *ids, const uint32_t 
     p.first = first;
     p.recent = recent;
     p.most = (uint32_t)(((uint64_t)keys + (1u << kv.shift) - 1) >> kv.shift);
-    p.chunk = 64;
     p.scores = (float *)workspace;
     const size_t need = select_q8_workspace_bytes(rows, keys, kv_heads, 1u << kv.shift, count);
     TS_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace != nullptr && aligned16(workspace))),
@@ -225,12 +248,12 @@ int select_q8(const void *q, const RowsQ8Dev &kv, uint32_t *ids, const uint32_t 
     TS_REQUIRE(rows <= 65535, "select_blocks (q8): %u rows are more than 65535", rows);
     cudaError_t e = cudaSuccess;
     if (need) {
-        const dim3 grid(ceil_div(p.most, p.chunk), kv_heads, rows);
-        e = width == 64    ? launch(score_blocks_kernel<64>, grid, dim3(128), 0, stream, pdl_enabled(), p)
-            : width == 128 ? launch(score_blocks_kernel<128>, grid, dim3(128), 0, stream, pdl_enabled(), p)
-                           : launch(score_blocks_kernel<256>, grid, dim3(128), 0, stream, pdl_enabled(), p);
+        const dim3 grid(ceil_div(p.most, kScore), kv_heads, rows);
+        e = width == 64    ? launch(score_blocks_kernel<64>, grid, dim3(kScore), 0, stream, pdl_enabled(), p)
+            : width == 128 ? launch(score_blocks_kernel<128>, grid, dim3(kScore), 0, stream, pdl_enabled(), p)
+                           : launch(score_blocks_kernel<256>, grid, dim3(kScore), 0, stream, pdl_enabled(), p);
     }
-    if (e == cudaSuccess) e = launch(pick_blocks_kernel, dim3(kv_heads, rows), dim3(kPick), 0, stream, pdl_enabled(), p);
+    if (e == cudaSuccess) e = launch(pick_blocks_kernel, dim3(kv_heads, rows), dim3(kPick), 0, stream, need ? true : pdl_enabled(), p);
     if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of select_blocks (q8) failed: %s", cudaGetErrorString(e));
     return TS_OK;
 }

@@ -237,15 +237,17 @@ def _refuse(message: str):
     raise _lib.TesseraError(_lib.TS_ERR_BAD_INPUT, message)
 
 
-# A step makes a few of these calls a layer, each a few microseconds of GPU time, so the checks below read every property
-# of a tensor once and build nothing that they do not need.
+# A step makes a few of these calls a layer, each a few microseconds of GPU time, so what follows reads every property of a
+# tensor once and builds nothing that it does not need.
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+
 
 def _q8_stream(kv: RowsQ8) -> tuple:
     """(device ordinal, stream): the current stream of the rows' device, which has to be the current device."""
     dev = kv.k.get_device()
     if dev < 0:
         _refuse("tensors must live on a CUDA device (there is no CPU path)")
-    if dev != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         _refuse(f"the rows are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
     return dev, torch._C._cuda_getCurrentRawStream(dev)
 
@@ -261,8 +263,8 @@ def _at(t, dtype, count, dev, name):
 
 def _kept_q8(kept: Kept, dev) -> TsKept:
     t = kept.table
-    if t is not None and (t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous()):
-        _refuse(f"page table: expected contiguous {torch.int32} on cuda:{dev}, got {t.dtype} on {t.device}")
+    if t is not None and (t.dtype is not _I32 or t.get_device() != dev or not t.is_contiguous()):
+        _refuse(f"page table: expected contiguous {_I32} on cuda:{dev}, got {t.dtype} on {t.device}")
     return kept.c()
 
 
@@ -271,10 +273,22 @@ def _q8_workspace(which: str, *sizes) -> int:
     return getattr(lib, which)(*sizes)
 
 
-def _scratch(nbytes: int, like) -> torch.Tensor | None:
-    """Scratch of one call, from the caching allocator: eager calls reuse it in stream order, a captured call keeps its
-    own in the graph's pool, so that two graphs never share it."""
-    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+_q8_scratch: dict = {}
+
+
+def _scratch(nbytes: int, dev: int, stream: int, like):
+    """(address, owner) of scratch for one call: one buffer a device and stream, which its calls use one after another.
+    A call that is being captured gets its own, in the graph's pool: graphs replay on any stream, and two of them at
+    once must not share it."""
+    if nbytes == 0:
+        return None, None
+    if torch._C._cuda_isCurrentStreamCapturing():
+        buf = like.new_empty(nbytes, dtype=torch.uint8)
+        return buf.data_ptr(), buf
+    buf = _q8_scratch.get((dev, stream))
+    if buf is None or buf.numel() < nbytes:
+        buf = _q8_scratch[dev, stream] = like.new_empty(max(nbytes, 1 << 20), dtype=torch.uint8)
+    return buf.data_ptr(), buf
 
 
 def qk_norm_rope_append_q8(qkv, q_norm, k_norm, inv_freq, slots, positions, kv: RowsQ8, kept: Kept, heads: int, *, eps: float,
@@ -284,13 +298,13 @@ def qk_norm_rope_append_q8(qkv, q_norm, k_norm, inv_freq, slots, positions, kv: 
     dev, stream = _q8_stream(kv)
     rows = slots.numel()
     _, kv_heads, _, width = kv.k.shape
-    a_qkv = _at(qkv, torch.bfloat16, rows * (heads + 2 * kv_heads) * width, dev, "qkv")
+    a_qkv = _at(qkv, _BF16, rows * (heads + 2 * kv_heads) * width, dev, "qkv")
     if out is None:
         out = qkv.new_empty((rows, heads, width))
-    args = (a_qkv, _at(q_norm, torch.float32, width, dev, "q_norm"),
-            _at(k_norm, torch.float32, width, dev, "k_norm"), _at(inv_freq, torch.float32, width // 2, dev, "inv_freq"),
-            _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions"),
-            _at(out, torch.bfloat16, rows * heads * width, dev, "out"))
+    args = (a_qkv, _at(q_norm, _F32, width, dev, "q_norm"),
+            _at(k_norm, _F32, width, dev, "k_norm"), _at(inv_freq, _F32, width // 2, dev, "inv_freq"),
+            _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions"),
+            _at(out, _BF16, rows * heads * width, dev, "out"))
     if rows:
         check(lib.ts_qk_norm_rope_append_q8(*args, kv.c(), _kept_q8(kept, dev), rows, heads, kv_heads, width, eps, stream))
     return out
@@ -303,7 +317,7 @@ def rows_unpack_q8(kv: RowsQ8, slots, positions, kept: Kept):
     _, kv_heads, _, width = kv.k.shape
     k_out = kv.k.new_empty((rows, kv_heads, width), dtype=torch.bfloat16)
     v_out = torch.empty_like(k_out)
-    args = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
+    args = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
     if rows:
         check(lib.ts_rows_unpack_q8(kv.c(), *args, k_out.data_ptr(), v_out.data_ptr(), _kept_q8(kept, dev), rows, kv_heads, width,
                                     stream))
@@ -322,18 +336,18 @@ def attend_rows_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, *, sc
     """Ragged causal attention over 8-bit kept rows, q and result bf16 [rows, heads, width]: ts_attend_rows_q8."""
     dev, stream = _q8_stream(kv)
     rows, heads, kv_heads, _, width = _heads_of(q, kv)
-    a_q = _at(q, torch.bfloat16, rows * heads * width, dev, "q")
+    a_q = _at(q, _BF16, rows * heads * width, dev, "q")
     if out is None:
         out = torch.empty_like(q)
         a_out = out.data_ptr()
     else:
-        a_out = _at(out, torch.bfloat16, rows * heads * width, dev, "out")
-    a_slots, a_pos = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
+        a_out = _at(out, _BF16, rows * heads * width, dev, "out")
+    a_slots, a_pos = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
     nbytes = _q8_workspace("ts_attend_rows_q8_workspace_bytes", rows, keys, heads, kv_heads, width, back)
-    ws = _scratch(nbytes, q)
+    ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:
         check(lib.ts_attend_rows_q8(a_q, kv.c(), a_out, a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads, width, back,
-                                    scale, ws.data_ptr() if nbytes else None, nbytes, stream))
+                                    scale, ws, nbytes, stream))
     return out
 
 
@@ -342,14 +356,14 @@ def select_blocks_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, cou
     (UINT32_MAX) in spare entries: ts_select_blocks_q8."""
     dev, stream = _q8_stream(kv)
     rows, heads, kv_heads, block, width = _heads_of(q, kv)
-    a_q = _at(q, torch.bfloat16, rows * heads * width, dev, "q")
-    a_slots, a_pos = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
+    a_q = _at(q, _BF16, rows * heads * width, dev, "q")
+    a_slots, a_pos = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
     ids = q.new_empty((rows, kv_heads, max(count, 0)), dtype=torch.int32)
     nbytes = _q8_workspace("ts_select_blocks_q8_workspace_bytes", rows, keys, kv_heads, block, max(count, 0))
-    ws = _scratch(nbytes, q)
+    ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:
         check(lib.ts_select_blocks_q8(a_q, kv.c(), ids.data_ptr(), a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads,
-                                      width, max(count, 0), first, recent, ws.data_ptr() if nbytes else None, nbytes, stream))
+                                      width, max(count, 0), first, recent, ws, nbytes, stream))
     return ids
 
 
@@ -358,19 +372,19 @@ def attend_blocks_q8(q, kv: RowsQ8, ids, slots, positions, kept: Kept, keys: int
     dev, stream = _q8_stream(kv)
     rows, heads, kv_heads, block, width = _heads_of(q, kv)
     count = ids.shape[-1]
-    a_q = _at(q, torch.bfloat16, rows * heads * width, dev, "q")
+    a_q = _at(q, _BF16, rows * heads * width, dev, "q")
     if out is None:
         out = torch.empty_like(q)
         a_out = out.data_ptr()
     else:
-        a_out = _at(out, torch.bfloat16, rows * heads * width, dev, "out")
-    a_ids = _at(ids, torch.int32, rows * kv_heads * count, dev, "ids")
-    a_slots, a_pos = _at(slots, torch.int32, rows, dev, "slots"), _at(positions, torch.int32, rows, dev, "positions")
+        a_out = _at(out, _BF16, rows * heads * width, dev, "out")
+    a_ids = _at(ids, _I32, rows * kv_heads * count, dev, "ids")
+    a_slots, a_pos = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
     nbytes = _q8_workspace("ts_attend_blocks_q8_workspace_bytes", rows, count, heads, kv_heads, width, block)
-    ws = _scratch(nbytes, q)
+    ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:
         check(lib.ts_attend_blocks_q8(a_q, kv.c(), a_ids, a_out, a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads,
-                                      width, count, scale, ws.data_ptr() if nbytes else None, nbytes, stream))
+                                      width, count, scale, ws, nbytes, stream))
     return out
 
 

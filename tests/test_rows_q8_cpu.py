@@ -79,7 +79,8 @@ def test_buffers_and_counts_are_checked(world):
     refused(_lib, lib.ts_attend_rows_q8(p, good, None, p, p, paged, 1, 64, 4, 2, 64, 0, 1.0, None, 0, None), "NULL")
     refused(_lib, lib.ts_attend_rows_q8(p, good, p, p, p, paged, 1, 64, 5, 2, 64, 0, 1.0, None, 0, None), "split over")
     refused(_lib, lib.ts_attend_rows_q8(p, good, p, p, p, paged, 1, 64, 0, 2, 64, 0, 1.0, None, 0, None), "split over")
-    refused(_lib, lib.ts_attend_rows_q8(p, good, p, p, p, paged, 1, 100000, 4, 2, 64, 0xFFFFFFFF, 1.0, None, 0, None), "workspace")
+    long = _lib.TsKept(2, 64, 2000, p, 4, 128)
+    refused(_lib, lib.ts_attend_rows_q8(p, good, p, p, p, long, 1, 100000, 4, 2, 64, 0xFFFFFFFF, 1.0, None, 0, None), "workspace")
     refused(_lib, lib.ts_attend_blocks_q8(p, good, None, p, p, p, paged, 1, 64, 4, 2, 64, 1, 1.0, None, 0, None), "ids")
     refused(_lib, lib.ts_attend_blocks_q8(p, good, p, p, p, p, paged, 1, 64, 4, 2, 64, 0, 1.0, None, 0, None), "1 to")
     bare = _lib.TsRowsQ8(p, p, p, p, None, 16, 8)
