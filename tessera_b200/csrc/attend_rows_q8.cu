@@ -745,10 +745,10 @@ attend_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 }
 
 // One block per (row, head): folds the partials of its tile in the order of their keys.  Threads take partials side by
-// side for their weights, then W / 4 threads read a partial's output and 1024 / W partials are under way at once.
-constexpr int kMergeThreads = 256;
-
-template <int W>
+// side for their weights, then W / 4 threads read a partial's output, THREADS * 4 / W partials side by side.  Few rows and
+// heads have many partials each and get 256 threads; many have few, and 64 let all of them be resident at once (3584 rows
+// and heads: 13 us with 256).
+template <int W, int kMergeThreads>
 __global__ void __launch_bounds__(kMergeThreads) attend_q8_merge_kernel(const AttendParams p) {
     constexpr uint32_t COLS = W / 4, SETS = kMergeThreads / COLS;
     extern __shared__ float weight[];  // [partials]
@@ -879,8 +879,9 @@ int launch_attend(const AttendParams &p, cudaStream_t stream) {
     const uint32_t grid = min(p.workers, (uint32_t)sm_count() * kBlocks);
     cudaError_t e = launch(attend_q8_kernel<W, LIST>, dim3(grid), dim3(kThreads), smem, stream, pdl_enabled(), map_k, map_v, p, status);
     if (e == cudaSuccess && p.merged)  // always as a dependent launch: it waits for the partials itself
-        e = launch(attend_q8_merge_kernel<W>, dim3(p.rows * p.heads), dim3(kMergeThreads),
-                   p.workers * sizeof(float), stream, true, p);
+        e = p.rows * p.heads > (uint32_t)sm_count() * 8
+                ? launch(attend_q8_merge_kernel<W, 64>, dim3(p.rows * p.heads), dim3(64), p.workers * sizeof(float), stream, true, p)
+                : launch(attend_q8_merge_kernel<W, 256>, dim3(p.rows * p.heads), dim3(256), p.workers * sizeof(float), stream, true, p);
     if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of attend (q8) failed: %s", cudaGetErrorString(e));
     return TS_OK;
 }
