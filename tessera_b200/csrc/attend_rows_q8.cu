@@ -424,6 +424,8 @@ __device__ __forceinline__ void value_step(Running<W, NT> &run, uint32_t tile, c
 }
 
 // 32 blocks' places in the pool and scales, one a lane: entry `first` + lane of the tile's blocks.
+constexpr uint32_t kNoKeys = 0xFFFFFFF0u;  // a unit's first key where there is no block: no row sees it
+
 struct Group {
     uint32_t blk, id;  // pool block or kNoBlock; which block of the slot's positions it is
     float ks, vs;
@@ -454,18 +456,31 @@ struct Ring {
     bool ok;  // false: a wait ran out, nothing is copied or computed any more
 };
 
-// Where a tile's result goes: the output, or a partial.
-struct Target {
-    bool partial;
-    size_t slot;  // worker * 2 + 0 or 1
+// A part of a worker's run: steps [begin, end) of a tile for one kv head and part of its heads.
+struct Segment {
+    Tile tile;
+    uint32_t unit, kvh, head0, part;  // unit: kv head and part of its heads as one number
+    uint32_t begin, end;
+    uint32_t start;    // where the tile's steps begin in all steps
+    bool partial;      // another worker has the rest of them
+    size_t slot;       // of the partial result
 };
 
+// What follows a segment, so that its first steps' copies leave while the segment's last steps are computed.
+struct Following {
+    Group group;
+    uint32_t begin, steps, kvh;  // steps: how many may be asked for early; 0: nothing follows
+};
+
+// Computes a segment, `asked` of whose steps are already on their way, and returns how many of the following one's are.
 template <int W, int NT, bool LIST>
-__device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtensorMap *map_k, const CUtensorMap *map_v, const Tile &tile,
-                                             uint32_t kvh, uint32_t head0, uint32_t part, uint32_t begin, uint32_t end, Target to,
-                                             Ring &ring, int *status, uint32_t lane) {
+__device__ __forceinline__ uint32_t attend_steps(const AttendParams &p, const CUtensorMap *map_k, const CUtensorMap *map_v, const Segment &seg,
+                                                 Group now, uint32_t asked, const Following &then, Ring &ring, int *status,
+                                                 uint32_t lane) {
     using namespace ptx;
     constexpr int KEYS = Step<W>::KEYS, U = Step<W>::UNITS, HALVES = Step<W>::HALVES, COLS = Step<W>::COLS, STAGES = kStages;
+    const Tile &tile = seg.tile;
+    const uint32_t kvh = seg.kvh, head0 = seg.head0, part = seg.part, begin = seg.begin, end = seg.end;
     const uint32_t in_block = p.kv.shift - 4;  // log2 of a block's 16-key units
     Running<W, NT> run;
 #pragma unroll
@@ -475,46 +490,54 @@ __device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtens
         run.m[t][0] = run.m[t][1] = -INFINITY;
         run.l[t][0] = run.l[t][1] = 0.0f;
     }
+    uint32_t early = 0;  // steps of what follows that are on their way
     if (tile.from < tile.to) {
         uint32_t first = (begin * U) >> in_block;  // entry of lane 0 of the current group
         const RawQueries<W, NT> raw = fetch_queries<W, NT>(p, tile, head0, part, lane);
-        Group now = group_of<LIST>(p, tile, kvh, first, lane);
         Group next = now;  // the first copies lie in the current group
         const uint32_t per = 1u << in_block, span = per < (uint32_t)U ? per : U;  // units of one copy
-        // Where step s's units lie in the pool; the current or the next group has its blocks.
-        auto find = [&](uint32_t s, uint32_t (&blk)[U]) {
+        constexpr bool CHAIN = NT == 1;  // with sixteen rows the registers for it cost more than it saves (62 us for 58)
+        const uint32_t last = CHAIN ? end + then.steps : end;
+        // Step s's units as rows of the tensor maps, -1 where there is no block; the current or the next group has its
+        // blocks, or what follows does.
+        auto find = [&](uint32_t s, int32_t (&y)[U]) {
+            const bool mine = !CHAIN || s < end;
+            const uint32_t unit = (mine ? s : then.begin + (s - end)) * U, head = mine ? kvh : then.kvh;
+            const uint32_t from = mine ? first : (then.begin * U) >> in_block;
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const uint32_t e = ((s * U + u) >> in_block) - first;
-                const uint32_t a = __shfl_sync(0xFFFFFFFFu, now.blk, e & 31), b = __shfl_sync(0xFFFFFFFFu, next.blk, e & 31);
-                blk[u] = e < 32 ? a : b;
+                y[u] = -1;
+                if ((u & (span - 1)) != 0) continue;  // lies in the copy of the unit before it
+                const uint32_t e = ((unit + u) >> in_block) - from;
+                const uint32_t blk = __shfl_sync(0xFFFFFFFFu, !mine ? then.group.blk : e < 32 ? now.blk : next.blk, e & 31);
+                if (blk != kNoBlock) y[u] = (int32_t)(((blk * p.kv_heads + head) << p.kv.shift) + (((unit + u) & (per - 1)) << 4));
             }
         };
-        // Copies of step s's K (values = 0) or V (1) into stage `at`.
-        auto copy = [&](uint32_t s, uint32_t at, const uint32_t (&blk)[U], const CUtensorMap *map, int values) {
+        // Copies of a step's K (values = 0) or V (1) into stage `at`.
+        auto copy = [&](uint32_t at, const int32_t (&y)[U], const CUtensorMap *map, int values) {
             if (lane == 0) {
                 uint64_t *bar = &ring.full[values * STAGES + at];
                 const uint32_t dst = ring.tiles + at * kStage + values * kHalfStage;
                 uint32_t bytes = 0;
 #pragma unroll
                 for (int u = 0; u < U; u++)
-                    if ((u & (span - 1)) == 0 && blk[u] != kNoBlock) bytes += span * 16 * W;
+                    if (y[u] >= 0) bytes += span * 16 * W;
                 mbar_expect_tx(bar, bytes);
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    if ((u & (span - 1)) != 0 || blk[u] == kNoBlock) continue;
-                    const int32_t y = (int32_t)(((blk[u] * p.kv_heads + kvh) << p.kv.shift) + (((s * U + u) & (per - 1)) << 4));
+                    if (y[u] < 0) continue;
 #pragma unroll
-                    for (int h = 0; h < HALVES; h++) copy_codes(dst + (h * KEYS + 16 * u) * COLS, map, smem_addr(bar), h * COLS, y);
+                    for (int h = 0; h < HALVES; h++) copy_codes(dst + (h * KEYS + 16 * u) * COLS, map, smem_addr(bar), h * COLS, y[u]);
                 }
             }
         };
-        uint32_t ahead = begin, blk[U];  // the next step to ask for, and where it lies
-        for (; ahead < end && ahead < begin + STAGES; ahead++) {
+        int32_t y[U];
+        uint32_t ahead = begin + asked;  // the next step to ask for; from `end` on, of what follows
+        for (; ahead < last && ahead < begin + STAGES; ahead++) {
             const uint32_t at = (ring.stage + (ahead - begin)) % STAGES;
-            find(ahead, blk);
-            copy(ahead, at, blk, map_k, 0);
-            copy(ahead, at, blk, map_v, 1);
+            find(ahead, y);
+            copy(at, y, map_k, 0);
+            copy(at, y, map_v, 1);
         }
         next = group_of<LIST>(p, tile, kvh, first + 32, lane);
         Queries<W, NT> qs;
@@ -536,12 +559,19 @@ __device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtens
             bool edge = false;
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const uint32_t unit = s * U + u, e = ((unit >> in_block) - first) & 31;
-                ks[u] = __shfl_sync(0xFFFFFFFFu, now.ks, e);
-                vs[u] = __shfl_sync(0xFFFFFFFFu, now.vs, e);
-                const uint32_t blk = __shfl_sync(0xFFFFFFFFu, now.blk, e), id = __shfl_sync(0xFFFFFFFFu, now.id, e);
-                key0[u] = blk == kNoBlock ? 0xFFFFFFF0u : (id << p.kv.shift) + ((unit & ((1u << in_block) - 1)) << 4);
-                edge = edge || key0[u] < all_lo || key0[u] + 16 > all_hi || blk == kNoBlock;
+                const uint32_t unit = s * U + u;
+                if (u == 0 || (unit & (per - 1)) == 0) {  // another block
+                    const uint32_t e = ((unit >> in_block) - first) & 31;
+                    ks[u] = __shfl_sync(0xFFFFFFFFu, now.ks, e);
+                    vs[u] = __shfl_sync(0xFFFFFFFFu, now.vs, e);
+                    const uint32_t id = __shfl_sync(0xFFFFFFFFu, now.blk == kNoBlock ? kNoBlock : now.id, e);
+                    key0[u] = id == kNoBlock ? kNoKeys : (id << p.kv.shift) + ((unit & (per - 1)) << 4);
+                } else {
+                    ks[u] = ks[u - (u > 0)];
+                    vs[u] = vs[u - (u > 0)];
+                    key0[u] = key0[u - (u > 0)] == kNoKeys ? kNoKeys : key0[u - (u > 0)] + 16;
+                }
+                edge = edge || key0[u] < all_lo || key0[u] > all_hi - 16 || all_hi < 16;
             }
             const uint32_t at = ring.tiles + ring.stage * kStage, odd = ring.parity >> ring.stage & 1;
             ring.parity ^= 1u << ring.stage;
@@ -555,35 +585,36 @@ __device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtens
                     mbar_wait(&ring.full[stage], ring.parity >> stage & 1);
                     mbar_wait(&ring.full[STAGES + stage], ring.parity >> stage & 1);
                 }
-                if (k_too && ahead < end) mbar_wait(&ring.full[ring.stage], odd ^ 1);
+                if (k_too && ahead < last) mbar_wait(&ring.full[ring.stage], odd ^ 1);
                 if (lane == 0) atomicExch(status, TS_ERR_TIMEOUT);
             };
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(&ring.full[ring.stage], odd))) {
                 give_up(false);
-                return;
+                return 0;
             }
             float x[U][NT][4];
             if (edge) score_step<W, NT, true>(qs, at, ks, vs, key0, x, lane);
             else score_step<W, NT, false>(qs, at, ks, vs, key0, x, lane);
             __syncwarp();
-            if (ahead < end) {
-                find(ahead, blk);
-                copy(ahead, ring.stage, blk, map_k, 0);
+            if (ahead < last) {
+                find(ahead, y);
+                copy(ring.stage, y, map_k, 0);
             }
             uint32_t b[U][NT][2];
             soften<W, NT>(run, x, vs, b);
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(&ring.full[STAGES + ring.stage], odd))) {
                 give_up(true);
-                return;
+                return 0;
             }
             value_step<W, NT>(run, at + kHalfStage, b, lane);
             __syncwarp();
-            if (ahead < end) {
-                copy(ahead, ring.stage, blk, map_v, 1);
+            if (ahead < last) {
+                copy(ring.stage, y, map_v, 1);
                 ahead++;
             }
             ring.stage = (ring.stage + 1) % STAGES;
         }
+        early = ahead - end;
     }
     // ---- this thread's channels of tile rows 8 t + 2 j + e ----
     const uint32_t r = lane >> 2, j = lane & 3;
@@ -596,7 +627,7 @@ __device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtens
             for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
             const uint32_t m = 8 * t + 2 * j + e;
             if (m >= tile.tokens * part) continue;
-            if (!to.partial) {
+            if (!seg.partial) {
                 const uint32_t token = m / part;
                 uint16_t *out = p.out + ((size_t)(tile.row + token) * p.heads + head0 + m - token * part) * W + 2 * r;
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -604,12 +635,13 @@ __device__ __forceinline__ void attend_steps(const AttendParams &p, const CUtens
                 for (int i = 0; i < W / 16; i++)
                     *reinterpret_cast<uint32_t *>(out + 16 * i) = pack_bf16(run.o[i][t][e] * inv, run.o[i][t][2 + e] * inv);
             } else {
-                float *o = p.part_o + (to.slot * p.most + m) * W + 2 * r;
+                float *o = p.part_o + (seg.slot * p.most + m) * W + 2 * r;
 #pragma unroll
                 for (int i = 0; i < W / 16; i++) *reinterpret_cast<float2 *>(o + 16 * i) = make_float2(run.o[i][t][e], run.o[i][t][2 + e]);
-                if (r == 0) *reinterpret_cast<float2 *>(p.part_ml + (to.slot * p.most + m) * 2) = make_float2(run.m[t][e], l);
+                if (r == 0) *reinterpret_cast<float2 *>(p.part_ml + (seg.slot * p.most + m) * 2) = make_float2(run.m[t][e], l);
             }
         }
+    return early;
 }
 
 template <int W, bool LIST>
@@ -705,39 +737,71 @@ attend_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                     rows = rows_from<W, LIST>(p, row_at(p, first, lane), first, lane);
                 }
             }
-            bool begun = false;  // whether the run has had a tile already
-            while (ring.ok) {
-                const Tile tile = tile_at<LIST>(p, rows, first, l);
-                const uint32_t n = taken(tile.steps);
-                uint32_t h = (at - before) / n;
-                uint32_t start = before + h * n;
-                for (; h < per_row && at < end && ring.ok; h++) {
-                    const uint32_t kvh = p.parts == 1 ? h : h / p.parts, hp = h - kvh * p.parts;
-                    const uint32_t head0 = kvh * p.group + hp * p.part, part = min(p.part, p.group - hp * p.part);
-                    const uint32_t from = at - start, stop = min(tile.steps, end - start);
-                    const Target to = {from > 0 || stop < tile.steps, (size_t)worker * 2 + begun};
-                    if (tile.tokens * part <= 8)
-                        attend_steps<W, 1, LIST>(p, &map_k, &map_v, tile, kvh, head0, part, from, stop, to, ring, status, lane);
-                    else
-                        attend_steps<W, 2, LIST>(p, &map_k, &map_v, tile, kvh, head0, part, from, stop, to, ring, status, lane);
-                    // who has the tile's first step says where its partials are
-                    if (from == 0 && p.merged && lane < tile.tokens)
-                        p.places[(size_t)(tile.row + lane) * per_row + h] = make_uint4(worker, (start + tile.steps - 1) / run, begun, lane * part);
-                    begun = true;
-                    start += n;
-                    at = start;
+            // The run's segments, one after another.
+            Tile tile = tile_at<LIST>(p, rows, first, l);
+            uint32_t n = taken(tile.steps), unit = (at - before) / n, start = before + unit * n, count = 0;
+            auto next_segment = [&](Segment *seg) {
+                if (at >= end) return false;
+                if (unit == per_row) {  // the next tile
+                    before += n * per_row;
+                    const uint32_t later = __ballot_sync(0xFFFFFFFFu, rows.steps != 0 && lane > l);
+                    if (later) {
+                        l = __ffs(later) - 1;
+                    } else {
+                        first += width;
+                        if (first >= p.rows) return false;
+                        rows = rows_from<W, LIST>(p, row_at(p, first, lane), first, lane);
+                        l = 0;
+                    }
+                    tile = tile_at<LIST>(p, rows, first, l);
+                    n = taken(tile.steps);
+                    unit = 0;
+                    start = before;
                 }
-                if (at >= end) break;
-                before += n * per_row;
-                const uint32_t later = __ballot_sync(0xFFFFFFFFu, rows.steps != 0 && lane > l);
-                if (later) {
-                    l = __ffs(later) - 1;
-                } else {
-                    first += width;
-                    if (first >= p.rows) break;
-                    rows = rows_from<W, LIST>(p, row_at(p, first, lane), first, lane);
-                    l = 0;
+                const uint32_t kvh = p.parts == 1 ? unit : unit / p.parts, hp = unit - kvh * p.parts;
+                seg->tile = tile;
+                seg->unit = unit;
+                seg->kvh = kvh;
+                seg->head0 = kvh * p.group + hp * p.part;
+                seg->part = min(p.part, p.group - hp * p.part);
+                seg->begin = at - start;
+                seg->end = min(tile.steps, end - start);
+                seg->start = start;
+                seg->partial = seg->begin > 0 || seg->end < tile.steps;
+                seg->slot = (size_t)worker * 2 + (count++ ? 1 : 0);
+                unit++;
+                start += n;
+                at = start;
+                return true;
+            };
+            auto group_for = [&](const Segment &seg) {
+                return group_of<LIST>(p, seg.tile, seg.kvh, (seg.begin * Step<W>::UNITS) >> (p.kv.shift - 4), lane);
+            };
+            Segment now;
+            bool any = next_segment(&now);
+            Group group = group_for(now);
+            uint32_t asked = 0;
+            while (any && ring.ok) {
+                Segment next;
+                const bool more = next_segment(&next);
+                Following then = {{kNoBlock, 0, 0.0f, 0.0f}, 0, 0, 0};
+                if (more) {
+                    then.group = group_for(next);
+                    then.begin = next.begin;
+                    then.steps = next.tile.from < next.tile.to ? min(next.end - next.begin, (uint32_t)kStages) : 0;
+                    then.kvh = next.kvh;
                 }
+                if (now.tile.tokens * now.part <= 8)
+                    asked = attend_steps<W, 1, LIST>(p, &map_k, &map_v, now, group, asked, then, ring, status, lane);
+                else
+                    asked = attend_steps<W, 2, LIST>(p, &map_k, &map_v, now, group, asked, then, ring, status, lane);
+                // who has a tile's first step says where its partials are
+                if (now.begin == 0 && p.merged && lane < now.tile.tokens)
+                    p.places[(size_t)(now.tile.row + lane) * per_row + now.unit] =
+                        make_uint4(worker, (now.start + now.tile.steps - 1) / run, (uint32_t)(now.slot & 1), lane * now.part);
+                now = next;
+                group = then.group;
+                any = more;
             }
         }
     }

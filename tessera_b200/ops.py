@@ -196,7 +196,8 @@ def attend_rows_append(qkv, q_norm, k_norm, inv_freq, k_rows, v_rows, slots, pos
 class RowsQ8:
     """Kept K and V rows as 8-bit codes: ts_rows_q8.  k, v int8 [blocks, kv_heads, block, width], k_scale, v_scale
     f32 [blocks, kv_heads], k_bounds int8 [blocks, kv_heads, 2, width] or None (needed only to select blocks).  The
-    record holds the tensors; calls read their addresses each time."""
+    record is made once, for as long as the rows are kept: it holds the tensors and the library's record of them, so the
+    tensors must not be resized or given other storage afterwards."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
@@ -215,6 +216,10 @@ class RowsQ8:
             if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous() or t.device != self.k.device:
                 _refuse(f"8-bit rows: expected contiguous {dtype} {tuple(shape)} on {self.k.device}, got {t.dtype} "
                         f"{tuple(t.shape)} on {t.device}")
+        bounds = self.k_bounds.data_ptr() if self.k_bounds is not None else None
+        record = TsRowsQ8(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), bounds, block, blocks)
+        # (the library's record, device ordinal or -1, kv heads, block, width)
+        object.__setattr__(self, "_held", (record, self.k.get_device() if self.k.is_cuda else -1, kv_heads, block, width))
 
     @staticmethod
     def empty(rows: int, kv_heads: int, width: int, block: int = 64, *, bounds: bool = True, device="cuda") -> "RowsQ8":
@@ -227,11 +232,6 @@ class RowsQ8:
                       make(blocks, kv_heads, dtype=torch.float32), make(blocks, kv_heads, dtype=torch.float32),
                       make(blocks, kv_heads, 2, width) if bounds else None)
 
-    def c(self) -> TsRowsQ8:
-        blocks, _, block, _ = self.k.shape
-        return TsRowsQ8(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-                        self.k_bounds.data_ptr() if self.k_bounds is not None else None, block, blocks)
-
 
 def _refuse(message: str):
     raise _lib.TesseraError(_lib.TS_ERR_BAD_INPUT, message)
@@ -242,14 +242,13 @@ def _refuse(message: str):
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
-def _q8_stream(kv: RowsQ8) -> tuple:
-    """(device ordinal, stream): the current stream of the rows' device, which has to be the current device."""
-    dev = kv.k.get_device()
+def _q8_stream(dev: int) -> int:
+    """The current stream of the rows' device, which has to be the current device."""
     if dev < 0:
         _refuse("tensors must live on a CUDA device (there is no CPU path)")
     if dev != torch._C._cuda_getDevice():
         _refuse(f"the rows are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
-    return dev, torch._C._cuda_getCurrentRawStream(dev)
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _at(t, dtype, count, dev, name):
@@ -295,9 +294,9 @@ def qk_norm_rope_append_q8(qkv, q_norm, k_norm, inv_freq, slots, positions, kv: 
                            out=None):
     """Per-head norm (gains f32 [width] or None) and rotation, q out in bf16 [rows, heads, width], k and v into their
     blocks: ts_qk_norm_rope_append_q8.  Rows that fall into the same block stand next to one another."""
-    dev, stream = _q8_stream(kv)
+    record, dev, kv_heads, _, width = kv._held
+    stream = _q8_stream(dev)
     rows = slots.numel()
-    _, kv_heads, _, width = kv.k.shape
     a_qkv = _at(qkv, _BF16, rows * (heads + 2 * kv_heads) * width, dev, "qkv")
     if out is None:
         out = qkv.new_empty((rows, heads, width))
@@ -306,36 +305,36 @@ def qk_norm_rope_append_q8(qkv, q_norm, k_norm, inv_freq, slots, positions, kv: 
             _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions"),
             _at(out, _BF16, rows * heads * width, dev, "out"))
     if rows:
-        check(lib.ts_qk_norm_rope_append_q8(*args, kv.c(), _kept_q8(kept, dev), rows, heads, kv_heads, width, eps, stream))
+        check(lib.ts_qk_norm_rope_append_q8(*args, record, _kept_q8(kept, dev), rows, heads, kv_heads, width, eps, stream))
     return out
 
 
 def rows_unpack_q8(kv: RowsQ8, slots, positions, kept: Kept):
     """The kept rows at (slots[r], positions[r]) as bf16 [rows, kv_heads, width], keys and values: ts_rows_unpack_q8."""
-    dev, stream = _q8_stream(kv)
+    record, dev, kv_heads, _, width = kv._held
+    stream = _q8_stream(dev)
     rows = slots.numel()
-    _, kv_heads, _, width = kv.k.shape
     k_out = kv.k.new_empty((rows, kv_heads, width), dtype=torch.bfloat16)
     v_out = torch.empty_like(k_out)
     args = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
     if rows:
-        check(lib.ts_rows_unpack_q8(kv.c(), *args, k_out.data_ptr(), v_out.data_ptr(), _kept_q8(kept, dev), rows, kv_heads, width,
+        check(lib.ts_rows_unpack_q8(record, *args, k_out.data_ptr(), v_out.data_ptr(), _kept_q8(kept, dev), rows, kv_heads, width,
                                     stream))
     return k_out, v_out
 
 
-def _heads_of(q, kv: RowsQ8) -> tuple:
-    _, kv_heads, block, width = kv.k.shape
+def _heads_of(q, kv_heads: int, width: int) -> tuple:
     shape = q.shape
     if len(shape) != 3 or shape[2] != width or shape[1] % kv_heads:
         _refuse(f"q {list(shape)} does not go with {kv_heads} kv heads of width {width}")
-    return shape[0], shape[1], kv_heads, block, width
+    return shape[0], shape[1]
 
 
 def attend_rows_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, *, scale: float, back=0xFFFFFFFF, out=None):
     """Ragged causal attention over 8-bit kept rows, q and result bf16 [rows, heads, width]: ts_attend_rows_q8."""
-    dev, stream = _q8_stream(kv)
-    rows, heads, kv_heads, _, width = _heads_of(q, kv)
+    record, dev, kv_heads, _, width = kv._held
+    stream = _q8_stream(dev)
+    rows, heads = _heads_of(q, kv_heads, width)
     a_q = _at(q, _BF16, rows * heads * width, dev, "q")
     if out is None:
         out = torch.empty_like(q)
@@ -346,7 +345,7 @@ def attend_rows_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, *, sc
     nbytes = _q8_workspace("ts_attend_rows_q8_workspace_bytes", rows, keys, heads, kv_heads, width, back)
     ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:
-        check(lib.ts_attend_rows_q8(a_q, kv.c(), a_out, a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads, width, back,
+        check(lib.ts_attend_rows_q8(a_q, record, a_out, a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads, width, back,
                                     scale, ws, nbytes, stream))
     return out
 
@@ -354,23 +353,25 @@ def attend_rows_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, *, sc
 def select_blocks_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, count: int, *, first: int = 1, recent: int = 1):
     """The `count` blocks of positions each row and kv head should read, ascending, int32 [rows, kv_heads, count] with -1
     (UINT32_MAX) in spare entries: ts_select_blocks_q8."""
-    dev, stream = _q8_stream(kv)
-    rows, heads, kv_heads, block, width = _heads_of(q, kv)
+    record, dev, kv_heads, block, width = kv._held
+    stream = _q8_stream(dev)
+    rows, heads = _heads_of(q, kv_heads, width)
     a_q = _at(q, _BF16, rows * heads * width, dev, "q")
     a_slots, a_pos = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
     ids = q.new_empty((rows, kv_heads, max(count, 0)), dtype=torch.int32)
     nbytes = _q8_workspace("ts_select_blocks_q8_workspace_bytes", rows, keys, kv_heads, block, max(count, 0))
     ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:
-        check(lib.ts_select_blocks_q8(a_q, kv.c(), ids.data_ptr(), a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads,
+        check(lib.ts_select_blocks_q8(a_q, record, ids.data_ptr(), a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads,
                                       width, max(count, 0), first, recent, ws, nbytes, stream))
     return ids
 
 
 def attend_blocks_q8(q, kv: RowsQ8, ids, slots, positions, kept: Kept, keys: int, *, scale: float, out=None):
     """Causal attention over the listed blocks only (ids int32 [rows, kv_heads, count], -1 = none): ts_attend_blocks_q8."""
-    dev, stream = _q8_stream(kv)
-    rows, heads, kv_heads, block, width = _heads_of(q, kv)
+    record, dev, kv_heads, block, width = kv._held
+    stream = _q8_stream(dev)
+    rows, heads = _heads_of(q, kv_heads, width)
     count = ids.shape[-1]
     a_q = _at(q, _BF16, rows * heads * width, dev, "q")
     if out is None:
@@ -383,7 +384,7 @@ def attend_blocks_q8(q, kv: RowsQ8, ids, slots, positions, kept: Kept, keys: int
     nbytes = _q8_workspace("ts_attend_blocks_q8_workspace_bytes", rows, count, heads, kv_heads, width, block)
     ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:
-        check(lib.ts_attend_blocks_q8(a_q, kv.c(), a_ids, a_out, a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads,
+        check(lib.ts_attend_blocks_q8(a_q, record, a_ids, a_out, a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads,
                                       width, count, scale, ws, nbytes, stream))
     return out
 
