@@ -64,6 +64,7 @@ struct AttendParams {
     uint32_t workers;
     int merged;                   // whether the second kernel runs
     uint32_t whole;               // without it: every tile counts as this many steps and is never cut
+    uint32_t cluster;             // blocks of a cluster that has a row and kv head to itself; 0: the other kernels
     float scale;
     float *part_o;    // [workers, 2, most, W]
     float *part_ml;   // [workers, 2, most, 2]
@@ -463,7 +464,8 @@ struct Segment {
     uint32_t begin, end;
     uint32_t start;    // where the tile's steps begin in all steps
     bool partial;      // another worker has the rest of them
-    size_t slot;       // of the partial result
+    uint32_t slot;     // of the worker's two partial results
+    float *part_o, *part_ml;  // where a partial result goes: [tile rows][W] and [tile rows][2]
 };
 
 // What follows a segment, so that its first steps' copies leave while the segment's last steps are computed.
@@ -635,10 +637,10 @@ __device__ __forceinline__ uint32_t attend_steps(const AttendParams &p, const CU
                 for (int i = 0; i < W / 16; i++)
                     *reinterpret_cast<uint32_t *>(out + 16 * i) = pack_bf16(run.o[i][t][e] * inv, run.o[i][t][2 + e] * inv);
             } else {
-                float *o = p.part_o + (seg.slot * p.most + m) * W + 2 * r;
+                float *o = seg.part_o + m * W + 2 * r;
 #pragma unroll
                 for (int i = 0; i < W / 16; i++) *reinterpret_cast<float2 *>(o + 16 * i) = make_float2(run.o[i][t][e], run.o[i][t][2 + e]);
-                if (r == 0) *reinterpret_cast<float2 *>(p.part_ml + (seg.slot * p.most + m) * 2) = make_float2(run.m[t][e], l);
+                if (r == 0) *reinterpret_cast<float2 *>(seg.part_ml + m * 2) = make_float2(run.m[t][e], l);
             }
         }
     return early;
@@ -768,7 +770,9 @@ attend_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 seg->end = min(tile.steps, end - start);
                 seg->start = start;
                 seg->partial = seg->begin > 0 || seg->end < tile.steps;
-                seg->slot = (size_t)worker * 2 + (count++ ? 1 : 0);
+                seg->slot = count++ ? 1 : 0;
+                seg->part_o = p.part_o + ((size_t)worker * 2 + seg->slot) * p.most * W;
+                seg->part_ml = p.part_ml + ((size_t)worker * 2 + seg->slot) * p.most * 2;
                 unit++;
                 start += n;
                 at = start;
@@ -798,7 +802,7 @@ attend_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                 // who has a tile's first step says where its partials are
                 if (now.begin == 0 && p.merged && lane < now.tile.tokens)
                     p.places[(size_t)(now.tile.row + lane) * per_row + now.unit] =
-                        make_uint4(worker, (now.start + now.tile.steps - 1) / run, (uint32_t)(now.slot & 1), lane * now.part);
+                        make_uint4(worker, (now.start + now.tile.steps - 1) / run, now.slot, lane * now.part);
                 now = next;
                 group = then.group;
                 any = more;
@@ -887,13 +891,100 @@ __global__ void __launch_bounds__(kMergeThreads) attend_q8_merge_kernel(const At
     pdl_launch_dependents();
 }
 
+// Few and short rows: a cluster of blocks has one row and kv head (or part of its heads), its warps cut the steps among them,
+// and the partial results meet through distributed shared memory: one launch, no pass over the rows, no workspace.
+template <int W, bool LIST>
+__global__ void __launch_bounds__(kThreads, kBlocks)
+attend_q8_cluster_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttendParams p, int *status) {
+    using namespace ptx;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ uint64_t bars[kWarps][2 * kStages];
+    __shared__ float2 sm_ml[kWarps][16];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = cluster_ctarank(), blocks = p.cluster;
+    Ring ring = {smem_addr(smem) + warp * (kStages * kStage), bars[warp], 0, 0, true};
+    if (lane == 0) {
+        for (int s = 0; s < 2 * kStages; s++) mbar_init(&ring.full[s], 1);
+        fence_barrier_init();
+        if (warp == 0) {
+            prefetch_tensormap(&map_k);
+            prefetch_tensormap(&map_v);
+        }
+    }
+    __syncwarp();
+    pdl_wait();
+    const uint32_t per_row = p.kv_heads * p.parts, job = blockIdx.x / blocks, worker = warp * blocks + rank;
+    Segment seg;
+    Tile &t = seg.tile;
+    t.row = job / per_row;
+    t.tokens = 1;
+    t.slot = p.slots[t.row];
+    seen(p, p.positions[t.row], &t.from, &t.to);
+    if (t.from >= t.to) t.from = t.to = 0;
+    t.base = LIST ? 0 : t.from >> p.kv.shift;
+    t.entries = LIST ? p.count : t.from < t.to ? ((t.to - 1) >> p.kv.shift) + 1 - t.base : 0;
+    t.steps = LIST            ? ((p.count << (p.kv.shift - 4)) + Step<W>::UNITS - 1) / Step<W>::UNITS
+              : t.from < t.to ? (t.to - 1 - (t.base << p.kv.shift)) / Step<W>::KEYS + 1 : 0;
+    seg.unit = job - t.row * per_row;
+    seg.kvh = p.parts == 1 ? seg.unit : seg.unit / p.parts;
+    const uint32_t hp = seg.unit - seg.kvh * p.parts;
+    seg.head0 = seg.kvh * p.group + hp * p.part;
+    seg.part = min(p.part, p.group - hp * p.part);
+    const uint32_t each = (t.steps + kWarps * blocks - 1) / (kWarps * blocks);
+    seg.begin = worker * each;
+    seg.end = min(t.steps, seg.begin + each);
+    seg.partial = true;
+    seg.part_o = reinterpret_cast<float *>(smem + warp * (kStages * kStage));  // its ring is empty by then
+    seg.part_ml = reinterpret_cast<float *>(sm_ml[warp]);
+    if (lane < 16) sm_ml[warp][lane] = make_float2(-INFINITY, 0.0f);
+    __syncwarp();
+    if (seg.begin < seg.end && t.from < t.to) {
+        const Group group = group_of<LIST>(p, t, seg.kvh, (seg.begin * Step<W>::UNITS) >> (p.kv.shift - 4), lane);
+        const Following none = {{kNoBlock, 0, 0.0f, 0.0f}, 0, 0, 0};
+        if (seg.part <= 8) attend_steps<W, 1, LIST>(p, &map_k, &map_v, seg, group, 0, none, ring, status, lane);
+        else attend_steps<W, 2, LIST>(p, &map_k, &map_v, seg, group, 0, none, ring, status, lane);
+    }
+    cluster_sync();
+    // Block `rank` folds its share of the row's heads' channels, four at a time, in the order of the keys: worker = warp *
+    // blocks + rank.
+    for (uint32_t i = (rank * kThreads + threadIdx.x) * 4; i < seg.part * W; i += blocks * kThreads * 4) {
+        const uint32_t m = i / W, d = i % W;
+        const uint32_t ml_at = smem_addr(&sm_ml[0][m]), o_at = smem_addr(smem) + (m * W + d) * 4;
+        float top = -INFINITY;
+        for (uint32_t w = 0; w < kWarps; w++)
+#pragma unroll 4
+            for (uint32_t b = 0; b < blocks; b++) top = fmaxf(top, ld_cluster_f32x2(map_to_rank(ml_at + w * (uint32_t)sizeof(sm_ml[0]), b)).x);
+        if (top == -INFINITY) top = 0.0f;
+        float l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t w = 0; w < kWarps; w++)
+#pragma unroll 4
+            for (uint32_t b = 0; b < blocks; b++) {
+                const float2 ml = ld_cluster_f32x2(map_to_rank(ml_at + w * (uint32_t)sizeof(sm_ml[0]), b));
+                const float4 v = ld_cluster_f32x4(map_to_rank(o_at + w * (kStages * kStage), b));
+                const float f = exp2_approx(ml.x - top);
+                l = fmaf(ml.y, f, l);
+                if (ml.x != -INFINITY) {  // else nobody wrote there (NaN scores leave -infinity too, and NaN in l)
+                    o.x = fmaf(v.x, f, o.x);
+                    o.y = fmaf(v.y, f, o.y);
+                    o.z = fmaf(v.z, f, o.z);
+                    o.w = fmaf(v.w, f, o.w);
+                }
+            }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        *reinterpret_cast<uint2 *>(p.out + ((size_t)t.row * p.heads + seg.head0 + m) * W + d) =
+            make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    }
+    pdl_launch_dependents();
+    cluster_sync();  // the other blocks have read this one's shared memory
+}
+
 __device__ int g_attend_status = 0;
 
 struct Plan {
-    uint32_t part, parts, tokens, workers, together, whole;
+    uint32_t part, parts, tokens, workers, together, whole, cluster;
     bool merged;
     size_t o_bytes, ml_bytes, places_bytes;
-    size_t bytes() const { return merged ? o_bytes + ml_bytes + places_bytes : 0; }
+    size_t bytes() const { return merged && !cluster ? o_bytes + ml_bytes + places_bytes : 0; }
 };
 
 Plan plan_of(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width, uint32_t back, uint32_t count,
@@ -917,6 +1008,12 @@ Plan plan_of(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, ui
     s.whole = steps <= 1 ? 1 : (uint32_t)(steps < 4 ? steps : 4);
     const uint64_t jobs = s.merged ? s.together * each : s.together * (each / steps);
     s.workers = (uint32_t)(jobs < most ? jobs : most);
+    // A cluster for each row and kv head, as small as leaves a warp two steps, or four: where all of them are resident at once.
+    s.cluster = 0;
+    const uint64_t rows_heads = (uint64_t)rows * kv_heads * s.parts;
+    for (uint32_t most_steps = 2; most_steps <= 4 && !s.cluster; most_steps += 2)
+        for (uint32_t c = 1; c <= 8 && !s.cluster; c *= 2)
+            if (rows_heads * c <= (uint64_t)sm_count() * kBlocks && steps <= (uint64_t)most_steps * kWarps * c) s.cluster = c;
     s.o_bytes = (size_t)s.workers * 2 * s.tokens * s.part * width * sizeof(float);
     s.ml_bytes = align_up((size_t)s.workers * 2 * s.tokens * s.part * 2 * sizeof(float), 16);
     s.places_bytes = (size_t)rows * kv_heads * s.parts * sizeof(uint4);
@@ -940,6 +1037,29 @@ int launch_attend(const AttendParams &p, cudaStream_t stream) {
     int rc = make_tensor_map_codes(&map_k, p.kv.k, rows, W, Step<W>::COLS, box);
     if (rc == TS_OK) rc = make_tensor_map_codes(&map_v, p.kv.v, rows, W, Step<W>::COLS, box);
     if (rc != TS_OK) return rc;
+    if (p.cluster) {
+        static OncePerDevice ready;
+        if (ready.needs()) {
+            TS_CUDA(cudaFuncSetAttribute(attend_q8_cluster_kernel<W, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            ready.done();
+        }
+        cudaLaunchAttribute attr[2] = {};
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = p.cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(p.rows * p.kv_heads * p.parts * p.cluster);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl_enabled() ? 2 : 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, attend_q8_cluster_kernel<W, LIST>, map_k, map_v, p, status);
+        if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of attend (q8, cluster) failed: %s", cudaGetErrorString(e));
+        return TS_OK;
+    }
     const uint32_t grid = min(p.workers, (uint32_t)sm_count() * kBlocks);
     cudaError_t e = launch(attend_q8_kernel<W, LIST>, dim3(grid), dim3(kThreads), smem, stream, pdl_enabled(), map_k, map_v, p, status);
     if (e == cudaSuccess && p.merged)  // always as a dependent launch: it waits for the partials itself
@@ -1000,8 +1120,9 @@ int attend_q8(const void *q, const RowsQ8Dev &kv, const uint32_t *ids, void *out
     p.workers = s.workers;
     p.merged = s.merged;
     p.whole = s.whole;
+    p.cluster = s.cluster;
     p.scale = scale;
-    if (s.merged) {
+    if (need) {
         p.part_o = (float *)workspace;
         p.part_ml = (float *)((uint8_t *)workspace + s.o_bytes);
         p.places = (uint4 *)((uint8_t *)workspace + s.o_bytes + s.ml_bytes);

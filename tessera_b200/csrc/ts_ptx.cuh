@@ -127,6 +127,17 @@ __device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float a, float b
                  : "memory");
 }
 
+__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
 // Asynchronous 16-byte store into (possibly another block's) shared memory; on completion the
 // destination's mbarrier `bar_addr` (same block as `addr`) is credited 16 transaction bytes.  The
 // sender never waits: visibility comes from the receiver's wait on that barrier.

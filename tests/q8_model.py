@@ -39,16 +39,11 @@ class Store:
 
     def keys_of(self, slot, head, positions):
         """(k, v) in f64 at positions of a slot; positions outside the pool are left out."""
-        ks, vs = [], []
-        for p in positions:
-            blk = self.at(slot, p // self.block)
-            if blk is None:
-                continue
-            i = p % self.block
-            ks.append(self.codes["k"][blk, head, i] * self.scale["k"][blk, head])
-            vs.append(self.codes["v"][blk, head, i] * self.scale["v"][blk, head])
-        w = self.width
-        return np.array(ks).reshape(-1, w), np.array(vs).reshape(-1, w)
+        positions = np.asarray(list(positions), np.int64)
+        where = {b: self.at(slot, int(b)) for b in np.unique(positions // self.block)}
+        blk = np.array([-1 if where[b] is None else where[b] for b in positions // self.block], np.int64)
+        i, blk = positions[blk >= 0] % self.block, blk[blk >= 0]
+        return tuple(self.codes[n][blk, head, i].reshape(-1, self.width) * self.scale[n][blk, head].reshape(-1, 1) for n in "kv")
 
 
 def prepared(qkv, q_norm, k_norm, inv_freq, positions, heads, kv_heads, width, eps):

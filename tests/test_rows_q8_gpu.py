@@ -279,6 +279,38 @@ def test_attention_over_whole_slots(case, lengths, each):
         check_attend(got, want, tol)
 
 
+@pytest.mark.parametrize("case", ATTENDS, ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("kind", ["steps", "drafts", "long"])
+def test_attention_of_many_rows_and_of_long_ones(case, kind):
+    """More rows and kv heads than thread blocks fit the GPU at once, or a context of thousands: the steps of all of
+    them are shared out evenly, whatever the lengths."""
+    from tessera_b200 import ops
+    rng = np.random.default_rng(crc32(repr((case, kind)).encode()))
+    heads, kv_heads, width, block = case[:4]
+    if kind == "long":
+        lengths, each = [9001, 40, 6000], 1
+    else:
+        each = 1 if kind == "steps" else 3
+        lengths = [int(n) for n in rng.integers(each, 300, (310 // kv_heads + 3) // each + 1)]
+        lengths[1] = 2500  # one far longer than the others
+    kv, kept, store = attend_case(rng, case, lengths)
+    slots = [s for s, n in enumerate(lengths) for _ in range(each)]
+    pos = [n - each + i for n in lengths for i in range(each)]
+    q = bf16(rng, len(slots), heads, width)
+    keys, scale = max(lengths), width ** -0.5
+    for back in (FAR, 700):
+        got = ops.attend_rows_q8(q, kv, dev_u32(slots), dev_u32(pos), kept, keys, scale=scale, back=back)
+        want, tol = M.attend(store, np64(q), slots, pos, keys, scale, back)
+        check_attend(got, want, tol)
+    # the same through lists that name every block, in reversed order
+    n = -(-keys // block)
+    if kind == "steps":
+        ids = np.broadcast_to(np.arange(n, dtype=np.uint32)[::-1], (len(slots), kv_heads, n))
+        got = ops.attend_blocks_q8(q, kv, dev_u32(ids), dev_u32(slots), dev_u32(pos), kept, keys, scale=scale)
+        want, tol = M.attend(store, np64(q), slots, pos, keys, scale)
+        check_attend(got, want, tol)
+
+
 def test_attention_of_rows_in_any_order_and_rows_that_see_nothing():
     """Rows of one slot out of order, the same row twice, positions past `keys`, slots and pages outside the pool."""
     from tessera_b200 import ops
