@@ -88,7 +88,7 @@ def test_buffers_and_counts_are_checked(world):
     for count, first, recent in ((0, 0, 0), (4097, 0, 0), (2, 2, 1), (2, 0, 3), (2, 3, 0), (2, 0xFFFFFFFF, 3)):
         refused(_lib, lib.ts_select_blocks_q8(p, good, p, p, p, paged, 1, 64, 4, 2, 64, count, first, recent, None, 0, None), "blocks (1 to 4096)")
     refused(_lib, lib.ts_select_blocks_q8(p, good, p, p, p, paged, 1, 64, 514, 2, 64, 1, 0, 0, None, 0, None), "at most 256")
-    refused(_lib, lib.ts_select_blocks_q8(p, good, p, p, p, paged, 1, 64, 4, 2, 64, 2, 0, 0, None, 0, None), "workspace")
+    refused(_lib, lib.ts_select_blocks_q8(p, good, p, p, p, long, 1, 100000, 4, 2, 64, 2, 0, 0, None, 0, None), "workspace")
     # no rows: nothing to do, and nothing of the GPU is touched
     assert lib.ts_attend_rows_q8(p, good, p, p, p, paged, 0, 64, 4, 2, 64, 0, 1.0, None, 0, None) == 0
     assert lib.ts_rows_unpack_q8(good, p, p, p, p, paged, 0, 2, 64, None) == 0
@@ -103,8 +103,9 @@ def test_workspace_sizes(world):
     assert lib.ts_attend_rows_q8_workspace_bytes(1, 100000, 16, 8, 128, 0xFFFFFFFF) > 0
     # a window bounds what a row reads, and with it the pieces
     assert lib.ts_attend_rows_q8_workspace_bytes(1, 100000, 16, 8, 128, 10) <= lib.ts_attend_rows_q8_workspace_bytes(1, 100000, 16, 8, 128, 50000)
-    assert lib.ts_select_blocks_q8_workspace_bytes(3, 1000, 2, 16, 63) == 0
-    assert lib.ts_select_blocks_q8_workspace_bytes(3, 1000, 2, 16, 62) >= 3 * 2 * 63 * 4
+    assert lib.ts_select_blocks_q8_workspace_bytes(3, 1000, 2, 16, 62) == 0                # scored and picked in one kernel
+    assert lib.ts_select_blocks_q8_workspace_bytes(3, 40000, 2, 16, 2500) == 0             # every block is taken
+    assert lib.ts_select_blocks_q8_workspace_bytes(3, 40000, 2, 16, 2499) >= 3 * 2 * 2500 * 4
     assert lib.ts_attend_blocks_q8_workspace_bytes(2, 0, 16, 8, 128, 64) == 0
 
 
