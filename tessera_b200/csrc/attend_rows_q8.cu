@@ -32,6 +32,12 @@
 // worker leaves at most two partial results (M, sum, output) in the workspace; tiles that lie within a run go straight
 // to the output.  A second kernel folds the partials of a tile in the order of their keys: no atomics, the same bits on
 // every run.
+//
+// What bounds it, measured with width 128.  Many decode rows: the codes' bytes (64 rows of up to 8192 keys, 8 kv heads of 2
+// heads: 134 us, 0.92 of the copy rate; 4 rows of up to 100003 keys, 8 kv heads of 4: 109 us, 0.90).  Listed blocks: the
+// same, in blocks that lie scattered, with a merge (64 rows x 4 kv heads x 64 blocks of 64: 61 us, 0.68).
+// Drafted tokens, where 16 queries share each key: the instructions around the products, the softmax's above all (16 slots
+// x 7 rows of up to 4099 keys, 4 kv heads of 8: 60 us, 0.14 of the copy rate).
 #include <cmath>
 
 #include "rows_q8.cuh"
@@ -892,7 +898,8 @@ __global__ void __launch_bounds__(kMergeThreads) attend_q8_merge_kernel(const At
 }
 
 // Few and short rows: a cluster of blocks has one row and kv head (or part of its heads), its warps cut the steps among them,
-// and the partial results meet through distributed shared memory: one launch, no pass over the rows, no workspace.
+// and the partial results meet through distributed shared memory: one launch, no pass over the rows, no workspace.  One row
+// of 517 keys: 9.0 us, 8 rows x 32 listed blocks of 16: 9.9; both wait for one load after another (position, page, scale, codes).
 template <int W, bool LIST>
 __global__ void __launch_bounds__(kThreads, kBlocks)
 attend_q8_cluster_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttendParams p, int *status) {

@@ -1,12 +1,12 @@
 // Kept rows in 8 bits: append (norm, rotation, block scales, key bounds) and reading rows back.
 //
 // Append.  A block of B positions has one scale per kv head, so the rows of a call that fall into one block are one
-// unit of work: run = the neighbouring rows of a (slot, block).  A long run (a prompt's) belongs to a thread block for each
-// kv head's keys and values: its eight warps take the block's positions in turn and agree on the largest magnitude
-// through shared memory.  A short run (a step's row) belongs to one warp.  Either way the prepared values stay in registers
-// until the scale is known, so that every value is read once and rounded once.  Held codes are read and rewritten only when
-// the scale grows (a new largest value: for values without a trend once in i rows at the block's i-th row).  Query
-// heads go to warps of their own, eight heads of a row each when there are many.
+// unit of work: run = the neighbouring rows of a (slot, block).  A long run (a prompt's) belongs to a team of
+// warps for each kv head's keys and values: they take the block's positions in turn, keep the prepared values in shared
+// memory and agree there on the largest magnitude.  A short run (a step's row) belongs to one warp, which keeps them in
+// registers.  Either way every value is read once and rounded once.  Held codes are read and rewritten only when the scale
+// grows (a new largest value: for values without a trend once in i rows at the block's i-th row).  Query heads go to warps
+// of their own, eight heads of a row each when there are many.
 //
 // W / 8 lanes hold a head: lane i of them the four pairs 4 i .. 4 i + 3, elements 4 i + e and W / 2 + 4 i + e, so that
 // loads are 8 bytes and stores of codes 4 a lane.
@@ -62,6 +62,11 @@ namespace {
 constexpr float kScaleFloor = 8.673617379884035e-19f;  // 2^-60
 constexpr float kLargest = 3.3895313892515355e38f;    // the largest finite bf16
 
+// Two f32 at a time: one instruction each on sm_100.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // Cosine and sine of pos * f.  In 32 bits the product would be off by 0.006 radians at position 100000, so the angle is
 // kept in turns as a 64-bit fraction: pos * round(2^64 f / 2 pi) modulo 2^64, whose rounding is below 1e-7 turns at any
 // position.  The upper 32 bits, less whole quarters, are an angle within pi / 4, where the series of sine to the ninth
@@ -71,16 +76,29 @@ __device__ __forceinline__ uint64_t turns_of(float f) {
     return __double2ull_rn((v - floor(v)) * 18446744073709551616.0);
 }
 
-__device__ __forceinline__ void sine_cosine(uint32_t pos, uint64_t turns, float *s, float *c) {
-    const uint32_t t = (uint32_t)((pos * turns) >> 32);
-    const uint32_t quarter = (t + (1u << 29)) >> 30;
-    const float x = (float)(int32_t)(t - (quarter << 30)) * 1.4629180792671596e-9f, x2 = x * x;  // 2 pi / 2^32
-    const float sine = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 2.7557319e-6f, -1.9841270e-4f), 8.3333333e-3f), -1.6666667e-1f), x);
-    const float cosine = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 2.4801587e-5f, -1.3888889e-3f), 4.1666667e-2f), -0.5f), 1.0f);
-    const bool swap = quarter & 1;
-    const float a = swap ? cosine : sine, b = swap ? sine : cosine;
-    *s = quarter & 2 ? -a : a;
-    *c = (quarter + 1) & 2 ? -b : b;
+// Of two pairs.
+__device__ __forceinline__ void sine_cosine(uint32_t pos, uint64_t turns0, uint64_t turns1, float2 *s, float2 *c) {
+    const uint32_t t[2] = {(uint32_t)((pos * turns0) >> 32), (uint32_t)((pos * turns1) >> 32)};
+    const uint32_t quarter[2] = {(t[0] + (1u << 29)) >> 30, (t[1] + (1u << 29)) >> 30};
+    const float2 x = mul2(make_float2((float)(int32_t)(t[0] - (quarter[0] << 30)), (float)(int32_t)(t[1] - (quarter[1] << 30))),
+                          both(1.4629180792671596e-9f));  // 2 pi / 2^32
+    const float2 x2 = mul2(x, x);
+    float2 sine = fma2(x2, both(2.7557319e-6f), both(-1.9841270e-4f));
+    sine = fma2(x2, sine, both(8.3333333e-3f));
+    sine = fma2(x2, sine, both(-1.6666667e-1f));
+    sine = fma2(mul2(x, x2), sine, x);
+    float2 cosine = fma2(x2, both(2.4801587e-5f), both(-1.3888889e-3f));
+    cosine = fma2(x2, cosine, both(4.1666667e-2f));
+    cosine = fma2(x2, cosine, both(-0.5f));
+    cosine = fma2(x2, cosine, both(1.0f));
+    auto settle = [](float sine, float cosine, uint32_t quarter, float *s, float *c) {
+        const bool swap = quarter & 1;
+        const uint32_t a = __float_as_uint(swap ? cosine : sine), b = __float_as_uint(swap ? sine : cosine);
+        *s = __uint_as_float(a ^ (quarter & 2) << 30);
+        *c = __uint_as_float(b ^ ((quarter + 1) & 2) << 30);
+    };
+    settle(sine.x, cosine.x, quarter[0], &s->x, &c->x);
+    settle(sine.y, cosine.y, quarter[1], &s->y, &c->y);
 }
 
 // What a lane holds of a head: lane i of the W / 8.
@@ -98,39 +116,49 @@ __device__ __forceinline__ Raw load_head(const uint16_t *src, uint32_t i) {
     return {*reinterpret_cast<const uint2 *>(src + 4 * i), *reinterpret_cast<const uint2 *>(src + W / 2 + 4 * i)};
 }
 
-__device__ __forceinline__ void widen(const Raw &raw, float (&x)[8]) {
-    x[0] = bf16_lo(raw.a.x); x[1] = bf16_hi(raw.a.x); x[2] = bf16_lo(raw.a.y); x[3] = bf16_hi(raw.a.y);
-    x[4] = bf16_lo(raw.b.x); x[5] = bf16_hi(raw.b.x); x[6] = bf16_lo(raw.b.y); x[7] = bf16_hi(raw.b.y);
+// A lane's eight values as pairs: x[0], x[1] are elements 4 i .., x[2], x[3] elements W / 2 + 4 i ..
+__device__ __forceinline__ void widen(const Raw &raw, float2 (&x)[4]) {
+    const uint32_t w[4] = {raw.a.x, raw.a.y, raw.b.x, raw.b.y};
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = make_float2(bf16_lo(w[i]), bf16_hi(w[i]));
+}
+
+// 1 / rms of a head, from every lane's values.
+template <int W>
+__device__ __forceinline__ float inverse_rms(const float2 (&x)[4], float eps) {
+    float2 sum = mul2(x[0], x[0]);
+#pragma unroll
+    for (int i = 1; i < 4; i++) sum = fma2(x[i], x[i], sum);
+    float ss = sum.x + sum.y;
+#pragma unroll
+    for (int o = 1; o < Lanes<W>::PER_HEAD; o <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+    return rsqrtf(fmaf(ss, 1.0f / (float)W, eps));
 }
 
 // Norm (g: the lane's gains) and rotation, in 32 bits.
 template <int W>
-__device__ __forceinline__ void norm_turn(float (&x)[8], bool normed, const float (&g)[8], const float (&sn)[4], const float (&cs)[4],
+__device__ __forceinline__ void norm_turn(float2 (&x)[4], bool normed, const float2 (&g)[4], const float2 (&sn)[2], const float2 (&cs)[2],
                                           float eps) {
     if (normed) {
-        float ss = 0.0f;
+        const float2 inv = both(inverse_rms<W>(x, eps));
 #pragma unroll
-        for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-        for (int o = 1; o < Lanes<W>::PER_HEAD; o <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-        const float inv = rsqrtf(fmaf(ss, 1.0f / (float)W, eps));
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] *= inv * g[i];
+        for (int i = 0; i < 4; i++) x[i] = mul2(x[i], mul2(inv, g[i]));
     }
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const float a = x[e], b = x[4 + e];
-        x[e] = a * cs[e] - b * sn[e];
-        x[4 + e] = a * sn[e] + b * cs[e];
+    for (int e = 0; e < 2; e++) {
+        const float2 a = x[e], b = x[2 + e];
+        x[e] = fma2(a, cs[e], mul2(b, make_float2(-sn[e].x, -sn[e].y)));
+        x[2 + e] = fma2(a, sn[e], mul2(b, cs[e]));
     }
 }
 
 template <int W>
-__device__ __forceinline__ void load_gains(const float *gain, uint32_t i, float (&g)[8]) {
+__device__ __forceinline__ void load_gains(const float *gain, uint32_t i, float2 (&g)[4]) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        g[e] = gain ? gain[4 * i + e] : 1.0f;
-        g[4 + e] = gain ? gain[W / 2 + 4 * i + e] : 1.0f;
+    for (int h = 0; h < 2; h++) {
+        const float *from = gain + h * (W / 2) + 4 * i;  // gains are as aligned as a float array is
+        g[2 * h] = gain ? make_float2(from[0], from[1]) : both(1.0f);
+        g[2 * h + 1] = gain ? make_float2(from[2], from[3]) : both(1.0f);
     }
 }
 
@@ -161,7 +189,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 __device__ __forceinline__ float tame(float x) { return x != x ? 0.0f : fminf(fmaxf(x, -kLargest), kLargest); }
 
 // round(x * inv) for |x * inv| < 2^22 in the low bits: the sum's last place is one.
-__device__ __forceinline__ uint32_t code_bits(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582912.0f)); }
+constexpr float kCodeBits = 12582912.0f;  // 1.5 * 2^23
+__device__ __forceinline__ uint32_t code_bits(float x, float inv) { return __float_as_uint(fmaf(x, inv, kCodeBits)); }
 __device__ __forceinline__ uint32_t pack_bits(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
@@ -190,11 +219,13 @@ __device__ __forceinline__ Scales grow(float was, bool fresh, float most) {
 
 // |x| <= most, so that no code passes 127.
 template <int W>
-__device__ __forceinline__ void write_row(int8_t *row, uint32_t i, const float (&x)[8], float inv) {
+__device__ __forceinline__ void write_row(int8_t *row, uint32_t i, const float2 (&x)[4], float inv) {
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int h = 0; h < 2; h++) {
+        const float2 a = fma2(x[2 * h], both(inv), both(kCodeBits)), b = fma2(x[2 * h + 1], both(inv), both(kCodeBits));
         *reinterpret_cast<uint32_t *>(row + h * (W / 2) + 4 * i) =
-            pack_bits(code_bits(x[4 * h], inv), code_bits(x[4 * h + 1], inv), code_bits(x[4 * h + 2], inv), code_bits(x[4 * h + 3], inv));
+            pack_bits(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+    }
 }
 
 // A held row's codes follow the scale (a code of -128, which append never writes, becomes -127 at most).
@@ -240,8 +271,12 @@ __device__ __forceinline__ void write_bounds(int8_t *bounds, uint32_t first, uin
 constexpr uint32_t kShort = 4;  // rows of a run that one warp takes
 constexpr int kAppendWarps = 4, kAppendThreads = kAppendWarps * 32;
 
+// Measured: 64 single rows with 16 + 8 + 8 heads of 128 take 6.1 us, most of it one load after another (slot, page, scale,
+// row, the block when the scale grows); 8165 rows of three prompts 40 us for 119 MB, 0.45 of the copy rate: the angles,
+// norms and roundings of 260,000 heads keep the schedulers busier than the memory.  Two values an instruction brought it
+// there from 43, five thread blocks an SM (92 registers, little spilled) from 41 with six (80 registers).
 template <int W, int B>
-__global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_kernel(const AppendParams p) {
     constexpr int L = Lanes<W>::PER_HEAD, T = Lanes<W>::TOGETHER;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, li = lane % L, which = lane / L;
     const uint32_t per_row = p.heads + 2 * p.kv_heads;
@@ -285,31 +320,72 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
         const uint32_t job = turn_q * kAppendWarps + warp;
         const uint32_t h0 = job % parts * p.per_warp, h1 = min(p.heads, h0 + p.per_warp);
         const uint32_t first = job / parts * p.q_rows;
-        float g[8];
+        const bool full = h1 - h0 == 8, normed = p.q_norm != nullptr;
+        float2 g[4];
         load_gains<W>(p.q_norm, li, g);
         for (uint32_t r = first; r < min(first + p.q_rows, p.rows); r++) {
-            const uint32_t pos = p.positions[r];
             constexpr int PASSES = 8 / T;
             const uint16_t *from = p.qkv + ((size_t)r * per_row + h0 + which) * W;
             uint16_t *to = p.q_out + ((size_t)r * p.heads + h0 + which) * W + 4 * li;
             Raw raw[PASSES];
+            if (full) {
 #pragma unroll
-            for (int k = 0; k < PASSES; k++) {
-                raw[k] = {make_uint2(0, 0), make_uint2(0, 0)};
-                if (h0 + k * T + which < h1) raw[k] = load_head<W>(from + k * T * W, li);
+                for (int k = 0; k < PASSES; k++) raw[k] = load_head<W>(from + k * T * W, li);
+            } else {
+#pragma unroll
+                for (int k = 0; k < PASSES; k++) {
+                    raw[k] = {make_uint2(0, 0), make_uint2(0, 0)};
+                    if (h0 + k * T + which < h1) raw[k] = load_head<W>(from + k * T * W, li);
+                }
             }
-            float sn[4], cs[4];
+            // the row's turn with the gains: first half a (g c) - b (g s), second half a (g s) + b (g c)
+            const uint32_t pos = p.positions[r];
+            float2 ac[2], as[2], bc[2], bs[2];
 #pragma unroll
-            for (int e = 0; e < 4; e++) sine_cosine(pos, turns[e], &sn[e], &cs[e]);
+            for (int e = 0; e < 2; e++) {
+                float2 sn, cs;
+                sine_cosine(pos, turns[2 * e], turns[2 * e + 1], &sn, &cs);
+                ac[e] = mul2(g[e], cs);
+                as[e] = mul2(g[e], sn);
+                bc[e] = mul2(g[2 + e], cs);
+                bs[e] = mul2(g[2 + e], make_float2(-sn.x, -sn.y));
+            }
+            auto turned = [&](const Raw &raw, uint2 (&out)[2]) {
+                float2 x[4];
+                widen(raw, x);
+                if (normed) {
+                    const float2 inv = both(inverse_rms<W>(x, p.eps));
 #pragma unroll
-            for (int k = 0; k < PASSES; k++) {
-                if (h0 + k * T >= h1) break;
-                float x[8];
-                widen(raw[k], x);
-                norm_turn<W>(x, p.q_norm != nullptr, g, sn, cs, p.eps);
-                if (h0 + k * T + which < h1) {
-                    *reinterpret_cast<uint2 *>(to + k * T * W) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-                    *reinterpret_cast<uint2 *>(to + k * T * W + W / 2) = make_uint2(pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+                    for (int i = 0; i < 4; i++) x[i] = mul2(x[i], inv);
+                }
+                uint32_t w[2][2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float2 y = fma2(x[e], ac[e], mul2(x[2 + e], bs[e])), z = fma2(x[e], as[e], mul2(x[2 + e], bc[e]));
+                    w[0][e] = pack_bf16(y.x, y.y);
+                    w[1][e] = pack_bf16(z.x, z.y);
+                }
+                out[0] = make_uint2(w[0][0], w[0][1]);
+                out[1] = make_uint2(w[1][0], w[1][1]);
+            };
+            if (full) {
+#pragma unroll
+                for (int k = 0; k < PASSES; k++) {
+                    uint2 out[2];
+                    turned(raw[k], out);
+                    *reinterpret_cast<uint2 *>(to + k * T * W) = out[0];
+                    *reinterpret_cast<uint2 *>(to + k * T * W + W / 2) = out[1];
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < PASSES; k++) {
+                    if (h0 + k * T >= h1) break;
+                    uint2 out[2];
+                    turned(raw[k], out);
+                    if (h0 + k * T + which < h1) {
+                        *reinterpret_cast<uint2 *>(to + k * T * W) = out[0];
+                        *reinterpret_cast<uint2 *>(to + k * T * W + W / 2) = out[1];
+                    }
                 }
             }
         }
@@ -328,7 +404,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
     __shared__ int all_src[TEAMS][B];  // the row that writes each position of the block, or -1
     __shared__ uint32_t all_stop[TEAMS];
     __shared__ uint32_t sm_max[kAppendWarps];
-    __shared__ float2 sm_step[W / 2];  // sine and cosine of STEP positions
+    __shared__ float4 sm_step[W / 4];  // sines and cosines of STEP positions, of two pairs
     int *src = all_src[team];
     uint32_t &stop = all_stop[team];
     // Long runs: a thread's prepared values wait here for the scale (in registers they would leave room for 12 warps an SM,
@@ -339,9 +415,13 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
     const uint32_t h = is_v ? unit - p.kv_heads : unit;
     const uint16_t *heads = p.qkv + (size_t)(p.heads + unit) * W;  // this unit's head of row 0
     const bool bounded = !is_v && p.kv.bounds != nullptr, normed = !is_v && p.k_norm != nullptr;
-    float g[8];
+    float2 g[4];
     load_gains<W>(normed ? p.k_norm : nullptr, li, g);
-    if (!is_v && threadIdx.x < W / 2) sine_cosine(STEP, sm_turns[threadIdx.x], &sm_step[threadIdx.x].x, &sm_step[threadIdx.x].y);
+    if (!is_v && threadIdx.x < W / 4) {
+        float2 sn, cs;
+        sine_cosine(STEP, sm_turns[2 * threadIdx.x], sm_turns[2 * threadIdx.x + 1], &sn, &cs);
+        sm_step[threadIdx.x] = make_float4(sn.x, sn.y, cs.x, cs.y);
+    }
     __syncthreads();
     for (uint32_t turn = 0; starts; turn++) {
         const uint32_t first = __ffs(starts) - 1;
@@ -371,7 +451,8 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
             }
             uint64_t written = 0;
             for (uint32_t k = 0; k < n; k++) written |= 1ull << (p.positions[s + k] & (B - 1));
-            float x[PASSES][8], low[8], high[8];
+            float2 x[PASSES][4];
+            float low[8], high[8];
             int8_t *row[PASSES];
 #pragma unroll
             for (int e = 0; e < 8; e++) low[e] = INFINITY, high[e] = -INFINITY;
@@ -388,18 +469,20 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
                 }
                 widen(raw, x[k]);
                 if (!is_v && k * T < n) {
-                    float sn[4], cs[4];
+                    float2 sn[2], cs[2];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sine_cosine(pos, turns[e], &sn[e], &cs[e]);
+                    for (int e = 0; e < 2; e++) sine_cosine(pos, turns[2 * e], turns[2 * e + 1], &sn[e], &cs[e]);
                     norm_turn<W>(x[k], normed, g, sn, cs, p.eps);
                 }
                 row[k] = live ? codes + (pos & (B - 1)) * W : nullptr;
                 if (live) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[k][e] = tame(x[k][e]);
-                        low[e] = fminf(low[e], x[k][e]);
-                        high[e] = fmaxf(high[e], x[k][e]);
+                    for (int e = 0; e < 4; e++) {
+                        x[k][e] = make_float2(tame(x[k][e].x), tame(x[k][e].y));
+                        low[2 * e] = fminf(low[2 * e], x[k][e].x);
+                        low[2 * e + 1] = fminf(low[2 * e + 1], x[k][e].y);
+                        high[2 * e] = fmaxf(high[2 * e], x[k][e].x);
+                        high[2 * e + 1] = fmaxf(high[2 * e + 1], x[k][e].y);
                     }
                 }
             }
@@ -477,10 +560,10 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
                 most = 0.0f;
 #pragma unroll
                 for (int u = 0; u < PASSES; u++) {
-                    float x[8];
+                    float2 x[4];
                     widen(raw[u], x);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(tame(x[e])));
+                    for (int e = 0; e < 4; e++) most = fmaxf(most, fmaxf(fabsf(tame(x[e].x)), fabsf(tame(x[e].y))));
                 }
                 top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
                 team_sync();
@@ -494,11 +577,11 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
             for (int u = 0; u < PASSES; u++) {
                 const uint32_t i = mine + STEP * u;
                 if (row_of(u) >= 0) {
-                    float x[8];
+                    float2 x[4];
                     widen(raw[u], x);
                     if (wild) {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = tame(x[e]);
+                        for (int e = 0; e < 4; e++) x[e] = make_float2(tame(x[e].x), tame(x[e].y));
                     }
                     write_row<W>(codes + i * W, li, x, sc.inv);
                 } else if (i < B && sc.ratio < 1.0f) {
@@ -519,9 +602,9 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
         float low[8], high[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) low[e] = INFINITY, high[e] = -INFINITY;
-        float sn[4], cs[4];
+        float2 sn[2], cs[2];
 #pragma unroll
-        for (int e = 0; e < 4; e++) sine_cosine((b << p.kv.shift) + mine, turns[e], &sn[e], &cs[e]);
+        for (int e = 0; e < 2; e++) sine_cosine((b << p.kv.shift) + mine, turns[2 * e], turns[2 * e + 1], &sn[e], &cs[e]);
         bool any = false;
         constexpr int GROUP = PASSES < 4 ? PASSES : 4;  // passes whose loads are under way together
         for (int u0 = 0; u0 < PASSES; u0 += GROUP) {
@@ -534,27 +617,29 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
             }
 #pragma unroll
             for (int k = 0; k < GROUP; k++) {
-                float x[8];
+                float2 x[4];
                 widen(raw[k], x);
                 norm_turn<W>(x, normed, g, sn, cs, p.eps);
                 // the next pass is STEP positions on: a turn by a fixed angle (at most 15 of them, 2^-24 each)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float2 by = sm_step[4 * li + e];
-                    const float s0 = sn[e], c0 = cs[e];
-                    cs[e] = c0 * by.y - s0 * by.x;
-                    sn[e] = s0 * by.y + c0 * by.x;
+                for (int e = 0; e < 2; e++) {
+                    const float4 by = sm_step[2 * li + e];
+                    const float2 s1 = make_float2(by.x, by.y), c1 = make_float2(by.z, by.w), s0 = sn[e], c0 = cs[e];
+                    cs[e] = fma2(c0, c1, mul2(s0, make_float2(-by.x, -by.y)));
+                    sn[e] = fma2(s0, c1, mul2(c0, s1));
                 }
                 if (row_of(u0 + k) >= 0) {
                     any = true;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        low[e] = min_nan(low[e], x[e]);
-                        high[e] = max_nan(high[e], x[e]);
+                    for (int e = 0; e < 4; e++) {
+                        low[2 * e] = min_nan(low[2 * e], x[e].x);
+                        low[2 * e + 1] = min_nan(low[2 * e + 1], x[e].y);
+                        high[2 * e] = max_nan(high[2 * e], x[e].x);
+                        high[2 * e + 1] = max_nan(high[2 * e + 1], x[e].y);
                     }
                 }
-                kept[(2 * (u0 + k)) * (TEAM * 32) + tid] = make_float4(x[0], x[1], x[2], x[3]);
-                kept[(2 * (u0 + k) + 1) * (TEAM * 32) + tid] = make_float4(x[4], x[5], x[6], x[7]);
+                kept[(2 * (u0 + k)) * (TEAM * 32) + tid] = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+                kept[(2 * (u0 + k) + 1) * (TEAM * 32) + tid] = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
             }
         }
         float most = 0.0f;
@@ -590,7 +675,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
             const uint32_t i = mine + STEP * u;
             if (row_of(u) >= 0) {
                 const float4 v = kept[(2 * u) * (TEAM * 32) + tid], w = kept[(2 * u + 1) * (TEAM * 32) + tid];
-                const float x[8] = {v.x, v.y, v.z, v.w, w.x, w.y, w.z, w.w};
+                const float2 x[4] = {make_float2(v.x, v.y), make_float2(v.z, v.w), make_float2(w.x, w.y), make_float2(w.z, w.w)};
                 write_row<W>(codes + i * W, li, x, sc.inv);
             } else if (i < B && sc.ratio < 1.0f) {
                 follow_row<W>(codes + i * W, li, sc.ratio);
@@ -626,9 +711,11 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 6) append_q8_ke
     pdl_launch_dependents();
 }
 
-// A thread has its 8 channels of a kv head's keys or values (a warp's stores then fill whole lines) and goes over ROWS rows: `pieces` threads hold a row (all of K,
-// then V), `together` rows lie side by side. The block first looks all its rows up, then every thread asks for the codes
-// of all its rows before it writes the first.
+// Reading rows back is a copy that widens: the codes once, twice as many bytes out.  A thread has its 8 channels of a kv
+// head's keys or values (a warp's stores then fill whole lines) and goes over ROWS rows: `pieces` threads hold a row (all of
+// K, then V), `together` rows lie side by side.  The block first looks all its rows up, then every thread asks for the codes
+// of all its rows before it writes the first.  2 x 16001 rows of 8 heads of 128: 30.4 us, 5.5 TB/s, 0.84 of the copy rate;
+// 160 rows: 2.4 us, a launch and two loads that wait for each other.
 template <int W, int ROWS>
 __global__ void __launch_bounds__(512) unpack_q8_kernel(const RowsQ8Dev kv, const uint32_t *slots, const uint32_t *positions,
                                                         uint4 *k_out, uint4 *v_out, uint32_t rows, uint32_t kv_heads, uint32_t pieces,
@@ -728,7 +815,7 @@ int append_q8(const void *qkv, const float *q_norm, const float *k_norm, const f
     p.heads = heads;
     p.kv_heads = kv_heads;
     p.eps = eps;
-    // A step's rows each have a run of their own: eight of them keep the warps of a thread block busy.  A prompt's
+    // A step's rows each have a run of their own: four of them keep the warps of a thread block busy.  A prompt's
     // rows come in runs of up to a block: looking at 32 rows leaves few thread blocks without a run to start.
     p.window = rows <= 1024 ? kAppendWarps : 32;
     // Eight heads a warp compute a row's angles once and have their loads under way together, four rows share what a warp

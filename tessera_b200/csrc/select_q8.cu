@@ -5,6 +5,9 @@
 // max(c hi, c lo) is max(c, 0) hi + min(c, 0) lo summed over heads first: one dot product of 2 * width whole numbers a
 // block whatever the group's size, taken with dp2a (16-bit weights, 8-bit bounds).  Nothing is rounded before the one
 // multiplication by the block's key scale, so any order of summation gives the same scores and the same choice.
+//
+// 64 rows x 4 kv heads x up to 512 blocks of width 128 take 13.3 us, of which the bounds' bytes would need 4: the pick's
+// passes over the ranks follow the last score.  8 rows x 8 kv heads x 256 blocks take 6.9 us, one load after another.
 #include <cmath>
 
 #include "rows_q8.cuh"
