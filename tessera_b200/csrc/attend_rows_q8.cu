@@ -16,10 +16,11 @@
 // 1152 is subtracted.
 //
 // The scales leave the products alone.  With s = raw * scale * k_scale in powers of two and
-//     x = s + log2(v_scale),   M = max x,   P = 2^(x - M)  <= 1   (f16 operand of P V)
-// the output is sum P code / sum P / v_scale: the block's value scale rides in the exponent, so that P needs no second
+//     x = s + log2(v_scale),   M ~ max x,   P = 2^(x - M)   (f16 operand of P V)
+// the output is sum(P code) / sum(P / v_scale): the block's value scale rides in the exponent, so that P needs no second
 // factor and stays within f16's range whatever the scales are, and M cancels.  A scale of zero counts as 2^-60, the
-// smallest that append writes.
+// smallest that append writes.  (The second sum is f32: a block whose value scale is below 2^-126 of another's, with
+// values of 10^38 beside ordinary ones, drops out of it.)
 //
 // What feeds it.  Every warp is a worker of its own: it streams a step's codes (4 KB of K, 4 KB of V: 32 keys of width
 // 128) into its own ring with TMA, so that no warp waits for another and the only barrier is the one a copy completes on.
@@ -36,8 +37,9 @@
 // What bounds it, measured with width 128.  Many decode rows: the codes' bytes (64 rows of up to 8192 keys, 8 kv heads of 2
 // heads: 134 us, 0.92 of the copy rate; 4 rows of up to 100003 keys, 8 kv heads of 4: 109 us, 0.90).  Listed blocks: the
 // same, in blocks that lie scattered, with a merge (64 rows x 4 kv heads x 64 blocks of 64: 61 us, 0.68).
-// Drafted tokens, where 16 queries share each key: the instructions around the products, the softmax's above all (16 slots
-// x 7 rows of up to 4099 keys, 4 kv heads of 8: 60 us, 0.14 of the copy rate).
+// Drafted tokens, where 16 queries share each key: the instructions around the products (16 slots x 7 rows of up to 4099 keys,
+// 4 kv heads of 8: 58 us, 0.14 of the copy rate, an instruction in 0.35 of the cycles from two warps a scheduler, which is
+// what their registers leave).
 #include <cmath>
 
 #include "rows_q8.cuh"
@@ -357,41 +359,49 @@ __device__ __forceinline__ void score_step(const Queries<W, NT> &qs, uint32_t ti
     }
 }
 
-// The running maximum and sum over a step's scores, the output brought to the new maximum; b: the probabilities as the
-// second product's operand.
+// The probabilities of a step's scores, as the second product's operand b, and their sum.  M need not be the maximum so
+// far: it stays until a score passes it by kSlack, so that most steps neither bring the maximum together across lanes nor
+// touch the output (16 rows found a new maximum in every other step: 61 us for 16 x 7 rows of up to 4099 keys, 58.5 so).  2^(x - M) then reaches 2^kSlack, well within f16.
+constexpr float kSlack = 8.0f;
+
 template <int W, int NT>
 __device__ __forceinline__ void soften(Running<W, NT> &run, const float (&x)[Step<W>::UNITS][NT][4], const float (&vs)[Step<W>::UNITS],
                                        uint32_t (&b)[Step<W>::UNITS][NT][2]) {
     constexpr int U = Step<W>::UNITS;
-    float scale[NT][2], top[NT][2];
-    bool same = true;
+    float most[NT][2];
+    bool past = false;
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            float most = -INFINITY;
+            most[t][e] = fmaxf(x[0][t][e], x[0][t][2 + e]);
 #pragma unroll
-            for (int u = 0; u < U; u++) most = fmaxf(most, fmaxf(x[u][t][e], x[u][t][2 + e]));
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-            const float now = fmaxf(run.m[t][e], most);
-            top[t][e] = now == -INFINITY ? 0.0f : now;  // nothing seen yet: 2^(-inf - 0) = 0
-            scale[t][e] = exp2_approx(run.m[t][e] - top[t][e]);
-            same = same && scale[t][e] == 1.0f;
-            run.m[t][e] = now;
-            run.l[t][e] *= scale[t][e];
+            for (int u = 1; u < U; u++) most[t][e] = fmaxf(most[t][e], fmaxf(x[u][t][e], x[u][t][2 + e]));
+            past = past || most[t][e] > run.m[t][e] + kSlack;
         }
-    if (!__all_sync(0xFFFFFFFFu, same)) {
+    if (__any_sync(0xFFFFFFFFu, past)) {
 #pragma unroll
-        for (int i = 0; i < W / 16; i++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+            for (int e = 0; e < 2; e++) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    run.o[i][t][e] *= scale[t][e];
-                    run.o[i][t][2 + e] *= scale[t][e];
+                for (int o = 4; o < 32; o <<= 1) most[t][e] = fmaxf(most[t][e], __shfl_xor_sync(0xFFFFFFFFu, most[t][e], o));
+                const float now = fmaxf(run.m[t][e], most[t][e]);
+                const float scale = exp2_approx(run.m[t][e] - (now == -INFINITY ? 0.0f : now));
+                run.m[t][e] = now;
+                run.l[t][e] *= scale;
+#pragma unroll
+                for (int i = 0; i < W / 16; i++) {
+                    run.o[i][t][e] *= scale;
+                    run.o[i][t][2 + e] *= scale;
                 }
+            }
     }
+    float top[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) top[t][e] = run.m[t][e] == -INFINITY ? 0.0f : run.m[t][e];  // nothing seen yet: 2^(-inf - 0) = 0
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const float inv = __fdividef(1.0f, fmaxf(vs[u], kScaleFloor));
