@@ -396,7 +396,8 @@ typedef struct {
  * NaN stores the code 0, an infinity the largest code, and counts as the largest finite bf16 in `a`, so that
  * what is kept reads back finite.
  * Rows of one call that fall into the same block must stand next to one another, in any order; of rows with the
- * same slot and position the last one counts (a launch that repeats its last row to fill up is fine). */
+ * same slot and position the last one counts (a launch that repeats its last row to fill up is fine).  q_out must not
+ * overlap qkv. */
 int ts_qk_norm_rope_append_q8(const void *qkv, const float *q_norm, const float *k_norm, const float *inv_freq,
                               const uint32_t *slots, const uint32_t *positions, void *q_out, const ts_rows_q8 *kv,
                               const ts_kept *kept, uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t width,
@@ -409,7 +410,10 @@ int ts_rows_unpack_q8(const ts_rows_q8 *kv, const uint32_t *slots, const uint32_
 
 /* ts_attend_rows_bf16 over such rows: q, out bf16 [rows, heads, width], row r sees keys [max(0, pos - back),
  * min(pos + 1, keys)) of its slot; a row that sees none gets zeros.  Neighbouring rows of one slot (drafted tokens, a
- * part of a prompt) share what they read.  Scores and sums are f32, probabilities f16. */
+ * part of a prompt) share what they read.  For its scores a query is rounded to 2^-16 of its head's largest magnitude;
+ * scores and sums are f32, probabilities f16.  A query with an infinite or NaN element makes its head's output NaN.
+ * Blocks whose value scales lie more than 2^126 apart within a slot (values of 10^38 beside ordinary ones) lose the
+ * weight of the smaller ones.  `out` must not overlap q. */
 size_t ts_attend_rows_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,
                                          uint32_t back);
 
@@ -434,7 +438,7 @@ int ts_select_blocks_q8(const void *q, const ts_rows_q8 *kv, uint32_t *ids, cons
 
 /* Causal attention over listed blocks only: ids u32 [rows, kv_heads, count] in any order (a block listed twice counts
  * twice); entries without a position <= min(pos, keys - 1), UINT32_MAX among them, are skipped, and a row and kv head
- * with nothing to see gets zeros. */
+ * with nothing to see gets zeros.  In 32 and 16 bits as ts_attend_rows_q8. */
 size_t ts_attend_blocks_q8_workspace_bytes(uint32_t rows, uint32_t count, uint32_t heads, uint32_t kv_heads, uint32_t width,
                                            uint32_t block);
 

@@ -222,6 +222,8 @@ int ts_qk_norm_rope_append_q8(const void *qkv, const float *q_norm, const float 
                               float eps, void *stream) {
     TS_REQUIRE(qkv && inv_freq && slots && positions && q_out, "qk_norm_rope_append (q8): a buffer is NULL");
     TS_REQUIRE(aligned16(qkv) && aligned16(q_out), "qk_norm_rope_append (q8): buffers must be 16-byte aligned");
+    TS_REQUIRE(aligned4(q_norm, k_norm, inv_freq) && aligned4(slots, positions),
+               "qk_norm_rope_append (q8): gains, frequencies, slots and positions must be 4-byte aligned");
     RowsQ8Dev dev;
     const int rc = rows_q8_to_dev("qk_norm_rope_append (q8)", kv, kept, kv_heads, width, &dev);
     if (rc != TS_OK) return rc;
@@ -235,6 +237,7 @@ int ts_rows_unpack_q8(const ts_rows_q8 *kv, const uint32_t *slots, const uint32_
                       const ts_kept *kept, uint32_t rows, uint32_t kv_heads, uint32_t width, void *stream) {
     TS_REQUIRE(slots && positions && k_out && v_out, "rows_unpack (q8): a buffer is NULL");
     TS_REQUIRE(aligned16(k_out) && aligned16(v_out), "rows_unpack (q8): buffers must be 16-byte aligned");
+    TS_REQUIRE(aligned4(slots, positions), "rows_unpack (q8): slots and positions must be 4-byte aligned");
     RowsQ8Dev dev;
     const int rc = rows_q8_to_dev("rows_unpack (q8)", kv, kept, kv_heads, width, &dev);
     if (rc != TS_OK) return rc;
@@ -253,6 +256,7 @@ static int check_attend_q8(const char *what, const void *q, const ts_rows_q8 *kv
                            uint32_t kv_heads, uint32_t width, RowsQ8Dev *dev, bool *done, void *stream) {
     TS_REQUIRE(q && out && slots && positions, "%s: a buffer is NULL", what);
     TS_REQUIRE(aligned16(q) && aligned16(out), "%s: buffers must be 16-byte aligned", what);
+    TS_REQUIRE(aligned4(slots, positions), "%s: slots and positions must be 4-byte aligned", what);
     const int rc = rows_q8_to_dev(what, kv, kept, kv_heads, width, dev);
     if (rc != TS_OK) return rc;
     TS_REQUIRE(heads > 0 && heads % kv_heads == 0, "%s: %u heads do not split over %u kv heads", what, heads, kv_heads);
@@ -284,6 +288,7 @@ int ts_select_blocks_q8(const void *q, const ts_rows_q8 *kv, uint32_t *ids, cons
                         void *stream) {
     TS_REQUIRE(q && ids && slots && positions, "select_blocks (q8): a buffer is NULL");
     TS_REQUIRE(aligned16(q), "select_blocks (q8): q must be 16-byte aligned");
+    TS_REQUIRE(aligned4(ids, slots, positions), "select_blocks (q8): ids, slots and positions must be 4-byte aligned");
     RowsQ8Dev dev;
     const int rc = rows_q8_to_dev("select_blocks (q8)", kv, kept, kv_heads, width, &dev);
     if (rc != TS_OK) return rc;
@@ -312,6 +317,7 @@ int ts_attend_blocks_q8(const void *q, const ts_rows_q8 *kv, const uint32_t *ids
                         size_t workspace_bytes, void *stream) {
     RowsQ8Dev dev;
     bool done = false;
+    TS_REQUIRE(aligned4(ids), "attend_blocks (q8): ids must be 4-byte aligned");
     TS_REQUIRE(ids != nullptr && count > 0 && count <= (1u << 24), "attend_blocks (q8): ids is NULL or %u blocks are not 1 to 2^24", count);
     const int rc = check_attend_q8("attend_blocks (q8)", q, kv, out, slots, positions, kept, rows, keys, heads, kv_heads, width,
                                    &dev, &done, stream);

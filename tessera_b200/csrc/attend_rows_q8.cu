@@ -1113,6 +1113,7 @@ int attend_q8(const void *q, const RowsQ8Dev &kv, const uint32_t *ids, void *out
     const size_t need = s.bytes();
     TS_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace != nullptr && aligned16(workspace))),
                "attend (q8): workspace of %zu bytes is smaller than the %zu needed, or not 16-byte aligned", workspace_bytes, need);
+    TS_REQUIRE(q != out, "attend (q8): out is where q lies, which other blocks still read");
     TS_REQUIRE((uint64_t)rows * heads < 0x7FFFFFFFull, "attend (q8): %u rows are too many for one launch", rows);
     TS_REQUIRE((((uint64_t)kv.blocks * kv_heads) << kv.shift) < 0x7FFFFFFFull, "attend (q8): a pool of %u blocks is too large", kv.blocks);
     TS_REQUIRE(s.together > 0, "attend (q8): %u keys of %u kv heads are too many for one launch", keys, kv_heads);

@@ -22,8 +22,7 @@ int rows_q8_to_dev(const char *what, const ts_rows_q8 *kv, const ts_kept *kept, 
     TS_REQUIRE(kv->k && kv->v && kv->k_scale && kv->v_scale, "%s: codes or scales are NULL", what);
     TS_REQUIRE(aligned16(kv->k) && aligned16(kv->v) && (kv->k_bounds == nullptr || aligned16(kv->k_bounds)),
                "%s: codes and bounds must be 16-byte aligned", what);
-    TS_REQUIRE(((reinterpret_cast<uintptr_t>(kv->k_scale) | reinterpret_cast<uintptr_t>(kv->v_scale)) & 3u) == 0,
-               "%s: scales must be 4-byte aligned", what);
+    TS_REQUIRE(aligned4(kv->k_scale, kv->v_scale), "%s: scales must be 4-byte aligned", what);
     TS_REQUIRE(kv->block == 16 || kv->block == 32 || kv->block == 64, "%s: a block of %u positions is not 16, 32 or 64", what,
                kv->block);
     TS_REQUIRE(kv->blocks > 0 && kv->blocks < kNoBlock, "%s: the pool has no block count", what);
@@ -48,6 +47,7 @@ int rows_q8_to_dev(const char *what, const ts_rows_q8 *kv, const ts_kept *kept, 
                    "%s: pages of %u rows do not hold whole blocks of %u", what, kept->page, kv->block);
         TS_REQUIRE(kept->table != nullptr && kept->table_len > 0 && kept->kept_scalar > 0,
                    "%s: a paged layout needs its page table, table_len and pages per slot", what);
+        TS_REQUIRE(aligned4(kept->table), "%s: the page table must be 4-byte aligned", what);
         while ((kv->block << d.per_shift) < kept->page) d.per_shift++;
         d.scalar = kept->kept_scalar;
         d.table = kept->table;
@@ -825,6 +825,7 @@ int append_q8(const void *qkv, const float *q_norm, const float *k_norm, const f
     p.q_rows = many ? 4 : 1;
     const uint64_t kv_ctas = (uint64_t)ceil_div(rows, p.window) * 2 * kv_heads;
     const uint64_t q_ctas = ((uint64_t)ceil_div(rows, p.q_rows) * ceil_div(heads, p.per_warp) + kAppendWarps - 1) / kAppendWarps;
+    TS_REQUIRE(qkv != q_out, "append (q8): q_out is where qkv lies");
     TS_REQUIRE(kv_ctas + q_ctas < 0x1FFFFFFFull, "append (q8): %u rows of %u heads are too many for one launch", rows, heads);
     const uint32_t grid = (uint32_t)(kv_ctas + q_ctas);
     p.q_ctas = (uint32_t)q_ctas;

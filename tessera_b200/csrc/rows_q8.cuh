@@ -35,6 +35,11 @@ __device__ __forceinline__ uint32_t block_of(const RowsQ8Dev &p, uint32_t slot, 
     return at < p.blocks ? (uint32_t)at : kNoBlock;
 }
 
+// Arrays of f32 or u32 that a kernel reads an element at a time (NULL is as aligned as any).
+inline bool aligned4(const void *a, const void *b = nullptr, const void *c = nullptr) {
+    return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & 3u) == 0;
+}
+
 // TS_OK, or the recorded failure; `what` names the entry point.
 int rows_q8_to_dev(const char *what, const ts_rows_q8 *kv, const ts_kept *kept, uint32_t kv_heads, uint32_t width,
                    RowsQ8Dev *out);

@@ -333,12 +333,7 @@ int select_q8(const void *q, const RowsQ8Dev &kv, uint32_t *ids, const uint32_t 
     const uint64_t room = (uint64_t)kv.scalar << (kv.per_shift + kv.shift);
     if (room < keys) keys = (uint32_t)room;
     SelectParams p = {};
-    p.q = (const uint16_t *)q;
     p.kv = kv;
-    p.ids = ids;
-    p.slots = slots;
-    p.positions = positions;
-    p.rows = rows;
     p.keys = keys;
     p.heads = heads;
     p.kv_heads = kv_heads;
@@ -346,26 +341,34 @@ int select_q8(const void *q, const RowsQ8Dev &kv, uint32_t *ids, const uint32_t 
     p.first = first;
     p.recent = recent;
     p.most = (uint32_t)(((uint64_t)keys + (1u << kv.shift) - 1) >> kv.shift);
-    p.scores = (float *)workspace;
     const size_t need = select_q8_workspace_bytes(rows, keys, kv_heads, 1u << kv.shift, count);
     TS_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace != nullptr && aligned16(workspace))),
                "select_blocks (q8): workspace of %zu bytes is smaller than the %zu needed, or not 16-byte aligned",
                workspace_bytes, need);
-    TS_REQUIRE(rows <= 65535, "select_blocks (q8): %u rows are more than 65535", rows);
-    cudaError_t e = cudaSuccess;
-    if (need) {
-        const dim3 grid(ceil_div(p.most, kScore), kv_heads, rows);
-        e = width == 64    ? launch(score_blocks_kernel<64>, grid, dim3(kScore), 0, stream, pdl_enabled(), p)
-            : width == 128 ? launch(score_blocks_kernel<128>, grid, dim3(kScore), 0, stream, pdl_enabled(), p)
-                           : launch(score_blocks_kernel<256>, grid, dim3(kScore), 0, stream, pdl_enabled(), p);
+    constexpr uint32_t kTogetherRows = 65535;  // a launch's
+    for (uint32_t row = 0; row < rows; row += kTogetherRows) {
+        const uint32_t n = min(kTogetherRows, rows - row);
+        p.rows = n;
+        p.q = (const uint16_t *)q + (size_t)row * heads * width;
+        p.ids = ids + (size_t)row * kv_heads * count;
+        p.slots = slots + row;
+        p.positions = positions + row;
+        p.scores = need ? (float *)workspace + (size_t)row * kv_heads * p.most : nullptr;
+        const dim3 each(kv_heads, n);
+        cudaError_t e;
+        if (need) {
+            const dim3 grid(ceil_div(p.most, kScore), kv_heads, n);
+            e = width == 64    ? launch(score_blocks_kernel<64>, grid, dim3(kScore), 0, stream, pdl_enabled(), p)
+                : width == 128 ? launch(score_blocks_kernel<128>, grid, dim3(kScore), 0, stream, pdl_enabled(), p)
+                               : launch(score_blocks_kernel<256>, grid, dim3(kScore), 0, stream, pdl_enabled(), p);
+            if (e == cudaSuccess) e = launch(pick_blocks_kernel, each, dim3(kPick), 0, stream, true, p);
+        } else {
+            e = width == 64    ? launch(select_blocks_kernel<64>, each, dim3(kPick), 0, stream, pdl_enabled(), p)
+                : width == 128 ? launch(select_blocks_kernel<128>, each, dim3(kPick), 0, stream, pdl_enabled(), p)
+                               : launch(select_blocks_kernel<256>, each, dim3(kPick), 0, stream, pdl_enabled(), p);
+        }
+        if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of select_blocks (q8) failed: %s", cudaGetErrorString(e));
     }
-    const dim3 each(kv_heads, rows);
-    if (!need)
-        e = width == 64    ? launch(select_blocks_kernel<64>, each, dim3(kPick), 0, stream, pdl_enabled(), p)
-            : width == 128 ? launch(select_blocks_kernel<128>, each, dim3(kPick), 0, stream, pdl_enabled(), p)
-                           : launch(select_blocks_kernel<256>, each, dim3(kPick), 0, stream, pdl_enabled(), p);
-    else if (e == cudaSuccess) e = launch(pick_blocks_kernel, each, dim3(kPick), 0, stream, true, p);
-    if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of select_blocks (q8) failed: %s", cudaGetErrorString(e));
     return TS_OK;
 }
 

@@ -323,7 +323,9 @@ def rows_unpack_q8(kv: RowsQ8, slots, positions, kept: Kept):
     return k_out, v_out
 
 
-def _heads_of(q, kv_heads: int, width: int) -> tuple:
+def _heads_of(q, kv_heads: int, width: int, keys: int) -> tuple:
+    if not 0 <= keys <= FAR:
+        _refuse(f"{keys} keys")
     shape = q.shape
     if len(shape) != 3 or shape[2] != width or shape[1] % kv_heads:
         _refuse(f"q {list(shape)} does not go with {kv_heads} kv heads of width {width}")
@@ -334,7 +336,7 @@ def attend_rows_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, *, sc
     """Ragged causal attention over 8-bit kept rows, q and result bf16 [rows, heads, width]: ts_attend_rows_q8."""
     record, dev, kv_heads, _, width = kv._held
     stream = _q8_stream(dev)
-    rows, heads = _heads_of(q, kv_heads, width)
+    rows, heads = _heads_of(q, kv_heads, width, keys)
     a_q = _at(q, _BF16, rows * heads * width, dev, "q")
     if out is None:
         out = torch.empty_like(q)
@@ -355,7 +357,7 @@ def select_blocks_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, cou
     (UINT32_MAX) in spare entries: ts_select_blocks_q8."""
     record, dev, kv_heads, block, width = kv._held
     stream = _q8_stream(dev)
-    rows, heads = _heads_of(q, kv_heads, width)
+    rows, heads = _heads_of(q, kv_heads, width, keys)
     a_q = _at(q, _BF16, rows * heads * width, dev, "q")
     a_slots, a_pos = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
     ids = q.new_empty((rows, kv_heads, max(count, 0)), dtype=torch.int32)
@@ -371,7 +373,7 @@ def attend_blocks_q8(q, kv: RowsQ8, ids, slots, positions, kept: Kept, keys: int
     """Causal attention over the listed blocks only (ids int32 [rows, kv_heads, count], -1 = none): ts_attend_blocks_q8."""
     record, dev, kv_heads, block, width = kv._held
     stream = _q8_stream(dev)
-    rows, heads = _heads_of(q, kv_heads, width)
+    rows, heads = _heads_of(q, kv_heads, width, keys)
     count = ids.shape[-1]
     a_q = _at(q, _BF16, rows * heads * width, dev, "q")
     if out is None:

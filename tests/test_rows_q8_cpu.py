@@ -89,6 +89,24 @@ def test_buffers_and_counts_are_checked(world):
         refused(_lib, lib.ts_select_blocks_q8(p, good, p, p, p, paged, 1, 64, 4, 2, 64, count, first, recent, None, 0, None), "blocks (1 to 4096)")
     refused(_lib, lib.ts_select_blocks_q8(p, good, p, p, p, paged, 1, 64, 514, 2, 64, 1, 0, 0, None, 0, None), "at most 256")
     refused(_lib, lib.ts_select_blocks_q8(p, good, p, p, p, long, 1, 100000, 4, 2, 64, 2, 0, 0, None, 0, None), "workspace")
+    for i in range(5):  # gains, frequencies, slots, positions, ids, page table
+        o = [p + 2 if k == i else p for k in range(5)]
+        refused(_lib, lib.ts_qk_norm_rope_append_q8(p, *o, p + 2048, good, paged, 1, 4, 2, 64, 1e-6, None), "4-byte")
+    for i in range(2):
+        o = [p + 2 if k == i else p for k in range(2)]
+        refused(_lib, lib.ts_rows_unpack_q8(good, *o, p, p, paged, 1, 2, 64, None), "4-byte")
+        refused(_lib, lib.ts_attend_rows_q8(p, good, p, *o, paged, 1, 64, 4, 2, 64, 0, 1.0, None, 0, None), "4-byte")
+        refused(_lib, lib.ts_attend_blocks_q8(p, good, p, p, *o, paged, 1, 64, 4, 2, 64, 1, 1.0, None, 0, None), "4-byte")
+    refused(_lib, lib.ts_attend_blocks_q8(p, good, p + 2, p, p, p, paged, 1, 64, 4, 2, 64, 1, 1.0, None, 0, None), "4-byte")
+    for i in range(3):
+        o = [p + 2 if k == i else p for k in range(3)]
+        refused(_lib, lib.ts_select_blocks_q8(p, good, *o, paged, 1, 64, 4, 2, 64, 1, 0, 0, None, 0, None), "4-byte")
+    odd = _lib.TsKept(2, 64, 2, p + 2, 4, 128)
+    refused(_lib, lib.ts_rows_unpack_q8(good, p, p, p, p, odd, 1, 2, 64, None), "4-byte")
+    # results over inputs that other blocks still read
+    refused(_lib, lib.ts_qk_norm_rope_append_q8(p, None, None, p, p, p, p, good, paged, 1, 4, 2, 64, 1e-6, None), "where qkv lies")
+    refused(_lib, lib.ts_attend_rows_q8(p, good, p, p, p, paged, 1, 64, 4, 2, 64, 0, 1.0, None, 0, None), "where q lies")
+    refused(_lib, lib.ts_attend_blocks_q8(p, good, p, p, p, p, paged, 1, 64, 4, 2, 64, 1, 1.0, None, 0, None), "where q lies")
     # no rows: nothing to do, and nothing of the GPU is touched
     assert lib.ts_attend_rows_q8(p, good, p, p, p, paged, 0, 64, 4, 2, 64, 0, 1.0, None, 0, None) == 0
     assert lib.ts_rows_unpack_q8(good, p, p, p, p, paged, 0, 2, 64, None) == 0

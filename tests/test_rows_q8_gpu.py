@@ -377,6 +377,80 @@ def test_attention_of_queries_of_any_size():
     assert torch.isnan(got[0, 0].float()).all() and torch.isfinite(got[0, 1].float()).all()
 
 
+@pytest.mark.parametrize("case", [(4, 4, 128, 64, 64, "dense"), (16, 2, 128, 32, 64, "paged"), (5, 1, 64, 16, 16, "paged"), (8, 1, 256, 64, 64, "dense")],
+                         ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("each", [1, 3])
+def test_attention_where_later_keys_score_higher(case, each):
+    """Every head's query along one channel that the keys climb (or fall, or jump over), by up to 2^9 a block of positions."""
+    from tessera_b200 import ops
+    rng = np.random.default_rng(20)
+    heads, kv_heads, width, block = case[:4]
+    n = 1000
+    kv, kept, store = attend_case(rng, case, [n])
+    at = np.array([store.at(0, b) for b in range(n // block)])
+    kv.k.zero_()
+    kv.k_scale.fill_(1.0)
+    q = torch.zeros((each, heads, width), dtype=torch.bfloat16, device="cuda")
+    q[:, :, 7] = 1.0
+    for path in (np.linspace(0, 127, len(at)), np.linspace(127, -127, len(at)), np.where(np.arange(len(at)) % 5 == 4, 100, -100) + np.arange(len(at)) // 3,
+                 np.where(np.arange(len(at)) == len(at) - 2, 127, np.arange(len(at)) % 7)):
+        codes = torch.from_numpy(np.rint(path).astype(np.int8)).cuda()
+        kv.k[torch.from_numpy(at).cuda(), :, :, 7] = codes[:, None, None]
+        store = M.Store(kv, store.layout, store.scalar, store.page, store.table)
+        pos = list(range(n - each, n))
+        # a score of 15 a step at most in powers of two: the products are whole numbers times the scale, exact
+        for scale in (0.02, 0.1):
+            got = ops.attend_rows_q8(q, kv, dev_u32([0] * each), dev_u32(pos), kept, n, scale=scale)
+            want, tol = M.attend(store, np64(q), [0] * each, pos, n, scale)
+            check_attend(got, want, tol)
+
+
+COLD = """
+import torch
+from tessera_b200 import ops
+kv = ops.RowsQ8.empty({pages} * 64, 2, 128, 64)
+kept = ops.Kept("dense", {pages} * 64, None, {pages} * 64)
+at, pos = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full((1,), {pages} * 64 - 1, dtype=torch.int32, device="cuda")
+qkv, freq = torch.ones((1, 8 * 128), dtype=torch.bfloat16, device="cuda"), torch.ones(64, device="cuda")
+g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+torch.cuda.synchronize()
+with torch.cuda.graph(g, stream=side):
+    q = ops.qk_norm_rope_append_q8(qkv, None, None, freq, at, pos, kv, kept, 4, eps=1e-6)
+    a = ops.attend_rows_q8(q, kv, at, pos, kept, {pages} * 64, scale=0.1)
+    ids = ops.select_blocks_q8(q, kv, at, pos, kept, {pages} * 64, 4)
+    b = ops.attend_blocks_q8(q, kv, ids, at, pos, kept, {pages} * 64, scale=0.1)
+    k, v = ops.rows_unpack_q8(kv, at, pos, kept)
+for _ in range(2):
+    g.replay()
+torch.cuda.synchronize()
+assert ids[0, 0, 3].item() == {pages} - 1 and (v.float() == 1).all() and a.float().abs().max() > 0 and b.float().abs().max() > 0
+print("replayed")
+"""
+
+
+@pytest.mark.parametrize("pages", [8, 700])
+def test_the_first_calls_of_a_process_may_be_captured(pages):
+    import subprocess
+    import sys
+    run = subprocess.run([sys.executable, "-c", COLD.format(pages=pages)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "replayed" in run.stdout, run.stderr[-2000:]
+
+
+def test_more_rows_than_one_launch_chooses_for():
+    from tessera_b200 import ops
+    rng = np.random.default_rng(21)
+    case = (2, 1, 64, 16, 16, "dense")
+    rows = 70001
+    for length in (160, 520 * 16):  # one kernel, and two
+        kv, kept, store = attend_case(rng, case, [length])
+        q = bf16(rng, 3, 2, 64).repeat(-(-rows // 3), 1, 1)[:rows].contiguous()
+        pos = torch.full((rows,), length - 1, dtype=torch.int32, device="cuda")
+        got = ops.select_blocks_q8(q, kv, torch.zeros_like(pos), pos, kept, length, 3)
+        want = M.select(store, np64(q[:3]), [0] * 3, [length - 1] * 3, length, 3, 1, 1)
+        want = torch.from_numpy(want.astype(np.int32)).cuda().repeat(-(-rows // 3), 1, 1)[:rows]
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("case", [(16, 8, 128, 16, 64, "paged"), (8, 1, 64, 32, 32, "paged"), (32, 4, 128, 64, 64, "paged"),
                                   (4, 2, 256, 64, 128, "dense"), (3, 1, 256, 16, 16, "paged")], ids=lambda c: "-".join(map(str, c)))
 @pytest.mark.parametrize("count,first,recent", [(1, 0, 0), (1, 0, 1), (3, 1, 1), (7, 0, 2), (40, 2, 3), (300, 1, 1)])
@@ -630,6 +704,8 @@ def test_python_refusals_on_the_device():
         lambda: ops.attend_rows_q8(q, kv, at, at, ops.Kept("interleaved", 2, None, 128), 64, scale=1.0),
         lambda: ops.attend_rows_q8(q, kv, at, at, ops.Kept("dense", 40, None, 128), 64, scale=1.0),
         lambda: ops.attend_rows_q8(q, kv, at, at, ops.Kept("paged", 2, at, 128, page=8), 64, scale=1.0),
+        lambda: ops.attend_rows_q8(q, kv, at, at, kept, -1, scale=1.0),
+        lambda: ops.attend_rows_q8(q, kv, at, at, kept, 64, scale=1.0, out=q),
         lambda: ops.select_blocks_q8(q, bare, at, at, kept, 64, 2),
         lambda: ops.select_blocks_q8(q, kv, at, at, kept, 64, 1, first=1, recent=1),
         lambda: ops.select_blocks_q8(q, kv, at, at, kept, 64, 0, first=0, recent=0),
