@@ -35,11 +35,12 @@
 // every run.
 //
 // What bounds it, measured with width 128.  Many decode rows: the codes' bytes (64 rows of up to 8192 keys, 8 kv heads of 2
-// heads: 134 us, 0.92 of the copy rate; 4 rows of up to 100003 keys, 8 kv heads of 4: 109 us, 0.90).  Listed blocks: the
-// same, in blocks that lie scattered, with a merge (64 rows x 4 kv heads x 64 blocks of 64: 61 us, 0.68).
+// heads: 138 us, 0.90 of the copy rate; 4 rows of up to 100003 keys, 8 kv heads of 4: 110 us, 0.89).  Listed blocks: the
+// same, in blocks that lie scattered, with a merge (64 rows x 4 kv heads x 64 blocks of 64: 58 us, 0.70).
 // Drafted tokens, where 16 queries share each key: the instructions around the products (16 slots x 7 rows of up to 4099 keys,
-// 4 kv heads of 8: 58 us, 0.14 of the copy rate, an instruction in 0.35 of the cycles from two warps a scheduler, which is
-// what their registers leave).
+// 4 kv heads of 8: 53 us, 0.15 of the copy rate, an instruction in a third of the cycles from two warps a scheduler, which
+// is what their registers leave).  Fewer instructions a step also draw less power: at the board's limit, where the clock
+// gives way, 64 x 8192 went from 150 us to 142 with one look-up, copy and scale a step and two stages.
 #include <cmath>
 
 #include "rows_q8.cuh"
@@ -54,10 +55,11 @@ __device__ constexpr uint32_t kRuns[6] = {1, 2, 3, 4, 6, 8};
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kScaleFloor = 8.673617379884035e-19f;  // 2^-60
 
-// Eight warps with three stages each fill an SM's shared memory (two blocks of 96 KB).  Twelve warps with two stages were
-// slower everywhere (64 rows x 8192 positions: 156 us against 145): they leave 168 registers a thread, which spills, and
-// a second tile behind every wait.  Six warps with four stages: 149.
-constexpr int kBlocks = 2, kStages = 3;
+// Eight warps, with two stages each, have 128 KB an SM under way, several times what the memory's latency asks for.  A third
+// stage made the reads less orderly and slower (64 rows x 8192 positions: 145 us against 140).  Twelve warps leave 168
+// registers a thread, which spills (156 us), six warps hide too little of a step's arithmetic (149).  Runs at the end that
+// whoever is done first claims from a counter even out the SMs' shares of the memory's rate, but cost what they gain.
+constexpr int kBlocks = 2, kStages = 2;
 
 struct AttendParams {
     const uint16_t *q;
@@ -316,15 +318,18 @@ __device__ __forceinline__ uint32_t piece_at(uint32_t tile, int u, int c, uint32
 }
 
 // A step's scores in powers of two with the value scale's exponent.  EDGE: some key of the step is not seen by some row.  A
-// unit without keys has key0 past every row's.
-template <int W, int NT, bool EDGE>
-__device__ __forceinline__ void score_step(const Queries<W, NT> &qs, uint32_t tile, const float (&ks)[Step<W>::UNITS],
-                                           const float (&vs)[Step<W>::UNITS], const uint32_t (&key0)[Step<W>::UNITS],
-                                           float (&x)[Step<W>::UNITS][NT][4], uint32_t lane) {
+// unit without keys has key0 past every row's.  N: the blocks a step may lie in, one (all its units) or one a unit.
+template <int W, int NT, int N, bool EDGE>
+__device__ __forceinline__ void score_step(const Queries<W, NT> &qs, uint32_t tile, const float (&ks)[N], const float (&vs)[N],
+                                           const uint32_t (&key0)[N], float (&x)[Step<W>::UNITS][NT][4], uint32_t lane) {
     constexpr int U = Step<W>::UNITS;
     const uint32_t r = lane >> 2;
+    float lv[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) lv[n] = log2_approx(fmaxf(vs[n], kScaleFloor));
 #pragma unroll
     for (int u = 0; u < U; u++) {
+        const int n = N == 1 ? 0 : u;
         int high[NT][4], low[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; t++)
@@ -340,17 +345,16 @@ __device__ __forceinline__ void score_step(const Queries<W, NT> &qs, uint32_t ti
                 mma_s8(low[t], a, qs.b[t][c / 2][1]);
             }
         }
-        const float lv = log2_approx(fmaxf(vs[u], kScaleFloor));
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float f = qs.f[t][e] * ks[u];
+                const float f = qs.f[t][e] * ks[n];
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    float y = fmaf(__int2float_rn(high[t][2 * k + e] * 256 + low[t][2 * k + e]), f, lv);
+                    float y = fmaf(__int2float_rn(high[t][2 * k + e] * 256 + low[t][2 * k + e]), f, lv[n]);
                     if (EDGE) {
-                        const uint32_t key = key0[u] + 8 * k + r;
+                        const uint32_t key = key0[n] + (N == 1 ? 16 * u : 0) + 8 * k + r;
                         if (key < qs.lo[t][e] || key >= qs.hi[t][e]) y = -INFINITY;
                     }
                     x[u][t][2 * k + e] = y;
@@ -364,8 +368,8 @@ __device__ __forceinline__ void score_step(const Queries<W, NT> &qs, uint32_t ti
 // touch the output (16 rows found a new maximum in every other step: 61 us for 16 x 7 rows of up to 4099 keys, 58.5 so).  2^(x - M) then reaches 2^kSlack, well within f16.
 constexpr float kSlack = 8.0f;
 
-template <int W, int NT>
-__device__ __forceinline__ void soften(Running<W, NT> &run, const float (&x)[Step<W>::UNITS][NT][4], const float (&vs)[Step<W>::UNITS],
+template <int W, int NT, int N>
+__device__ __forceinline__ void soften(Running<W, NT> &run, const float (&x)[Step<W>::UNITS][NT][4], const float (&vs)[N],
                                        uint32_t (&b)[Step<W>::UNITS][NT][2]) {
     constexpr int U = Step<W>::UNITS;
     float most[NT][2];
@@ -402,9 +406,11 @@ __device__ __forceinline__ void soften(Running<W, NT> &run, const float (&x)[Ste
     for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int e = 0; e < 2; e++) top[t][e] = run.m[t][e] == -INFINITY ? 0.0f : run.m[t][e];  // nothing seen yet: 2^(-inf - 0) = 0
+    float inv[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) inv[n] = __fdividef(1.0f, fmaxf(vs[n], kScaleFloor));
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const float inv = __fdividef(1.0f, fmaxf(vs[u], kScaleFloor));
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             float p[4];
@@ -412,7 +418,7 @@ __device__ __forceinline__ void soften(Running<W, NT> &run, const float (&x)[Ste
             for (int e = 0; e < 2; e++) {
                 p[e] = exp2_approx(x[u][t][e] - top[t][e]);
                 p[2 + e] = exp2_approx(x[u][t][2 + e] - top[t][e]);
-                run.l[t][e] = fmaf(p[e] + p[2 + e], inv, run.l[t][e]);
+                run.l[t][e] = fmaf(p[e] + p[2 + e], inv[N == 1 ? 0 : u], run.l[t][e]);
             }
             b[u][t][0] = transpose_8x8(pack_f16(p[0], p[1]));
             b[u][t][1] = transpose_8x8(pack_f16(p[2], p[3]));
@@ -441,7 +447,7 @@ __device__ __forceinline__ void value_step(Running<W, NT> &run, uint32_t tile, c
 }
 
 // 32 blocks' places in the pool and scales, one a lane: entry `first` + lane of the tile's blocks.
-constexpr uint32_t kNoKeys = 0xFFFFFFF0u;  // a unit's first key where there is no block: no row sees it
+constexpr uint32_t kNoKeys = 0xFFFFFF00u;  // a unit's first key where there is no block: rows see less (attend_q8 sees to it)
 
 struct Group {
     uint32_t blk, id;  // pool block or kNoBlock; which block of the slot's positions it is
@@ -491,12 +497,15 @@ struct Following {
 };
 
 // Computes a segment, `asked` of whose steps are already on their way, and returns how many of the following one's are.
-template <int W, int NT, bool LIST>
+// ONE: every step lies within one block.  follow() fills `then` in; it is called once the segment's own copies have all been
+// asked for, so that its look-ups wait while they are under way.
+template <int W, int NT, bool LIST, bool ONE, class Follow>
 __device__ __forceinline__ uint32_t attend_steps(const AttendParams &p, const CUtensorMap *map_k, const CUtensorMap *map_v, const Segment &seg,
-                                                 Group now, uint32_t asked, const Following &then, Ring &ring, int *status,
-                                                 uint32_t lane) {
+                                                 Group now, uint32_t asked, const Following &then, Follow &&follow, Ring &ring,
+                                                 int *status, uint32_t lane) {
     using namespace ptx;
     constexpr int KEYS = Step<W>::KEYS, U = Step<W>::UNITS, HALVES = Step<W>::HALVES, COLS = Step<W>::COLS, STAGES = kStages;
+    constexpr int N = ONE ? 1 : U, SPAN = U / N;  // blocks a step may lie in, units of each
     const Tile &tile = seg.tile;
     const uint32_t kvh = seg.kvh, head0 = seg.head0, part = seg.part, begin = seg.begin, end = seg.end;
     const uint32_t in_block = p.kv.shift - 4;  // log2 of a block's 16-key units
@@ -513,50 +522,54 @@ __device__ __forceinline__ uint32_t attend_steps(const AttendParams &p, const CU
         uint32_t first = (begin * U) >> in_block;  // entry of lane 0 of the current group
         const RawQueries<W, NT> raw = fetch_queries<W, NT>(p, tile, head0, part, lane);
         Group next = now;  // the first copies lie in the current group
-        const uint32_t per = 1u << in_block, span = per < (uint32_t)U ? per : U;  // units of one copy
+        const uint32_t per = 1u << in_block, span = ONE ? U : per < (uint32_t)U ? per : U;  // units of one copy
         constexpr bool CHAIN = NT == 1;  // with sixteen rows the registers for it cost more than it saves (62 us for 58)
-        const uint32_t last = CHAIN ? end + then.steps : end;
+        uint32_t last = end;
+        bool followed = !CHAIN;
         // Step s's units as rows of the tensor maps, -1 where there is no block; the current or the next group has its
         // blocks, or what follows does.
-        auto find = [&](uint32_t s, int32_t (&y)[U]) {
+        auto find = [&](uint32_t s, int32_t (&y)[N]) {
             const bool mine = !CHAIN || s < end;
             const uint32_t unit = (mine ? s : then.begin + (s - end)) * U, head = mine ? kvh : then.kvh;
             const uint32_t from = mine ? first : (then.begin * U) >> in_block;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                y[u] = -1;
-                if ((u & (span - 1)) != 0) continue;  // lies in the copy of the unit before it
-                const uint32_t e = ((unit + u) >> in_block) - from;
+            for (int n = 0; n < N; n++) {
+                y[n] = -1;
+                if (!ONE && (n & (span - 1)) != 0) continue;  // lies in the copy of the unit before it
+                const uint32_t e = ((unit + n) >> in_block) - from;
                 const uint32_t blk = __shfl_sync(0xFFFFFFFFu, !mine ? then.group.blk : e < 32 ? now.blk : next.blk, e & 31);
-                if (blk != kNoBlock) y[u] = (int32_t)(((blk * p.kv_heads + head) << p.kv.shift) + (((unit + u) & (per - 1)) << 4));
+                if (blk != kNoBlock) y[n] = (int32_t)(((blk * p.kv_heads + head) << p.kv.shift) + (((unit + n) & (per - 1)) << 4));
             }
         };
         // Copies of a step's K (values = 0) or V (1) into stage `at`.
-        auto copy = [&](uint32_t at, const int32_t (&y)[U], const CUtensorMap *map, int values) {
+        auto copy = [&](uint32_t at, const int32_t (&y)[N], const CUtensorMap *map, int values) {
             if (lane == 0) {
                 uint64_t *bar = &ring.full[values * STAGES + at];
                 const uint32_t dst = ring.tiles + at * kStage + values * kHalfStage;
                 uint32_t bytes = 0;
 #pragma unroll
-                for (int u = 0; u < U; u++)
-                    if (y[u] >= 0) bytes += span * 16 * W;
+                for (int n = 0; n < N; n++)
+                    if (y[n] >= 0) bytes += span * 16 * W;
                 mbar_expect_tx(bar, bytes);
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (y[u] < 0) continue;
+                for (int n = 0; n < N; n++) {
+                    if (y[n] < 0) continue;
 #pragma unroll
-                    for (int h = 0; h < HALVES; h++) copy_codes(dst + (h * KEYS + 16 * u) * COLS, map, smem_addr(bar), h * COLS, y[u]);
+                    for (int h = 0; h < HALVES; h++) copy_codes(dst + (h * KEYS + 16 * n) * COLS, map, smem_addr(bar), h * COLS, y[n]);
                 }
             }
         };
-        int32_t y[U];
+        int32_t y[N];
         uint32_t ahead = begin + asked;  // the next step to ask for; from `end` on, of what follows
-        for (; ahead < last && ahead < begin + STAGES; ahead++) {
-            const uint32_t at = (ring.stage + (ahead - begin)) % STAGES;
-            find(ahead, y);
-            copy(at, y, map_k, 0);
-            copy(at, y, map_v, 1);
-        }
+        auto fill = [&](uint32_t s) {  // the stages that are free at step s
+            for (; ahead < last && ahead < s + STAGES; ahead++) {
+                const uint32_t at = (ring.stage + (ahead - s)) % STAGES;
+                find(ahead, y);
+                copy(at, y, map_k, 0);
+                copy(at, y, map_v, 1);
+            }
+        };
+        fill(begin);
         next = group_of<LIST>(p, tile, kvh, first + 32, lane);
         Queries<W, NT> qs;
         load_queries<W, NT>(p, tile, raw, part, lane, qs);
@@ -566,30 +579,39 @@ __device__ __forceinline__ uint32_t attend_steps(const AttendParams &p, const CU
             seen(p, p.positions[tile.row], &x, &all_hi);
             seen(p, p.positions[tile.row + tile.tokens - 1], &all_lo, &x);
         }
+        // Keys [k, k + 16 SPAN) are all seen where k - inner_lo <= inner; nowhere: k is a multiple of 16, never 1.
+        const bool any_inner = all_hi >= 16 * SPAN && all_lo <= all_hi - 16 * SPAN;
+        const uint32_t inner_lo = any_inner ? all_lo : 1, inner = any_inner ? all_hi - 16 * SPAN - all_lo : 0;
         for (uint32_t s = begin; s < end; s++) {
             if (((s * U) >> in_block) - first >= 32) {
                 first += 32;
                 now = next;
                 next = group_of<LIST>(p, tile, kvh, first + 32, lane);
             }
-            float ks[U], vs[U];
-            uint32_t key0[U];
+            if (!followed && ahead >= end) {
+                follow();
+                followed = true;
+                last = end + then.steps;
+                fill(s);
+            }
+            float ks[N], vs[N];
+            uint32_t key0[N];
             bool edge = false;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const uint32_t unit = s * U + u;
-                if (u == 0 || (unit & (per - 1)) == 0) {  // another block
+            for (int n = 0; n < N; n++) {
+                const uint32_t unit = s * U + n;
+                if (n == 0 || (unit & (per - 1)) == 0) {  // another block
                     const uint32_t e = ((unit >> in_block) - first) & 31;
-                    ks[u] = __shfl_sync(0xFFFFFFFFu, now.ks, e);
-                    vs[u] = __shfl_sync(0xFFFFFFFFu, now.vs, e);
+                    ks[n] = __shfl_sync(0xFFFFFFFFu, now.ks, e);
+                    vs[n] = __shfl_sync(0xFFFFFFFFu, now.vs, e);
                     const uint32_t id = __shfl_sync(0xFFFFFFFFu, now.blk == kNoBlock ? kNoBlock : now.id, e);
-                    key0[u] = id == kNoBlock ? kNoKeys : (id << p.kv.shift) + ((unit & (per - 1)) << 4);
+                    key0[n] = id == kNoBlock ? kNoKeys : (id << p.kv.shift) + ((unit & (per - 1)) << 4);
                 } else {
-                    ks[u] = ks[u - (u > 0)];
-                    vs[u] = vs[u - (u > 0)];
-                    key0[u] = key0[u - (u > 0)] == kNoKeys ? kNoKeys : key0[u - (u > 0)] + 16;
+                    ks[n] = ks[n - (n > 0)];
+                    vs[n] = vs[n - (n > 0)];
+                    key0[n] = key0[n - (n > 0)] == kNoKeys ? kNoKeys : key0[n - (n > 0)] + 16;
                 }
-                edge = edge || key0[u] < all_lo || key0[u] > all_hi - 16 || all_hi < 16;
+                edge = edge || key0[n] - inner_lo > inner;
             }
             const uint32_t at = ring.tiles + ring.stage * kStage, odd = ring.parity >> ring.stage & 1;
             ring.parity ^= 1u << ring.stage;
@@ -611,15 +633,15 @@ __device__ __forceinline__ uint32_t attend_steps(const AttendParams &p, const CU
                 return 0;
             }
             float x[U][NT][4];
-            if (edge) score_step<W, NT, true>(qs, at, ks, vs, key0, x, lane);
-            else score_step<W, NT, false>(qs, at, ks, vs, key0, x, lane);
+            if (edge) score_step<W, NT, N, true>(qs, at, ks, vs, key0, x, lane);
+            else score_step<W, NT, N, false>(qs, at, ks, vs, key0, x, lane);
             __syncwarp();
             if (ahead < last) {
                 find(ahead, y);
                 copy(ring.stage, y, map_k, 0);
             }
             uint32_t b[U][NT][2];
-            soften<W, NT>(run, x, vs, b);
+            soften<W, NT, N>(run, x, vs, b);
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(&ring.full[STAGES + ring.stage], odd))) {
                 give_up(true);
                 return 0;
@@ -662,7 +684,7 @@ __device__ __forceinline__ uint32_t attend_steps(const AttendParams &p, const CU
     return early;
 }
 
-template <int W, bool LIST>
+template <int W, bool LIST, bool ONE>
 __global__ void __launch_bounds__(kThreads, kBlocks)
 attend_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttendParams p, int *status) {
     using namespace ptx;
@@ -803,18 +825,23 @@ attend_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             uint32_t asked = 0;
             while (any && ring.ok) {
                 Segment next;
-                const bool more = next_segment(&next);
+                bool more = false, followed = false;
                 Following then = {{kNoBlock, 0, 0.0f, 0.0f}, 0, 0, 0};
-                if (more) {
-                    then.group = group_for(next);
-                    then.begin = next.begin;
-                    then.steps = next.tile.from < next.tile.to ? min(next.end - next.begin, (uint32_t)kStages) : 0;
-                    then.kvh = next.kvh;
-                }
+                auto follow = [&] {
+                    followed = true;
+                    more = next_segment(&next);
+                    if (more) {
+                        then.group = group_for(next);
+                        then.begin = next.begin;
+                        then.steps = next.tile.from < next.tile.to ? min(next.end - next.begin, (uint32_t)kStages) : 0;
+                        then.kvh = next.kvh;
+                    }
+                };
                 if (now.tile.tokens * now.part <= 8)
-                    asked = attend_steps<W, 1, LIST>(p, &map_k, &map_v, now, group, asked, then, ring, status, lane);
+                    asked = attend_steps<W, 1, LIST, ONE>(p, &map_k, &map_v, now, group, asked, then, follow, ring, status, lane);
                 else
-                    asked = attend_steps<W, 2, LIST>(p, &map_k, &map_v, now, group, asked, then, ring, status, lane);
+                    asked = attend_steps<W, 2, LIST, ONE>(p, &map_k, &map_v, now, group, asked, then, follow, ring, status, lane);
+                if (!followed) follow();
                 // who has a tile's first step says where its partials are
                 if (now.begin == 0 && p.merged && lane < now.tile.tokens)
                     p.places[(size_t)(now.tile.row + lane) * per_row + now.unit] =
@@ -910,7 +937,7 @@ __global__ void __launch_bounds__(kMergeThreads) attend_q8_merge_kernel(const At
 // Few and short rows: a cluster of blocks has one row and kv head (or part of its heads), its warps cut the steps among them,
 // and the partial results meet through distributed shared memory: one launch, no pass over the rows, no workspace.  One row
 // of 517 keys: 9.0 us, 8 rows x 32 listed blocks of 16: 9.9; both wait for one load after another (position, page, scale, codes).
-template <int W, bool LIST>
+template <int W, bool LIST, bool ONE>
 __global__ void __launch_bounds__(kThreads, kBlocks)
 attend_q8_cluster_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttendParams p, int *status) {
     using namespace ptx;
@@ -950,6 +977,7 @@ attend_q8_cluster_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     seg.begin = worker * each;
     seg.end = min(t.steps, seg.begin + each);
     seg.partial = true;
+    static_assert(16 * W * sizeof(float) <= kStages * kStage, "a warp's ring holds its partial results");
     seg.part_o = reinterpret_cast<float *>(smem + warp * (kStages * kStage));  // its ring is empty by then
     seg.part_ml = reinterpret_cast<float *>(sm_ml[warp]);
     if (lane < 16) sm_ml[warp][lane] = make_float2(-INFINITY, 0.0f);
@@ -957,8 +985,8 @@ attend_q8_cluster_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     if (seg.begin < seg.end && t.from < t.to) {
         const Group group = group_of<LIST>(p, t, seg.kvh, (seg.begin * Step<W>::UNITS) >> (p.kv.shift - 4), lane);
         const Following none = {{kNoBlock, 0, 0.0f, 0.0f}, 0, 0, 0};
-        if (seg.part <= 8) attend_steps<W, 1, LIST>(p, &map_k, &map_v, seg, group, 0, none, ring, status, lane);
-        else attend_steps<W, 2, LIST>(p, &map_k, &map_v, seg, group, 0, none, ring, status, lane);
+        if (seg.part <= 8) attend_steps<W, 1, LIST, ONE>(p, &map_k, &map_v, seg, group, 0, none, [] {}, ring, status, lane);
+        else attend_steps<W, 2, LIST, ONE>(p, &map_k, &map_v, seg, group, 0, none, [] {}, ring, status, lane);
     }
     cluster_sync();
     // Block `rank` folds its share of the row's heads' channels, four at a time, in the order of the keys: worker = warp *
@@ -1037,12 +1065,12 @@ Plan plan_of(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, ui
     return s;
 }
 
-template <int W, bool LIST>
+template <int W, bool LIST, bool ONE>
 int launch_attend(const AttendParams &p, cudaStream_t stream) {
     constexpr size_t smem = kWarps * kStages * kStage;
     static OncePerDevice configured;
     if (configured.needs()) {
-        TS_CUDA(cudaFuncSetAttribute(attend_q8_kernel<W, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        TS_CUDA(cudaFuncSetAttribute(attend_q8_kernel<W, LIST, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         configured.done();
     }
     int *status = nullptr;
@@ -1057,7 +1085,7 @@ int launch_attend(const AttendParams &p, cudaStream_t stream) {
     if (p.cluster) {
         static OncePerDevice ready;
         if (ready.needs()) {
-            TS_CUDA(cudaFuncSetAttribute(attend_q8_cluster_kernel<W, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            TS_CUDA(cudaFuncSetAttribute(attend_q8_cluster_kernel<W, LIST, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             ready.done();
         }
         cudaLaunchAttribute attr[2] = {};
@@ -1073,18 +1101,27 @@ int launch_attend(const AttendParams &p, cudaStream_t stream) {
         cfg.stream = stream;
         cfg.attrs = attr;
         cfg.numAttrs = pdl_enabled() ? 2 : 1;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, attend_q8_cluster_kernel<W, LIST>, map_k, map_v, p, status);
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, attend_q8_cluster_kernel<W, LIST, ONE>, map_k, map_v, p, status);
         if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of attend (q8, cluster) failed: %s", cudaGetErrorString(e));
         return TS_OK;
     }
     const uint32_t grid = min(p.workers, (uint32_t)sm_count() * kBlocks);
-    cudaError_t e = launch(attend_q8_kernel<W, LIST>, dim3(grid), dim3(kThreads), smem, stream, pdl_enabled(), map_k, map_v, p, status);
+    cudaError_t e = launch(attend_q8_kernel<W, LIST, ONE>, dim3(grid), dim3(kThreads), smem, stream, pdl_enabled(), map_k, map_v, p, status);
     if (e == cudaSuccess && p.merged)  // always as a dependent launch: it waits for the partials itself
         e = p.rows * p.heads > (uint32_t)sm_count() * 8
                 ? launch(attend_q8_merge_kernel<W, 64>, dim3(p.rows * p.heads), dim3(64), p.workers * sizeof(float), stream, true, p)
                 : launch(attend_q8_merge_kernel<W, 256>, dim3(p.rows * p.heads), dim3(256), p.workers * sizeof(float), stream, true, p);
     if (e != cudaSuccess) return fail(TS_ERR_CUDA, "launch of attend (q8) failed: %s", cudaGetErrorString(e));
     return TS_OK;
+}
+
+// Blocks that hold whole steps of keys need one look-up, copy and scale a step.
+template <int W>
+int launch_attend(const AttendParams &p, cudaStream_t stream) {
+    if (Step<W>::UNITS == 1 || (1u << p.kv.shift) >= (uint32_t)Step<W>::KEYS)
+        return p.ids ? launch_attend<W, true, true>(p, stream) : launch_attend<W, false, true>(p, stream);
+    if constexpr (Step<W>::UNITS > 1)
+        return p.ids ? launch_attend<W, true, false>(p, stream) : launch_attend<W, false, false>(p, stream);
 }
 
 }  // namespace
@@ -1109,6 +1146,7 @@ int attend_q8(const void *q, const RowsQ8Dev &kv, const uint32_t *ids, void *out
     // A slot has no keys past what its stride or its pages hold (and fewer keys never ask for a larger workspace).
     const uint64_t room = (uint64_t)kv.scalar << (kv.per_shift + kv.shift);
     if (room < keys) keys = (uint32_t)room;
+    if (keys > kNoKeys) keys = kNoKeys;
     const Plan s = plan_of(rows, keys, heads, kv_heads, width, back, count, 1u << kv.shift);
     const size_t need = s.bytes();
     TS_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace != nullptr && aligned16(workspace))),
@@ -1152,9 +1190,9 @@ int attend_q8(const void *q, const RowsQ8Dev &kv, const uint32_t *ids, void *out
         p.slots = slots + row;
         p.positions = positions + row;
         p.rows = min(s.together, rows - row);
-        const int rc = width == 64    ? (ids ? launch_attend<64, true>(p, stream) : launch_attend<64, false>(p, stream))
-                       : width == 128 ? (ids ? launch_attend<128, true>(p, stream) : launch_attend<128, false>(p, stream))
-                                      : (ids ? launch_attend<256, true>(p, stream) : launch_attend<256, false>(p, stream));
+        const int rc = width == 64    ? launch_attend<64>(p, stream)
+                       : width == 128 ? launch_attend<128>(p, stream)
+                                      : launch_attend<256>(p, stream);
         if (rc != TS_OK) return rc;
     }
     return TS_OK;
