@@ -16,7 +16,7 @@
 // 1152 is subtracted.
 //
 // The scales leave the products alone.  With s = raw * scale * k_scale in powers of two and
-//     x = s + log2(v_scale),   M ~ max x,   P = 2^(x - M)   (f16 operand of P V)
+//     x = s + log2(v_scale),   M ~ max x - 7,   P = 2^(x - M)   (f16 operand of P V)
 // the output is sum(P code) / sum(P / v_scale): the block's value scale rides in the exponent, so that P needs no second
 // factor and stays within f16's range whatever the scales are, and M cancels.  A scale of zero counts as 2^-60, the
 // smallest that append writes.  (The second sum is f32: a block whose value scale is below 2^-126 of another's, with
@@ -365,8 +365,13 @@ __device__ __forceinline__ void score_step(const Queries<W, NT> &qs, uint32_t ti
 
 // The probabilities of a step's scores, as the second product's operand b, and their sum.  M need not be the maximum so
 // far: it stays until a score passes it by kSlack, so that most steps neither bring the maximum together across lanes nor
-// touch the output (16 rows found a new maximum in every other step: 61 us for 16 x 7 rows of up to 4099 keys, 58.5 so).  2^(x - M) then reaches 2^kSlack, well within f16.
-constexpr float kSlack = 8.0f;
+// touch the output (16 rows found a new maximum in every other step: 61 us for 16 x 7 rows of up to 4099 keys, 58.5 so).
+//
+// P = 2^(x - M + kLift) reaches 2^15 then, the last power of two within f16.  The factor of 2^kLift is in both sums and in
+// every partial result alike, so it cancels; without it a weight below 2^-14 of the largest lost digits in the first sum
+// and was gone below 2^-25 of it, but not in the second (8192 keys with 1.5 * 2^-24 each beside one whose value is zero:
+// the output was off by a third).  Now that begins at 2^-21 and 2^-32, at no cost that can be measured.
+constexpr float kSlack = 8.0f, kLift = 7.0f;
 
 template <int W, int NT, int N>
 __device__ __forceinline__ void soften(Running<W, NT> &run, const float (&x)[Step<W>::UNITS][NT][4], const float (&vs)[N],
@@ -405,7 +410,7 @@ __device__ __forceinline__ void soften(Running<W, NT> &run, const float (&x)[Ste
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) top[t][e] = run.m[t][e] == -INFINITY ? 0.0f : run.m[t][e];  // nothing seen yet: 2^(-inf - 0) = 0
+        for (int e = 0; e < 2; e++) top[t][e] = run.m[t][e] == -INFINITY ? 0.0f : run.m[t][e] - kLift;  // nothing seen yet: 2^(-inf - 0) = 0
     float inv[N];
 #pragma unroll
     for (int n = 0; n < N; n++) inv[n] = __fdividef(1.0f, fmaxf(vs[n], kScaleFloor));
