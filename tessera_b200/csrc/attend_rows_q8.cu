@@ -326,7 +326,7 @@ __device__ __forceinline__ void score_step(const Queries<W, NT> &qs, uint32_t ti
     const uint32_t r = lane >> 2;
     float lv[N];
 #pragma unroll
-    for (int n = 0; n < N; n++) lv[n] = log2_approx(fmaxf(vs[n], kScaleFloor));
+    for (int n = 0; n < N; n++) lv[n] = log2_approx(max_nan(vs[n], kScaleFloor));  // NaN stays NaN: it shows in rows that see the block
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int n = N == 1 ? 0 : u;
@@ -413,7 +413,7 @@ __device__ __forceinline__ void soften(Running<W, NT> &run, const float (&x)[Ste
         for (int e = 0; e < 2; e++) top[t][e] = run.m[t][e] == -INFINITY ? 0.0f : run.m[t][e] - kLift;  // nothing seen yet: 2^(-inf - 0) = 0
     float inv[N];
 #pragma unroll
-    for (int n = 0; n < N; n++) inv[n] = __fdividef(1.0f, fmaxf(vs[n], kScaleFloor));
+    for (int n = 0; n < N; n++) inv[n] = __fdividef(1.0f, fmaxf(vs[n], kScaleFloor));  // no NaN here: rows that see nothing of the block have P = 0
 #pragma unroll
     for (int u = 0; u < U; u++) {
 #pragma unroll

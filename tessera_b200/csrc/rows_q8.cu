@@ -180,11 +180,6 @@ __device__ __forceinline__ float min_nan(float a, float b) {  // NaN if either i
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
     return v;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float v;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
-    return v;
-}
 // What is kept of an infinity and of NaN.
 __device__ __forceinline__ float tame(float x) { return x != x ? 0.0f : fminf(fmaxf(x, -kLargest), kLargest); }
 

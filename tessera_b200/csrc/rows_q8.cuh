@@ -35,6 +35,12 @@ __device__ __forceinline__ uint32_t block_of(const RowsQ8Dev &p, uint32_t slot, 
     return at < p.blocks ? (uint32_t)at : kNoBlock;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float v;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
+    return v;
+}
+
 // Arrays of f32 or u32 that a kernel reads an element at a time (NULL is as aligned as any).
 inline bool aligned4(const void *a, const void *b = nullptr, const void *c = nullptr) {
     return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & 3u) == 0;

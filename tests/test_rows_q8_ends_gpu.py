@@ -44,3 +44,40 @@ def test_many_small_weights_beside_one_large_one_that_adds_nothing(width, heads,
         tol = 2.0 ** -8 * np.abs(want) + 2.0 ** -10 * a + keys * 2.0 ** -32 * largest * top
         off = np.abs(got[r::2] - want)
         assert np.all(off <= tol), (off / np.abs(want)).max()
+
+
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("case", [(16, 8, 128, 64, 64, "paged"), (8, 2, 128, 16, 32, "paged"), (6, 2, 64, 16, 64, "dense"), (4, 2, 256, 32, 64, "paged")],
+                         ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("rows", [6, 600])
+def test_a_scale_that_is_no_number_shows_in_every_row_that_sees_its_block_and_in_no_other(which, case, rows):
+    """One kv head of the block of positions 64 .. 64 + block has it.  Drafted rows (some see the block, some do not) and
+    rows of a window behind it; the few rows take the cluster's kernel, the many the other one."""
+    from tessera_b200 import ops
+    rng = np.random.default_rng(31)
+    heads, kv_heads, width, block = case[:4]
+    kv, kept, store = attend_case(rng, case, [300, 200])
+    pos = [61, 62, 63, 64, 65, 66] if rows == 6 else [61 + i % 120 for i in range(rows)]
+    pos[0] = 199
+    q = bf16(rng, len(pos), heads, width)
+    slots, at = dev_u32([0] * len(pos)), dev_u32(pos)
+    group = heads // kv_heads
+    blk, h = store.at(0, 64 // block), kv_heads - 1
+    for back in (FAR, 40):
+        clean = ops.attend_rows_q8(q, kv, slots, at, kept, 300, scale=width ** -0.5, back=back)
+        ids = dev_u32(np.broadcast_to(np.arange(6, dtype=np.uint32), (len(pos), kv_heads, 6)))
+        clean_listed = ops.attend_blocks_q8(q, kv, ids, slots, at, kept, 300, scale=width ** -0.5)
+        scales = getattr(kv, which)
+        was = scales[blk, h].clone()
+        scales[blk, h] = float("nan")
+        got = ops.attend_rows_q8(q, kv, slots, at, kept, 300, scale=width ** -0.5, back=back)
+        listed = ops.attend_blocks_q8(q, kv, ids, slots, at, kept, 300, scale=width ** -0.5)
+        scales[blk, h] = was
+        for out, want, low in ((got, clean, [max(0, p - back) for p in pos]), (listed, clean_listed, [0] * len(pos))):
+            sees = torch.tensor([p >= 64 and l < 64 + block for p, l in zip(pos, low)], device="cuda")
+            if out is listed:
+                sees &= 64 // block < 6
+            mine = out[:, h * group:(h + 1) * group]
+            assert torch.isnan(mine[sees].float()).all()
+            assert torch.equal(mine[~sees], want[~sees][:, h * group:(h + 1) * group])
+            assert torch.equal(out[:, :h * group], want[:, :h * group])
