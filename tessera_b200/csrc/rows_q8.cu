@@ -183,9 +183,16 @@ __device__ __forceinline__ float min_nan(float a, float b) {  // NaN if either i
 // What is kept of an infinity and of NaN.
 __device__ __forceinline__ float tame(float x) { return x != x ? 0.0f : fminf(fmaxf(x, -kLargest), kLargest); }
 
-// round(x * inv) for |x * inv| < 2^22 in the low bits: the sum's last place is one.
-constexpr float kCodeBits = 12582912.0f;  // 1.5 * 2^23
-__device__ __forceinline__ uint32_t code_bits(float x, float inv) { return __float_as_uint(fmaf(x, inv, kCodeBits)); }
+// round(x / s) for |x / s| < 2^22 in the low bits: the last place of a sum with 1.5 * 2^23 is one.  1 / s comes in two parts,
+// so that the quotient is rounded to f32 as a division's is.  With 1 / s alone its error decided where x / s is half-way
+// between two codes, which is common for values (they are bf16, and s is a bf16 over 127): one code in 1500 was the other one.
+constexpr float kCodeBits = 12582912.0f;
+struct Factor {
+    float high, low;
+};
+__device__ __forceinline__ uint32_t code_bits(float x, Factor f) {
+    return __float_as_uint(__fadd_rn(fmaf(x, f.high, __fmul_rn(x, f.low)), kCodeBits));
+}
 __device__ __forceinline__ uint32_t pack_bits(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
@@ -198,7 +205,8 @@ __device__ __forceinline__ float code_at(uint32_t w, int i) {
 
 // A block's scale before and after, and how its codes follow.
 struct Scales {
-    float inv, ratio, now;
+    Factor inv, ratio;
+    float now;
     bool fresh;
 };
 
@@ -206,25 +214,31 @@ __device__ __forceinline__ Scales grow(float was, bool fresh, float most) {
     const float old = fresh ? 0.0f : was;
     Scales s;
     s.now = fmaxf(old, fmaxf(most / 127.0f, kScaleFloor));
-    s.inv = 1.0f / s.now;
-    s.ratio = fresh ? 1.0f : old / s.now;  // within [0, 1] for every scale that append writes
+    s.inv.high = 1.0f / s.now;
+    s.inv.low = fmaf(-s.inv.high, s.now, 1.0f) * s.inv.high;
+    s.ratio = {1.0f, 0.0f};
+    if (!fresh) {
+        s.ratio.high = old / s.now;  // within [0, 1] for every scale that append writes
+        s.ratio.low = fmaf(-s.ratio.high, s.now, old) * s.inv.high;
+    }
     s.fresh = fresh;
     return s;
 }
 
 // |x| <= most, so that no code passes 127.
 template <int W>
-__device__ __forceinline__ void write_row(int8_t *row, uint32_t i, const float2 (&x)[4], float inv) {
+__device__ __forceinline__ void write_row(int8_t *row, uint32_t i, const float2 (&x)[4], Factor f) {
+    auto codes = [&](float2 v) { return __fadd2_rn(fma2(v, both(f.high), mul2(v, both(f.low))), both(kCodeBits)); };
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const float2 a = fma2(x[2 * h], both(inv), both(kCodeBits)), b = fma2(x[2 * h + 1], both(inv), both(kCodeBits));
+        const float2 a = codes(x[2 * h]), b = codes(x[2 * h + 1]);
         *reinterpret_cast<uint32_t *>(row + h * (W / 2) + 4 * i) =
             pack_bits(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
     }
 }
 
 // A held row's codes follow the scale (a code of -128, which append never writes, becomes -127 at most).
-__device__ __forceinline__ uint32_t follow(uint32_t w, float ratio) {
+__device__ __forceinline__ uint32_t follow(uint32_t w, Factor ratio) {
     uint32_t c[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) c[e] = code_bits(fmaxf(code_at(w, e), -127.0f), ratio);
@@ -232,7 +246,7 @@ __device__ __forceinline__ uint32_t follow(uint32_t w, float ratio) {
 }
 
 template <int W>
-__device__ __forceinline__ void follow_row(int8_t *row, uint32_t i, float ratio) {
+__device__ __forceinline__ void follow_row(int8_t *row, uint32_t i, Factor ratio) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         uint32_t *at = reinterpret_cast<uint32_t *>(row + h * (W / 2) + 4 * i);
@@ -490,7 +504,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
 #pragma unroll
             for (int k = 0; k < PASSES; k++)
                 if (row[k]) write_row<W>(row[k], li, x[k], sc.inv);
-            if (sc.ratio < 1.0f)
+            if (sc.ratio.high < 1.0f)
                 for (uint32_t i = which; i < (uint32_t)B; i += T)
                     if (!(written >> i & 1)) follow_row<W>(codes + i * W, li, sc.ratio);
             if (bounded) {
@@ -579,7 +593,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
                         for (int e = 0; e < 4; e++) x[e] = make_float2(tame(x[e].x), tame(x[e].y));
                     }
                     write_row<W>(codes + i * W, li, x, sc.inv);
-                } else if (i < B && sc.ratio < 1.0f) {
+                } else if (i < B && sc.ratio.high < 1.0f) {
                     follow_row<W>(codes + i * W, li, sc.ratio);
                 }
             }
@@ -672,7 +686,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
                 const float4 v = kept[(2 * u) * (TEAM * 32) + tid], w = kept[(2 * u + 1) * (TEAM * 32) + tid];
                 const float2 x[4] = {make_float2(v.x, v.y), make_float2(v.z, v.w), make_float2(w.x, w.y), make_float2(w.z, w.w)};
                 write_row<W>(codes + i * W, li, x, sc.inv);
-            } else if (i < B && sc.ratio < 1.0f) {
+            } else if (i < B && sc.ratio.high < 1.0f) {
                 follow_row<W>(codes + i * W, li, sc.ratio);
             }
         }

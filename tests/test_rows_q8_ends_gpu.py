@@ -81,3 +81,54 @@ def test_a_scale_that_is_no_number_shows_in_every_row_that_sees_its_block_and_in
             assert torch.isnan(mine[sees].float()).all()
             assert torch.equal(mine[~sees], want[~sees][:, h * group:(h + 1) * group])
             assert torch.equal(out[:, :h * group], want[:, :h * group])
+
+
+@pytest.mark.parametrize("width,block", [(64, 16), (128, 64), (128, 16), (256, 32)])
+@pytest.mark.parametrize("length", [1, 3, 64])
+def test_values_half_way_between_two_codes_take_the_even_one(width, block, length):
+    """Values are bf16 and kept as they come, so that x / scale is often exactly half-way.  The codes equal round(x / scale)
+    with the quotient rounded to f32 and no step more; codes that follow a grown scale equal round(code * old / new) so.
+    The scales are maxima / 127 in f32.  Keys at position 0 with no norm are turned by nothing: the same."""
+    from tessera_b200 import ops
+    rng = np.random.default_rng(32)
+    heads, kv_heads, slots, page = 1, 4, 60, 64
+    kv = make(rng, kv_heads, width, block, 2 * slots, page)
+    kept = ops.Kept("dense", 2 * page, None, 2 * slots * page)
+    old = {n: getattr(kv, n).cpu().numpy() for n in ("v", "v_scale")}
+    begin = [0 if s % 2 else 3 for s in range(slots)]  # fresh blocks, and blocks that hold other rows
+    row_slots = [s for s in range(slots) for _ in range(length)]
+    row_pos = [begin[s] + i for s in range(slots) for i in range(length)]
+    # a largest value per slot, some below what is held, some above
+    size = np.exp2(rng.integers(-4, 4, (slots, 1))).repeat(length, 0)[..., None]
+    qkv = torch.from_numpy((rng.standard_normal((slots * length, heads + 2 * kv_heads, width)) * size).astype(np.float32)).cuda().bfloat16()
+    ops.qk_norm_rope_append_q8(qkv.reshape(len(row_pos), -1), None, None, inv_freq(width), dev_u32(row_slots), dev_u32(row_pos), kv, kept,
+                               heads, eps=1e-6)
+    x = qkv.float().cpu().numpy()[:, heads + kv_heads:].reshape(slots, length, kv_heads, width)
+    v, scale = kv.v.cpu().numpy(), kv.v_scale.cpu().numpy()
+    per = 2 * page // block
+    follows = 0
+    for s in range(slots):
+        for b in range((begin[s] + length - 1) // block + 1):
+            blk, rows = s * per + b, [i for i in range(length) if (begin[s] + i) // block == b]
+            at = [(begin[s] + i) % block for i in rows]
+            most = np.abs(x[s, rows]).max((0, 2))
+            was = np.zeros(kv_heads, np.float32) if 0 in at else old["v_scale"][blk]
+            now = np.maximum(was, most / np.float32(127))
+            assert np.array_equal(scale[blk], now)
+            want = np.rint(x[s, rows] / now[:, None])  # f32
+            assert np.array_equal(v[blk][:, at].transpose(1, 0, 2), want)
+            held = [i for i in range(block) if i not in at]
+            if 0 not in at:
+                moved = (old["v"][blk][:, held].astype(np.float64) * was.astype(np.float64)[:, None, None] / now.astype(np.float64)[:, None, None])
+                assert np.array_equal(v[blk][:, held], np.rint(moved.astype(np.float32)))
+                follows += (now > was).sum()
+    assert follows > 0 or length == 64 and block < 64
+    fresh = [s for s in range(slots) if begin[s] == 0]
+    k, k_scale = kv.k.cpu().numpy(), kv.k_scale.cpu().numpy()
+    first = qkv.float().cpu().numpy()[[s * length for s in fresh], heads:heads + kv_heads]
+    for i, s in enumerate(fresh):
+        assert np.array_equal(k[s * per, :, 0], np.rint(first[i] / k_scale[s * per][:, None]))
+    blocks = np.array([s * per for s in fresh])
+    for j, pick in ((0, "min"), (1, "max")):  # and the bounds are those of the codes
+        n = min(length, block)
+        assert np.array_equal(kv.k_bounds.cpu().numpy()[blocks, :, j], getattr(k[blocks][:, :, :n], pick)(2))
