@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 from dataclasses import dataclass
+from threading import get_ident
 
 import torch
 
@@ -41,12 +42,14 @@ def _dtype_code(dtype: torch.dtype) -> int:
 
 
 def workspace(nbytes: int, device) -> torch.Tensor | None:
-    """A caller-owned scratch buffer, grown on demand and reused: one per device and stream, so that launches on
-    two streams that may run side by side never share scratch."""
+    """A caller-owned scratch buffer, grown on demand and reused: one per host thread, device and stream, so that
+    launches on two streams that may run side by side never share scratch, nor calls of two threads: the library runs
+    without the interpreter's lock and may queue several kernels that meet in the scratch, and another thread's could
+    come to stand between them.  (Buffers stay when a thread ends: a captured graph may use them.)"""
     if nbytes == 0:
         return None
     dev = torch.device(device)
-    key = (dev.index or 0, torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else 0)
+    key = (dev.index or 0, torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else 0, get_ident())
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
@@ -276,17 +279,18 @@ _q8_scratch: dict = {}
 
 
 def _scratch(nbytes: int, dev: int, stream: int, like):
-    """(address, owner) of scratch for one call: one buffer a device and stream, which its calls use one after another.
-    A call that is being captured gets its own, in the graph's pool: graphs replay on any stream, and two of them at
-    once must not share it."""
+    """(address, owner) of scratch for one call: one buffer a host thread, device and stream (see `workspace`), which its
+    calls use one after another.  A call that is being captured gets its own, in the graph's pool: graphs replay on any
+    stream, and two of them at once must not share it."""
     if nbytes == 0:
         return None, None
     if torch._C._cuda_isCurrentStreamCapturing():
         buf = like.new_empty(nbytes, dtype=torch.uint8)
         return buf.data_ptr(), buf
-    buf = _q8_scratch.get((dev, stream))
+    key = (dev, stream, get_ident())
+    buf = _q8_scratch.get(key)
     if buf is None or buf.numel() < nbytes:
-        buf = _q8_scratch[dev, stream] = like.new_empty(max(nbytes, 1 << 20), dtype=torch.uint8)
+        buf = _q8_scratch[key] = like.new_empty(max(nbytes, 1 << 20), dtype=torch.uint8)
     return buf.data_ptr(), buf
 
 

@@ -1,0 +1,50 @@
+"""Scratch of the Python face: what a call is given while another one's kernels may still be queued."""
+import threading
+
+import pytest
+import torch
+
+
+def in_threads(n, work):
+    """work() on n threads that are all alive at once; their results."""
+    got, meet = [None] * n, threading.Barrier(n, timeout=60)
+
+    def one(i):
+        meet.wait()
+        got[i] = work()
+        meet.wait()
+
+    threads = [threading.Thread(target=one, args=(i,)) for i in range(n)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    return got
+
+
+@pytest.fixture
+def ops(monkeypatch):
+    from tessera_b200 import ops
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False)
+    monkeypatch.setattr(ops, "_workspaces", {})
+    monkeypatch.setattr(ops, "_q8_scratch", {})
+    return ops
+
+
+def test_threads_on_one_stream_have_scratch_of_their_own(ops):
+    """A call's kernels meet in its scratch, and the library is called without the interpreter's lock: with one buffer for
+    two threads, one's second kernel can read what the other's first one left."""
+    like = torch.zeros(1)
+    for work in (lambda: ops._scratch(100, 0, 7, like)[0], lambda: ops.workspace(100, "cpu").data_ptr()):
+        got = in_threads(4, work)
+        assert len(set(got)) == 4
+
+
+def test_a_thread_keeps_its_scratch_and_streams_do_not_share(ops):
+    like = torch.zeros(1)
+    first, owner = ops._scratch(100, 0, 7, like)
+    assert ops._scratch(200, 0, 7, like)[0] == first
+    assert ops._scratch(100, 0, 8, like)[0] != first and ops._scratch(100, 1, 7, like)[0] != first
+    grown, larger = ops._scratch(owner.numel() + 1, 0, 7, like)
+    assert larger.numel() > owner.numel() and ops._scratch(100, 0, 7, like)[0] == grown
+    assert ops._scratch(0, 0, 7, like) == (None, None)

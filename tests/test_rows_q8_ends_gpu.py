@@ -132,3 +132,35 @@ def test_values_half_way_between_two_codes_take_the_even_one(width, block, lengt
     for j, pick in ((0, "min"), (1, "max")):  # and the bounds are those of the codes
         n = min(length, block)
         assert np.array_equal(kv.k_bounds.cpu().numpy()[blocks, :, j], getattr(k[blocks][:, :, :n], pick)(2))
+
+
+def test_host_threads_on_one_stream_get_their_own_results():
+    """Both calls leave partial results in scratch for a second kernel, and the library runs without the interpreter's lock."""
+    import threading
+    from tessera_b200 import ops
+    rng = np.random.default_rng(33)
+    case = (16, 8, 128, 16, 64, "paged")
+    jobs = []
+    for lengths in ([9000, 40, 8500], [8800, 8800, 9]):
+        kv, kept, _ = attend_case(rng, case, lengths)
+        q, slots, pos = bf16(rng, 3, 16, 128), dev_u32([0, 1, 2]), dev_u32([n - 1 for n in lengths])
+        jobs.append(lambda q=q, kv=kv, slots=slots, pos=pos, kept=kept: (
+            ops.attend_rows_q8(q, kv, slots, pos, kept, 9000, scale=0.09), ops.select_blocks_q8(q, kv, slots, pos, kept, 9000, 20)))
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    stream, bad, meet = torch.cuda.Stream(), [], threading.Barrier(2, timeout=60)
+
+    def work(i):
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                meet.wait()
+                got = [jobs[i]() for _ in range(20)]
+                if not all(torch.equal(a, b) for g in got for a, b in zip(g, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
