@@ -271,7 +271,8 @@ def _kept_q8(kept: Kept, dev) -> TsKept:
 
 
 @functools.lru_cache(maxsize=256)
-def _q8_workspace(which: str, *sizes) -> int:
+def _q8_workspace(which: str, dev: int, *sizes) -> int:
+    """The library's answer for these sizes on device `dev`, the current one: it goes by that device's multiprocessors."""
     return getattr(lib, which)(*sizes)
 
 
@@ -348,7 +349,7 @@ def attend_rows_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, *, sc
     else:
         a_out = _at(out, _BF16, rows * heads * width, dev, "out")
     a_slots, a_pos = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
-    nbytes = _q8_workspace("ts_attend_rows_q8_workspace_bytes", rows, keys, heads, kv_heads, width, back)
+    nbytes = _q8_workspace("ts_attend_rows_q8_workspace_bytes", dev, rows, keys, heads, kv_heads, width, back)
     ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:
         check(lib.ts_attend_rows_q8(a_q, record, a_out, a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads, width, back,
@@ -365,7 +366,7 @@ def select_blocks_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, cou
     a_q = _at(q, _BF16, rows * heads * width, dev, "q")
     a_slots, a_pos = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
     ids = q.new_empty((rows, kv_heads, max(count, 0)), dtype=torch.int32)
-    nbytes = _q8_workspace("ts_select_blocks_q8_workspace_bytes", rows, keys, kv_heads, block, max(count, 0))
+    nbytes = _q8_workspace("ts_select_blocks_q8_workspace_bytes", dev, rows, keys, kv_heads, block, max(count, 0))
     ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:
         check(lib.ts_select_blocks_q8(a_q, record, ids.data_ptr(), a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads,
@@ -387,7 +388,7 @@ def attend_blocks_q8(q, kv: RowsQ8, ids, slots, positions, kept: Kept, keys: int
         a_out = _at(out, _BF16, rows * heads * width, dev, "out")
     a_ids = _at(ids, _I32, rows * kv_heads * count, dev, "ids")
     a_slots, a_pos = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
-    nbytes = _q8_workspace("ts_attend_blocks_q8_workspace_bytes", rows, count, heads, kv_heads, width, block)
+    nbytes = _q8_workspace("ts_attend_blocks_q8_workspace_bytes", dev, rows, count, heads, kv_heads, width, block)
     ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:
         check(lib.ts_attend_blocks_q8(a_q, record, a_ids, a_out, a_slots, a_pos, _kept_q8(kept, dev), rows, keys, heads, kv_heads,

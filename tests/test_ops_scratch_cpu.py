@@ -48,3 +48,20 @@ def test_a_thread_keeps_its_scratch_and_streams_do_not_share(ops):
     grown, larger = ops._scratch(owner.numel() + 1, 0, 7, like)
     assert larger.numel() > owner.numel() and ops._scratch(100, 0, 7, like)[0] == grown
     assert ops._scratch(0, 0, 7, like) == (None, None)
+
+
+def test_workspace_sizes_are_kept_by_device(ops, monkeypatch):
+    """A size goes by the current device's multiprocessors."""
+    class Library:
+        count = 0
+
+        def ts_size(self, rows, keys):
+            self.count += 1
+            return self.count
+
+    monkeypatch.setattr(ops, "lib", Library())
+    ops._q8_workspace.cache_clear()
+    try:
+        assert [ops._q8_workspace("ts_size", dev, 5, 6) for dev in (0, 1, 0, 1)] == [1, 2, 1, 2]
+    finally:
+        ops._q8_workspace.cache_clear()
