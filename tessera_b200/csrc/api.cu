@@ -318,7 +318,7 @@ int ts_attend_blocks_q8(const void *q, const ts_rows_q8 *kv, const uint32_t *ids
     RowsQ8Dev dev;
     bool done = false;
     TS_REQUIRE(aligned4(ids), "attend_blocks (q8): ids must be 4-byte aligned");
-    TS_REQUIRE(ids != nullptr && count > 0 && count <= (1u << 24), "attend_blocks (q8): ids is NULL or %u blocks are not 1 to 2^24", count);
+    TS_REQUIRE(ids != nullptr && count > 0 && count <= kMostListed, "attend_blocks (q8): ids is NULL or %u blocks are not 1 to 2^24", count);
     const int rc = check_attend_q8("attend_blocks (q8)", q, kv, out, slots, positions, kept, rows, keys, heads, kv_heads, width,
                                    &dev, &done, stream);
     if (rc != TS_OK || done) return rc;

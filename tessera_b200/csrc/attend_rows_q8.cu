@@ -1142,6 +1142,8 @@ size_t attend_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t heads, u
                                  uint32_t count, uint32_t block) {
     if (rows == 0 || keys == 0 || heads == 0 || kv_heads == 0 || heads % kv_heads) return 0;
     if (width != 64 && width != 128 && width != 256) return 0;
+    // sizes that the calls refuse (a count of blocks and keys past 32 bits would overflow the plan's steps)
+    if ((block != 16 && block != 32 && block != 64) || count > kMostListed || kv_heads > 65535) return 0;
     return plan_of(rows, keys, heads, kv_heads, width, back, count, block).bytes();
 }
 

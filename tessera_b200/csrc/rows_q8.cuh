@@ -7,6 +7,7 @@
 namespace ts {
 
 constexpr uint32_t kNoBlock = 0xFFFFFFFFu;
+constexpr uint32_t kMostListed = 1u << 24;  // blocks that a row and kv head may list
 
 struct RowsQ8Dev {
     int8_t *k, *v;
