@@ -1056,7 +1056,9 @@ Plan plan_of(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, ui
     // A tile of up to four steps is not worth cutting: a worker does it in less time than a second kernel takes.
     s.merged = steps > 4;
     s.whole = steps <= 1 ? 1 : (uint32_t)(steps < 4 ? steps : 4);
-    const uint64_t jobs = s.merged ? s.together * each : s.together * (each / steps);
+    // (Where not even one tile's steps fit, the call reads less, its slots' room, or is refused: workspace as for one tile.)
+    const uint64_t planned = s.together ? s.together : min(rows, s.tokens);
+    const uint64_t jobs = s.merged ? planned * each : planned * (each / steps);
     s.workers = (uint32_t)(jobs < most ? jobs : most);
     // A cluster for each row and kv head, as small as leaves a warp two steps, or four: where all of them are resident at once.
     s.cluster = 0;

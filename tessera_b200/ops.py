@@ -328,6 +328,11 @@ def rows_unpack_q8(kv: RowsQ8, slots, positions, kept: Kept):
     return k_out, v_out
 
 
+def _room(kept: Kept, keys: int) -> int:
+    """`keys`, or what a slot's stride or pages hold: more are never read, nor is workspace for them needed."""
+    return min(keys, kept.scalar * (1 if kept.layout == "dense" else kept.page or KEPT_PAGE[kept.layout]))
+
+
 def _heads_of(q, kv_heads: int, width: int, keys: int) -> tuple:
     if not 0 <= keys <= FAR:
         _refuse(f"{keys} keys")
@@ -349,6 +354,7 @@ def attend_rows_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, *, sc
     else:
         a_out = _at(out, _BF16, rows * heads * width, dev, "out")
     a_slots, a_pos = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
+    keys = _room(kept, keys)
     nbytes = _q8_workspace("ts_attend_rows_q8_workspace_bytes", dev, rows, keys, heads, kv_heads, width, back)
     ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:
@@ -366,6 +372,7 @@ def select_blocks_q8(q, kv: RowsQ8, slots, positions, kept: Kept, keys: int, cou
     a_q = _at(q, _BF16, rows * heads * width, dev, "q")
     a_slots, a_pos = _at(slots, _I32, rows, dev, "slots"), _at(positions, _I32, rows, dev, "positions")
     ids = q.new_empty((rows, kv_heads, max(count, 0)), dtype=torch.int32)
+    keys = _room(kept, keys)
     nbytes = _q8_workspace("ts_select_blocks_q8_workspace_bytes", dev, rows, keys, kv_heads, block, max(count, 0))
     ws, _owner = _scratch(nbytes, dev, stream, q)
     if rows:

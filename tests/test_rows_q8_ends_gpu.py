@@ -164,3 +164,25 @@ def test_host_threads_on_one_stream_get_their_own_results():
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("case", [(16, 8, 128, 64, 64, "paged"), (4, 4, 64, 16, 32, "dense"), (20, 1, 256, 32, 64, "paged")], ids=lambda c: "-".join(map(str, c)))
+def test_keys_without_a_limit_are_the_room_of_a_slot(case):
+    from tessera_b200 import _lib, ops
+    import ctypes as C
+    rng = np.random.default_rng(34)
+    kv, kept, _ = attend_case(rng, case, [20000, 700])
+    heads, kv_heads, width, block = case[:4]
+    q, slots, pos = bf16(rng, 4, heads, width), dev_u32([0, 1, 1, 0]), dev_u32([19999, 5, 6, FAR])
+    room = kept.scalar * (case[4] if case[5] == "paged" else 1)
+    want = ops.attend_rows_q8(q, kv, slots, pos, kept, room, scale=0.09), ops.select_blocks_q8(q, kv, slots, pos, kept, room, 9)
+    for keys in (room + 1, 1 << 28, FAR):
+        assert torch.equal(ops.attend_rows_q8(q, kv, slots, pos, kept, keys, scale=0.09), want[0])
+        assert torch.equal(ops.select_blocks_q8(q, kv, slots, pos, kept, keys, 9), want[1])
+        # and through the library's own face, with the workspace that it asks for
+        nbytes = _lib.lib.ts_attend_rows_q8_workspace_bytes(4, keys, heads, kv_heads, width, FAR)
+        ws, out = torch.empty(nbytes, dtype=torch.uint8, device="cuda"), torch.empty_like(q)
+        p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+        _lib.check(_lib.lib.ts_attend_rows_q8(p(q), kv._held[0], p(out), p(slots), p(pos), kept.c(), 4, keys, heads, kv_heads, width, FAR,
+                                              0.09, p(ws), nbytes, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(out, want[0])
