@@ -395,9 +395,10 @@ typedef struct {
  * follow: those of the new key codes alone in a fresh block, else joined with round(bound * s_old / s_new).
  * NaN stores the code 0, an infinity the largest code, and counts as the largest finite bf16 in `a`, so that
  * what is kept reads back finite.
- * Rows of one call that fall into the same block must stand next to one another, in any order; of rows with the
- * same slot and position the last one counts (a launch that repeats its last row to fill up is fine).  q_out must not
- * overlap qkv. */
+ * In a call of up to 1024 rows, the rows that fall into the same block may stand anywhere; in a larger one they must
+ * stand next to one another, in any order (nothing looks for the others: what the block holds afterwards, its scale and
+ * bounds would be undefined).  Of rows with the same slot and position the last one counts (a launch that repeats its
+ * last row to fill up is fine).  q_out must not overlap qkv. */
 int ts_qk_norm_rope_append_q8(const void *qkv, const float *q_norm, const float *k_norm, const float *inv_freq,
                               const uint32_t *slots, const uint32_t *positions, void *q_out, const ts_rows_q8 *kv,
                               const ts_kept *kept, uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t width,

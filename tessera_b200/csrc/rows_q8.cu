@@ -1,16 +1,17 @@
 // Kept rows in 8 bits: append (norm, rotation, block scales, key bounds) and reading rows back.
 //
 // Append.  A block of B positions has one scale per kv head, so the rows of a call that fall into one block are one
-// unit of work: run = the neighbouring rows of a (slot, block).  A long run (a prompt's) belongs to a team of
-// warps for each kv head's keys and values: they take the block's positions in turn, keep the prepared values in shared
-// memory and agree there on the largest magnitude.  A short run (a step's row) belongs to one warp, which keeps them in
-// registers.  Either way every value is read once and rounded once.  Held codes are read and rewritten only when the scale
-// grows (a new largest value: for values without a trend once in i rows at the block's i-th row).  Query heads go to warps
-// of their own, eight heads of a row each when there are many.
+// unit of work: run = the neighbouring rows of a (slot, block), in a call of few rows all of them wherever they stand.  A
+// long run (a prompt's) belongs to a team of warps for each kv head's keys and values: they take the block's positions in
+// turn, keep the prepared values in shared memory and agree there on the largest magnitude.  A short run (a step's row)
+// belongs to one warp, which keeps them in registers.  Either way every value is read once and rounded once.  Held codes are
+// read and rewritten only when the scale grows (a new largest value: for values without a trend once in i rows at the
+// block's i-th row).  Query heads go to warps of their own, eight heads of a row each when there are many.
 //
 // W / 8 lanes hold a head: lane i of them the four pairs 4 i .. 4 i + 3, elements 4 i + e and W / 2 + 4 i + e, so that
 // loads are 8 bytes and stores of codes 4 a lane.
 #include <cmath>
+#include <type_traits>
 
 #include "rows_q8.cuh"
 
@@ -279,12 +280,17 @@ __device__ __forceinline__ void write_bounds(int8_t *bounds, uint32_t first, uin
 
 constexpr uint32_t kShort = 4;  // rows of a run that one warp takes
 constexpr int kAppendWarps = 4, kAppendThreads = kAppendWarps * 32;
+// Rows of a call up to which a block's rows may stand anywhere in it (drafted tokens laid out draft by draft): thread
+// blocks then look after kAppendWarps rows and compare every row of the call with them, which at 1024 rows is 33 MB from
+// L2 in all, and grows with the rows' square: 64 single rows take 13.2 us for 12.6 without, 512 take 44.0 for 40.7.  A
+// kernel of its own (GATHERS): 8165 rows took 42.7 us for 40.7 when one kernel did both.
+constexpr uint32_t kGathered = 1024;
 
 // Measured: 64 single rows with 16 + 8 + 8 heads of 128 take 6.1 us, most of it one load after another (slot, page, scale,
 // row, the block when the scale grows); 8165 rows of three prompts 40 us for 119 MB, 0.45 of the copy rate: the angles,
 // norms and roundings of 260,000 heads keep the schedulers busier than the memory.  Two values an instruction brought it
 // there from 43, five thread blocks an SM (92 registers, little spilled) from 41 with six (80 registers).
-template <int W, int B>
+template <int W, int B, bool GATHERS>
 __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_kernel(const AppendParams p) {
     constexpr int L = Lanes<W>::PER_HEAD, T = Lanes<W>::TOGETHER;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, li = lane % L, which = lane / L;
@@ -301,7 +307,11 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
     const uint32_t units = 2 * p.kv_heads, unit = kv_block % units;
     const uint32_t r0 = kv_block / units * p.window, r1 = min(p.rows, r0 + p.window);
     uint32_t slot = 0, blk_pos = 0xFFFFFFFFu, starts = 0;
+    __shared__ uint32_t sm_rows[kAppendWarps], sm_last[kAppendWarps], sm_earlier;  // by run: see below
+    bool odd = false;  // a row of some run's slot stands outside the thread block's rows, or in another run among them
     if (!queries) {
+        uint32_t any_slot = 0;
+        if (GATHERS && threadIdx.x < p.rows) any_slot = p.slots[threadIdx.x];
         if (r0 + lane < r1) {
             slot = p.slots[r0 + lane];
             blk_pos = p.positions[r0 + lane] >> p.kv.shift;
@@ -316,6 +326,26 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
         if (starts == 0) {
             pdl_launch_dependents();
             return;
+        }
+        if constexpr (GATHERS) {
+            // only the slots are compared here: a thread block one of whose slots comes up elsewhere looks closely below
+            uint32_t s[kAppendWarps];
+#pragma unroll
+            for (int w = 0; w < kAppendWarps; w++) s[w] = __shfl_sync(0xFFFFFFFFu, slot, min((uint32_t)w, r1 - r0 - 1));
+#pragma unroll
+            for (int o = 1; o < kAppendWarps; o++) {
+                const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, slot, o);
+                odd = odd || (begins && lane >= (uint32_t)o && (starts >> (lane - o) & 1) && slot == before);
+            }
+            for (uint32_t i = threadIdx.x; i < p.rows; i += kAppendThreads) {
+                if (i >= (uint32_t)kAppendThreads) any_slot = p.slots[i];
+                bool same = any_slot == s[0];
+#pragma unroll
+                for (int w = 1; w < kAppendWarps; w++) same = same || any_slot == s[w];
+                odd = odd || (same && i - r0 >= (uint32_t)kAppendWarps);
+            }
+            if (threadIdx.x < kAppendWarps) sm_rows[threadIdx.x] = sm_last[threadIdx.x] = 0;
+            if (threadIdx.x == 0) sm_earlier = 0;
         }
     }
     if (threadIdx.x < W / 2) sm_turns[threadIdx.x] = turns_of(freq);
@@ -431,10 +461,33 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
         sine_cosine(STEP, sm_turns[2 * threadIdx.x], sm_turns[2 * threadIdx.x + 1], &sn, &cs);
         sm_step[threadIdx.x] = make_float4(sn.x, sn.y, cs.x, cs.y);
     }
-    __syncthreads();
+    bool gather = false;
+    if constexpr (GATHERS) {
+        gather = __syncthreads_or(odd);
+        if (gather) {
+            // Of each run's block: whether rows before the run fall into it (then it is not this run's), how many do from the
+            // run's start on, and the last of them.
+            for (uint32_t i = threadIdx.x; i < p.rows; i += kAppendThreads)
+#pragma unroll
+                for (int w = 0; w < kAppendWarps; w++) {
+                    const uint32_t at = r0 + w;
+                    if (!(starts >> w & 1) || p.slots[i] != p.slots[at] || (p.positions[i] ^ p.positions[at]) >> p.kv.shift) continue;
+                    if (i < at) {
+                        atomicOr(&sm_earlier, 1u << w);
+                    } else {
+                        atomicAdd(&sm_rows[w], 1u);
+                        atomicMax(&sm_last[w], i);
+                    }
+                }
+            __syncthreads();
+        }
+    } else {
+        __syncthreads();
+    }
     for (uint32_t turn = 0; starts; turn++) {
         const uint32_t first = __ffs(starts) - 1;
         starts &= starts - 1;
+        if (gather && (sm_earlier >> first & 1)) continue;  // belongs to the block's first row
         const uint32_t s = r0 + first, run_slot = __shfl_sync(0xFFFFFFFFu, slot, first), b = __shfl_sync(0xFFFFFFFFu, blk_pos, first);
         const uint32_t blk = block_of(p.kv, run_slot, b);
         auto same = [&](uint32_t i) { return i < p.rows && p.slots[i] == run_slot && (p.positions[i] >> p.kv.shift) == b; };
@@ -444,12 +497,13 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
             const uint32_t out = ~__ballot_sync(0xFFFFFFFFu, lane < n || (lane <= kShort && same(s + lane)));
             n = __ffs(out) - 1;
         }
+        const bool apart = gather && sm_last[first] - s + 1 != sm_rows[first];  // other rows stand between the block's
         const size_t at = (size_t)(blk == kNoBlock ? 0 : blk) * p.kv_heads + h;
         float *scale = (is_v ? p.kv.v_scale : p.kv.k_scale) + at;
         int8_t *codes = (is_v ? p.kv.v : p.kv.k) + at * B * W;
         int8_t *bounds = p.kv.bounds + at * 2 * W;
         const float was = *scale;  // asked for before it is needed
-        if (n <= kShort) {
+        if (n <= kShort && !apart) {
             // ---- a warp's run ----
             if (turn % kAppendWarps != warp || blk == kNoBlock) continue;
             constexpr int PASSES = kShort / T > 0 ? kShort / T : 1;
@@ -533,7 +587,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
         for (uint32_t base = s; base < p.rows; base += TEAM * 32) {
             const uint32_t i = base + tid;
             const bool in = same(i);
-            if (!in && i < p.rows) atomicMin(&stop, i);
+            if (!in && i < p.rows && !apart) atomicMin(&stop, i);
             team_sync();
             const uint32_t end = stop;  // later passes only bring it down to rows past this one's
             if (in && i < end) atomicMax(&src[p.positions[i] & (B - 1)], (int)i);
@@ -787,23 +841,27 @@ constexpr size_t append_smem() {
     return (size_t)(kAppendWarps / team) * passes * 2 * team * 32 * sizeof(float4);
 }
 
-template <int W, int B>
+template <int W, int B, bool GATHERS>
 cudaError_t launch_append(const AppendParams &p, uint32_t grid, cudaStream_t stream) {
     constexpr size_t smem = append_smem<W, B>();
     static OncePerDevice configured;
     if (smem > 48 * 1024 && configured.needs()) {
-        const cudaError_t e = cudaFuncSetAttribute(append_q8_kernel<W, B>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = cudaFuncSetAttribute(append_q8_kernel<W, B, GATHERS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
         configured.done();
     }
-    return launch(append_q8_kernel<W, B>, dim3(grid), dim3(kAppendThreads), smem, stream, pdl_enabled(), p);
+    return launch(append_q8_kernel<W, B, GATHERS>, dim3(grid), dim3(kAppendThreads), smem, stream, pdl_enabled(), p);
 }
 
 template <int W>
 cudaError_t launch_append(const AppendParams &p, uint32_t grid, cudaStream_t stream) {
-    return p.kv.shift == 4   ? launch_append<W, 16>(p, grid, stream)
-           : p.kv.shift == 5 ? launch_append<W, 32>(p, grid, stream)
-                             : launch_append<W, 64>(p, grid, stream);
+    auto go = [&](auto gathers) {
+        constexpr bool GATHERS = decltype(gathers)::value;
+        return p.kv.shift == 4   ? launch_append<W, 16, GATHERS>(p, grid, stream)
+               : p.kv.shift == 5 ? launch_append<W, 32, GATHERS>(p, grid, stream)
+                                 : launch_append<W, 64, GATHERS>(p, grid, stream);
+    };
+    return p.rows <= kGathered ? go(std::true_type{}) : go(std::false_type{});
 }
 
 }  // namespace
@@ -826,7 +884,7 @@ int append_q8(const void *qkv, const float *q_norm, const float *k_norm, const f
     p.eps = eps;
     // A step's rows each have a run of their own: four of them keep the warps of a thread block busy.  A prompt's
     // rows come in runs of up to a block: looking at 32 rows leaves few thread blocks without a run to start.
-    p.window = rows <= 1024 ? kAppendWarps : 32;
+    p.window = rows <= kGathered ? kAppendWarps : 32;
     // Eight heads a warp compute a row's angles once and have their loads under way together, four rows share what a warp
     // sets up; a step's few heads go to as many warps as there are.
     const bool many = (uint64_t)rows * heads > 32768;

@@ -298,7 +298,8 @@ def _scratch(nbytes: int, dev: int, stream: int, like):
 def qk_norm_rope_append_q8(qkv, q_norm, k_norm, inv_freq, slots, positions, kv: RowsQ8, kept: Kept, heads: int, *, eps: float,
                            out=None):
     """Per-head norm (gains f32 [width] or None) and rotation, q out in bf16 [rows, heads, width], k and v into their
-    blocks: ts_qk_norm_rope_append_q8.  Rows that fall into the same block stand next to one another."""
+    blocks: ts_qk_norm_rope_append_q8.  With more than 1024 rows, those that fall into the same block must stand next to
+    one another."""
     record, dev, kv_heads, _, width = kv._held
     stream = _q8_stream(dev)
     rows = slots.numel()

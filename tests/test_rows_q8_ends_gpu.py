@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import q8_model as M
-from tests.test_rows_q8_gpu import attend_case, bf16, inv_freq, make, np64, paged
+from tests.test_rows_q8_gpu import attend_case, bf16, check_append, inv_freq, make, np64, paged
 from tests.util import dev_u32
 
 pytestmark = pytest.mark.gpu
@@ -186,3 +186,51 @@ def test_keys_without_a_limit_are_the_room_of_a_slot(case):
         _lib.check(_lib.lib.ts_attend_rows_q8(p(q), kv._held[0], p(out), p(slots), p(pos), kept.c(), 4, keys, heads, kv_heads, width, FAR,
                                               0.09, p(ws), nbytes, torch.cuda.current_stream().cuda_stream))
         assert torch.equal(out, want[0])
+
+
+@pytest.mark.parametrize("case", [(16, 128, 4, 2, 64, True), (64, 128, 4, 2, 64, False), (32, 64, 3, 1, 32, True), (16, 256, 2, 2, 32, True), (64, 64, 2, 1, 64, True)],
+                         ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("order", ["draft by draft", "pairs apart", "any", "1024"])
+def test_rows_of_a_block_may_stand_anywhere_in_a_call(case, order):
+    """Against the definition, which knows no order but that of rows of one slot and position, the last of which counts; and
+    the values, which are kept as they come, equal those of the same rows slot by slot to the bit.  (Keys do not have to:
+    a run of up to four rows takes its angles from the positions, a longer one turns on by a fixed angle from pass to
+    pass, at most 15 times 2^-24; the tolerances of check_append hold for both.)"""
+    from tessera_b200 import ops
+    rng = np.random.default_rng(35)
+    block, width, heads, kv_heads, page, norm = case
+    slots, per = 11, 5
+    kv = make(rng, kv_heads, width, block, slots * per, page)
+    kept, table = paged(rng, slots, per, slots * per, page)
+    store = M.Store(kv, "paged", per, page, table)
+    begin = rng.integers(0, 2 * block, slots)
+    each = {"draft by draft": 5, "pairs apart": 2, "any": block + 3, "1024": 93}[order]
+    where = [(s, int(begin[s]) + i) for i in range(each) for s in range(slots)]
+    where = [w for w in where if w[1] < per * page]
+    if order in ("any", "1024"):
+        where = [where[i] for i in rng.permutation(len(where))] + where[:4]  # some of them twice
+        where = where[:1024]
+    if order == "1024" and len(where) > 1000:
+        where += [where[0]] * (1024 - len(where))
+    qkv = bf16(rng, len(where), (heads + 2 * kv_heads) * width, std=1.5)
+    gain = torch.ones(width, device="cuda") * 1.25 if norm else None
+    twin, other = (ops.RowsQ8(*(t.clone() for t in (kv.k, kv.v, kv.k_scale, kv.v_scale, kv.k_bounds))) for _ in range(2))
+
+    def feed(into, rows):
+        at = [dev_u32([where[r][j] for r in rows]) for j in (0, 1)]
+        return ops.qk_norm_rope_append_q8(qkv[torch.tensor(rows, device="cuda")].contiguous(), gain, gain, inv_freq(width), *at, into, kept, heads, eps=1e-6)
+
+    row_slots, row_pos = [w[0] for w in where], [w[1] for w in where]
+    f = None if gain is None else gain.cpu().numpy().astype(np.float64)
+    want_q, k, v = M.prepared(np64(qkv), f, f, inv_freq(width).cpu().numpy(), row_pos, heads, kv_heads, width, 1e-6)
+    raw = M.append(store, k, v, row_slots, row_pos)
+    got = feed(kv, list(range(len(where))))
+    check_append(kv, None, store, raw, want_q, got)
+    feed(other, list(range(len(where))))
+    last = {w: r for r, w in enumerate(where)}
+    for s in range(slots):
+        feed(twin, [r for w, r in sorted(last.items()) if w[0] == s])
+    assert torch.equal(kv.v, twin.v) and torch.equal(kv.v_scale, twin.v_scale)
+    for n in ("k", "v", "k_scale", "v_scale", "k_bounds"):  # nothing of it is left to chance
+        again = getattr(other, n)
+        assert torch.equal(again, getattr(kv, n)), n
