@@ -415,7 +415,8 @@ int ts_rows_unpack_q8(const ts_rows_q8 *kv, const uint32_t *slots, const uint32_
  * scores and sums are f32.  A probability meets the value codes times its block's value scale, as f16: off by 2^-11 of
  * itself, or, where that product is below 2^-21 of the row's largest, by 2^-32 of the largest.
  * A query with an infinite or NaN element makes its head's output NaN, and so does a scale that is NaN (append writes
- * none) of a block that the row sees.
+ * none) of a block that the row sees, or a score of +infinity: keys kept of infinities are 10^38, and leave f32 with
+ * ordinary queries.
  * Blocks whose value scales lie more than 2^126 apart within a slot (values of 10^38 beside ordinary ones) lose the
  * weight of the smaller ones.  `out` must not overlap q. */
 size_t ts_attend_rows_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t heads, uint32_t kv_heads, uint32_t width,

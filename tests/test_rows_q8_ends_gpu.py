@@ -234,3 +234,31 @@ def test_rows_of_a_block_may_stand_anywhere_in_a_call(case, order):
     for n in ("k", "v", "k_scale", "v_scale", "k_bounds"):  # nothing of it is left to chance
         again = getattr(other, n)
         assert torch.equal(again, getattr(kv, n)), n
+
+
+@pytest.mark.parametrize("case", [(4, 2, 128, 16, 16, "dense"), (16, 1, 64, 32, 32, "paged"), (2, 1, 256, 64, 64, "dense")], ids=lambda c: "-".join(map(str, c)))
+def test_attention_over_infinities_as_append_keeps_them(case):
+    """An infinite value is kept as the largest finite one: outputs stay finite.  So is an infinite key, but its score leaves
+    f32: where it is +infinity the head is NaN, where it is -infinity the key has no weight."""
+    from tessera_b200 import ops
+    rng = np.random.default_rng(36)
+    heads, kv_heads, width, block = case[:4]
+    n = 3 * block
+    kv, kept, _ = attend_case(rng, case, [n, n])
+    where = [(s, p) for s in (0, 1) for p in range(n)]
+    qkv = bf16(rng, len(where), heads + 2 * kv_heads, width)
+    qkv[5, heads + kv_heads:, 3] = float("inf")  # a value of slot 0
+    qkv[n, heads:heads + kv_heads, 3] = float("inf")  # the key at slot 1's position 0, which rotation leaves as it is but for ...
+    qkv[n, heads:heads + kv_heads, width // 2 + 3] = 0.0  # ... 0 * infinity: its pair is NaN then, which is kept as 0
+    ops.qk_norm_rope_append_q8(qkv.reshape(len(where), -1), None, None, inv_freq(width), dev_u32([w[0] for w in where]),
+                               dev_u32([w[1] for w in where]), kv, kept, heads, eps=1e-6)
+    k8, v8 = ops.rows_unpack_q8(kv, dev_u32([0, 1]), dev_u32([5, 0]), kept)
+    assert torch.isfinite(k8.float()).all() and torch.isfinite(v8.float()).all()
+    assert (v8[0, :, 3].float() > 3e38).all() and (k8[1, :, 3].float() > 3e38).all()
+    q = bf16(rng, 3, heads, width)
+    q[1, :, 3], q[2, :, 3] = 8.0, -8.0
+    for run in (lambda: ops.attend_rows_q8(q, kv, dev_u32([0, 1, 1]), dev_u32([n - 1] * 3), kept, n, scale=1.0),
+                lambda: ops.attend_blocks_q8(q, kv, dev_u32(np.broadcast_to(np.arange(3, dtype=np.uint32), (3, kv_heads, 3))),
+                                             dev_u32([0, 1, 1]), dev_u32([n - 1] * 3), kept, n, scale=1.0)):
+        out = run()
+        assert torch.isfinite(out[0].float()).all() and torch.isnan(out[1].float()).all() and torch.isfinite(out[2].float()).all()
