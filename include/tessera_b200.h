@@ -411,7 +411,9 @@ int ts_rows_unpack_q8(const ts_rows_q8 *kv, const uint32_t *slots, const uint32_
 
 /* ts_attend_rows_bf16 over such rows: q, out bf16 [rows, heads, width], row r sees keys [max(0, pos - back),
  * min(pos + 1, keys)) of its slot; a row that sees none gets zeros.  Neighbouring rows of one slot (drafted tokens, a
- * part of a prompt) share what they read.  For its scores a query is rounded to 2^-16 of its head's largest magnitude;
+ * part of a prompt) share what they read.  For its scores a query is rounded to 2^-16 of its head's largest magnitude,
+ * whatever its other elements are (with keys of unit variance and scale = 1 / sqrt(width) a score is off by about
+ * 9e-6 of that magnitude: little beside ordinary elements, not beside ones a few hundred times smaller);
  * scores and sums are f32.  A probability meets the value codes times its block's value scale, as f16: off by 2^-11 of
  * itself, or, where that product is below 2^-21 of the row's largest, by 2^-32 of the largest.
  * A query with an infinite or NaN element makes its head's output NaN, and so does a scale that is NaN (append writes

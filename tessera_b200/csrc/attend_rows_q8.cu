@@ -10,9 +10,11 @@
 //
 // K goes into its product as it lies, without a conversion: a query row becomes whole numbers of 15 bits and a sign,
 // Q = round(q * 32639 / max |q|), in two signed digits Q = 256 q1 + q0, each a product of its own; the sums are exact in 32
-// bits (256 * 32639 * 127 < 2^31) and rounded once.  What this costs is the rounding of q to 2^-16 of the row's largest,
-// below what the probabilities' f16 costs; what it saves is half of all instructions (two conversions for every pair of
-// codes).  V's codes become f16, which holds them exactly: the bytes are set as the low bits of 1024 + (128 + code) and
+// bits (256 * 32639 * 127 < 2^31) and rounded once.  What it saves is half of all instructions (two conversions for every pair of codes).
+// What it costs is the rounding of q to 2^-16 of the row's largest magnitude, which so sets the error of every element: with
+// keys of unit variance and a scale of 1 / sqrt(W) a score is off by 9e-6 max |q| (one sigma).  That is less than f16 costs a
+// probability (2e-4) up to 24 times the others' root mean square, and less than bf16 costs the output (1e-3) up to 120 times.
+// After a per-head norm the largest is at most sqrt(W) <= 16 times it, gains aside.  V's codes become f16, which holds them exactly: the bytes are set as the low bits of 1024 + (128 + code) and
 // 1152 is subtracted.
 //
 // The scales leave the products alone.  With s = raw * scale * k_scale in powers of two and

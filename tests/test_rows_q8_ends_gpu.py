@@ -262,3 +262,36 @@ def test_attention_over_infinities_as_append_keeps_them(case):
                                              dev_u32([0, 1, 1]), dev_u32([n - 1] * 3), kept, n, scale=1.0)):
         out = run()
         assert torch.isfinite(out[0].float()).all() and torch.isnan(out[1].float()).all() and torch.isfinite(out[2].float()).all()
+
+
+@pytest.mark.parametrize("case", [(4, 2, 128, 64, 64, "dense"), (16, 1, 64, 16, 64, "paged"), (8, 1, 256, 32, 64, "dense")], ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("ratio", [30, 300, 3000])
+def test_queries_with_one_channel_far_above_the_others(case, ratio):
+    """A query is rounded to steps of its head's largest magnitude / 32639: with the queries rounded so in 64 bits the
+    tolerance is the usual one.  An element counted in steps is off by two roundings, 2^-23 of itself, so those nearer than
+    2^-21 of themselves to a half may be rounded the other way: a score is then off by a step times those keys' magnitudes,
+    d in all, and the output by (e^(2 d) - 1) sum p |v|.  Against the queries as they are, every element may be off by half
+    a step.  (The keys of the large channel are zero, so that the others decide.)"""
+    from tessera_b200 import ops
+    rng = np.random.default_rng(37)
+    heads, kv_heads, width, block = case[:4]
+    n = 700
+    kv, kept, store = attend_case(rng, case, [n, n])
+    kv.k[..., 5] = 0
+    store = M.Store(kv, store.layout, store.scalar, store.page, store.table)
+    slots, pos, scale = [0, 1, 1, 0], [n - 1, 333, 334, 20], 5 * width ** -0.5
+    q = bf16(rng, 4, heads, width)
+    q[..., 5] = torch.tensor([1.0, -1.0], device="cuda").repeat(heads // 2) * ratio
+    got = np64(ops.attend_rows_q8(q, kv, dev_u32(slots), dev_u32(pos), kept, n, scale=scale))
+    x = np64(q)
+    step = np.abs(x).max(-1, keepdims=True) / 32639
+    units = x / step
+    rounded = np.rint(units) * step
+    unsure = np.abs(np.abs(units - np.floor(units)) - 0.5) < 2.0 ** -21 * np.abs(units)
+    group = heads // kv_heads
+    most = np.stack([np.abs(store.keys_of(s, h, range(p + 1))[0]).max(0) for s, p in zip(slots, pos) for h in range(kv_heads)])
+    most = most.reshape(4, kv_heads, 1, width).repeat(group, 2).reshape(4, heads, width)
+    for query, off in ((rounded, scale * (step * unsure * most).sum(-1)), (x, scale * (step * 0.51 * most).sum(-1))):
+        want, tol = M.attend(store, query, slots, pos, n, scale)
+        weighed = (tol - 2.0 ** -8 * np.abs(want)) * 2.0 ** 10  # at least the sum of p |v|
+        assert np.all(np.abs(got - want) <= tol + np.expm1(2 * off)[..., None] * weighed)
