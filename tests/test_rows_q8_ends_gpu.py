@@ -295,3 +295,30 @@ def test_queries_with_one_channel_far_above_the_others(case, ratio):
         want, tol = M.attend(store, query, slots, pos, n, scale)
         weighed = (tol - 2.0 ** -8 * np.abs(want)) * 2.0 ** 10  # at least the sum of p |v|
         assert np.all(np.abs(got - want) <= tol + np.expm1(2 * off)[..., None] * weighed)
+
+
+def test_more_rows_than_one_attention_launch_counts_steps_for():
+    """Steps are counted in 32 bits by a slot's room: with 2^22 positions of 8 kv heads a launch takes 2040 rows.  The rows
+    of all launches, the shorter last one among them, equal those of calls of their own."""
+    from tessera_b200 import ops
+    rng = np.random.default_rng(38)
+    heads, kv_heads, width, block, room, rows = 16, 8, 128, 64, 1 << 22, 4500
+    kv = make(rng, kv_heads, width, block, 8, 64)
+    kept = ops.Kept("dense", room, None, 8 * 64)  # a pool far smaller than the room: positions past it are not there
+    q = bf16(rng, rows, heads, width)
+    at = rng.integers(0, 500, rows).astype(np.uint32)
+    at[1000:1040] = np.arange(100, 140)  # drafted rows too, and some on both sides of a launch's end
+    at[2030:2060] = np.arange(200, 230)
+    slots, pos = dev_u32([0] * rows), dev_u32(at)
+    got = ops.attend_rows_q8(q, kv, slots, pos, kept, room, scale=0.09)
+    cuts = list(range(0, rows, 300)) + [rows]
+    for a, b in zip(cuts, cuts[1:]):
+        want = ops.attend_rows_q8(q[a:b].contiguous(), kv, slots[a:b].contiguous(), pos[a:b].contiguous(), kept, 512, scale=0.09)
+        # the two calls cut a row's keys in different places: two roundings to bf16 and the sums' own error apart
+        x, y = got[a:b].float(), want.float()
+        assert torch.all((x - y).abs() <= 2.0 ** -7 * y.abs() + 2.0 ** -9 * 127 * 0.05), (x - y).abs().max()
+    store = M.Store(kv, "dense", room)
+    sample = [0, 1, 1005, 2031, 2038, 2039, 2040, 2041, 2055, 4079, 4080, 4499]
+    want, tol = M.attend(store, np64(q[torch.tensor(sample, device="cuda")]), [0] * len(sample), at[sample], room, 0.09)
+    off = np.abs(np64(got[torch.tensor(sample, device="cuda")]) - want)
+    assert np.all(off <= tol)
