@@ -8,6 +8,7 @@
 //
 // 64 rows x 4 kv heads x up to 512 blocks of width 128 take 13.3 us, of which the bounds' bytes would need 4: the pick's
 // passes over the ranks follow the last score.  8 rows x 8 kv heads x 256 blocks take 6.9 us, one load after another.
+// Thousands of blocks, in two launches: 1 row x 8 kv heads x 6000 28 us, 8 rows 45, 64 rows 170 (of which the bounds' bytes 120).
 #include <cmath>
 
 #include "rows_q8.cuh"
@@ -313,17 +314,31 @@ __global__ void __launch_bounds__(kPick) select_blocks_kernel(const SelectParams
     pdl_launch_dependents();
 }
 
-// Blocks up to which one kernel scores and picks.  64 rows x 4 kv heads x 512 blocks: 13.3 us against 13.9 in two launches,
-// one launch less for the host; past that a thread block's own pass over its bounds is what takes the time.
-constexpr uint32_t kTogether = 512;
-static_assert(kTogether <= kHeld * kPick, "the scores are held in registers");
+// Whether one kernel scores and picks.  It has a thread block for a (row, kv head), two of them fit an SM, and each goes over
+// its bounds by itself; of the two launches, the first one spreads them over the GPU.  Measured in us, one kernel / two
+// launches, width 128 where no other is given:
+//   up to two thread blocks an SM, up to 256 blocks: 1 x 8 (rows x kv heads) 6.5 / 7.1, 37 x 8 8.0 / 9.0, 64 x 4 8.7 / 9.6
+//   more of them than that, whatever the blocks: 64 x 8 12.9 / 9.4 (128 blocks), 26.2 / 21.3 (512), 512 x 8 99 / 42 (70)
+//   more blocks: few thread blocks leave SMs idle for long, 1 x 8 8.3 / 7.6 (512), 8 x 4 9.3 / 8.8; from 128 of them on one
+//   kernel is as good or better up to 512 blocks, 16 x 8 8.9 / 9.2, 64 x 4 14.7 / 15.6 (24 x 8 11.0 / 10.5), but at width
+//   256, 16 x 8 22.0 / 13.7; at 768 blocks 64 x 4 19.9 / 19.2, at 1024 8 x 8 12.0 / 10.3
+bool together(uint64_t jobs, uint32_t blocks, uint32_t width) {
+    if (jobs > 2ull * sm_count()) return false;
+    return blocks <= 256 || (blocks <= 512 && jobs >= 128 && width <= 128);
+}
+static_assert(512 <= kHeld * kPick, "the scores are held in registers");
+
+size_t scores_bytes(uint32_t rows, uint32_t most, uint32_t kv_heads, uint32_t count, uint32_t width) {
+    if (most <= count || together((uint64_t)rows * kv_heads, most, width)) return 0;
+    return (size_t)rows * kv_heads * most * sizeof(float);
+}
 
 }  // namespace
 
 size_t select_q8_workspace_bytes(uint32_t rows, uint32_t keys, uint32_t kv_heads, uint32_t block, uint32_t count) {
     if (rows == 0 || keys == 0 || block == 0) return 0;
     const uint32_t most = (uint32_t)(((uint64_t)keys + block - 1) / block);
-    return most <= count || most <= kTogether ? 0 : (size_t)rows * kv_heads * most * sizeof(float);
+    return scores_bytes(rows, most, kv_heads, count, 256);  // what suffices at any width
 }
 
 int select_q8(const void *q, const RowsQ8Dev &kv, uint32_t *ids, const uint32_t *slots, const uint32_t *positions, uint32_t rows,
@@ -341,7 +356,7 @@ int select_q8(const void *q, const RowsQ8Dev &kv, uint32_t *ids, const uint32_t 
     p.first = first;
     p.recent = recent;
     p.most = (uint32_t)(((uint64_t)keys + (1u << kv.shift) - 1) >> kv.shift);
-    const size_t need = select_q8_workspace_bytes(rows, keys, kv_heads, 1u << kv.shift, count);
+    const size_t need = scores_bytes(rows, p.most, kv_heads, count, width);
     TS_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace != nullptr && aligned16(workspace))),
                "select_blocks (q8): workspace of %zu bytes is smaller than the %zu needed, or not 16-byte aligned",
                workspace_bytes, need);

@@ -322,3 +322,20 @@ def test_more_rows_than_one_attention_launch_counts_steps_for():
     want, tol = M.attend(store, np64(q[torch.tensor(sample, device="cuda")]), [0] * len(sample), at[sample], room, 0.09)
     off = np.abs(np64(got[torch.tensor(sample, device="cuda")]) - want)
     assert np.all(off <= tol)
+
+
+@pytest.mark.parametrize("width", [64, 128, 256])
+@pytest.mark.parametrize("kv_heads,rows", [(1, 3), (1, 127), (1, 128), (8, 37), (8, 38), (2, 149)])
+@pytest.mark.parametrize("blocks", [65, 256, 257, 512, 513])
+def test_choices_on_both_sides_of_one_and_two_launches(width, kv_heads, rows, blocks):
+    """One kernel or two launches, by rows x kv heads, blocks and width: the ids are the definition's either way."""
+    from tessera_b200 import ops
+    rng = np.random.default_rng(39)
+    block, heads = 16, 2 * kv_heads
+    kv, kept, store = attend_case(rng, (heads, kv_heads, width, block, 16, "dense"), [blocks * block])
+    three = bf16(rng, 3, heads, width)
+    which = torch.arange(rows, device="cuda") % 3
+    q, pos = three[which].contiguous(), [blocks * block - 1, blocks * block - 5, 70 * block]
+    got = ops.select_blocks_q8(q, kv, dev_u32([0] * rows), dev_u32([pos[r % 3] for r in range(rows)]), kept, blocks * block, 40, first=1, recent=2)
+    want = M.select(store, np64(three), [0, 0, 0], pos, blocks * block, 40, 1, 2)
+    assert torch.equal(got, torch.from_numpy(want.astype(np.int32)).cuda()[which])
