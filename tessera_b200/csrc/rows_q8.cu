@@ -282,8 +282,8 @@ constexpr uint32_t kShort = 4;  // rows of a run that one warp takes
 constexpr int kAppendWarps = 4, kAppendThreads = kAppendWarps * 32;
 // Rows of a call up to which a block's rows may stand anywhere in it (drafted tokens laid out draft by draft): thread
 // blocks then look after kAppendWarps rows and compare every row of the call with them, which at 1024 rows is 33 MB from
-// L2 in all, and grows with the rows' square: 64 single rows take 13.2 us for 12.6 without, 512 take 44.0 for 40.7.  A
-// kernel of its own (GATHERS): 8165 rows took 42.7 us for 40.7 when one kernel did both.
+// L2 in all, and grows with the rows' square: 64 single rows take 12.9 us for 12.6 without, 512 take 43.3 for 40.7, a
+// prompt's 1000 rows 21.6 for 18.9.  A kernel of its own (GATHERS): 8165 rows took 42.7 us for 40.7 when one kernel did both.
 constexpr uint32_t kGathered = 1024;
 
 // Measured: 64 single rows with 16 + 8 + 8 heads of 128 take 6.1 us, most of it one load after another (slot, page, scale,
@@ -308,10 +308,10 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
     const uint32_t r0 = kv_block / units * p.window, r1 = min(p.rows, r0 + p.window);
     uint32_t slot = 0, blk_pos = 0xFFFFFFFFu, starts = 0;
     __shared__ uint32_t sm_rows[kAppendWarps], sm_last[kAppendWarps], sm_earlier;  // by run: see below
-    bool odd = false;  // a row of some run's slot stands outside the thread block's rows, or in another run among them
+    bool odd = false;  // another run of the block of one of this thread block's runs begins somewhere in the call
     if (!queries) {
-        uint32_t any_slot = 0;
-        if (GATHERS && threadIdx.x < p.rows) any_slot = p.slots[threadIdx.x];
+        uint32_t some = 0;
+        if (GATHERS && threadIdx.x < p.rows) some = p.slots[threadIdx.x];
         if (r0 + lane < r1) {
             slot = p.slots[r0 + lane];
             blk_pos = p.positions[r0 + lane] >> p.kv.shift;
@@ -328,21 +328,22 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
             return;
         }
         if constexpr (GATHERS) {
-            // only the slots are compared here: a thread block one of whose slots comes up elsewhere looks closely below
-            uint32_t s[kAppendWarps];
+            uint32_t s[kAppendWarps], b[kAppendWarps];
 #pragma unroll
-            for (int w = 0; w < kAppendWarps; w++) s[w] = __shfl_sync(0xFFFFFFFFu, slot, min((uint32_t)w, r1 - r0 - 1));
-#pragma unroll
-            for (int o = 1; o < kAppendWarps; o++) {
-                const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, slot, o);
-                odd = odd || (begins && lane >= (uint32_t)o && (starts >> (lane - o) & 1) && slot == before);
+            for (int w = 0; w < kAppendWarps; w++) {
+                s[w] = __shfl_sync(0xFFFFFFFFu, slot, w);
+                b[w] = __shfl_sync(0xFFFFFFFFu, starts >> lane & 1 ? blk_pos : 0xFFFFFFFFu, w);  // no row's block
             }
-            for (uint32_t i = threadIdx.x; i < p.rows; i += kAppendThreads) {
-                if (i >= (uint32_t)kAppendThreads) any_slot = p.slots[i];
-                bool same = any_slot == s[0];
 #pragma unroll
-                for (int w = 1; w < kAppendWarps; w++) same = same || any_slot == s[w];
-                odd = odd || (same && i - r0 >= (uint32_t)kAppendWarps);
+            for (int w = 0; w + 1 < kAppendWarps; w++) odd |= begins & lane > w & slot == s[w] & blk_pos == b[w];
+            for (uint32_t i = threadIdx.x; i < p.rows; i += kAppendThreads) {
+                if (i >= (uint32_t)kAppendThreads) some = p.slots[i];
+                if ((some == s[0] | some == s[1] | some == s[2] | some == s[3]) & i - r0 >= (uint32_t)kAppendWarps) {
+                    const uint32_t block = p.positions[i] >> p.kv.shift, before = max(i, 1u) - 1;
+                    const bool goes_on = i > 0 & p.slots[before] == some & p.positions[before] >> p.kv.shift == block;
+#pragma unroll
+                    for (int w = 0; w < kAppendWarps; w++) odd |= !goes_on & some == s[w] & block == b[w];
+                }
             }
             if (threadIdx.x < kAppendWarps) sm_rows[threadIdx.x] = sm_last[threadIdx.x] = 0;
             if (threadIdx.x == 0) sm_earlier = 0;
@@ -467,11 +468,12 @@ __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_ke
         if (gather) {
             // Of each run's block: whether rows before the run fall into it (then it is not this run's), how many do from the
             // run's start on, and the last of them.
+#pragma unroll 1
             for (uint32_t i = threadIdx.x; i < p.rows; i += kAppendThreads)
-#pragma unroll
-                for (int w = 0; w < kAppendWarps; w++) {
-                    const uint32_t at = r0 + w;
-                    if (!(starts >> w & 1) || p.slots[i] != p.slots[at] || (p.positions[i] ^ p.positions[at]) >> p.kv.shift) continue;
+#pragma unroll 1
+                for (uint32_t m = starts; m; m &= m - 1) {
+                    const uint32_t w = __ffs(m) - 1, at = r0 + w;
+                    if (p.slots[i] != p.slots[at] || (p.positions[i] ^ p.positions[at]) >> p.kv.shift) continue;
                     if (i < at) {
                         atomicOr(&sm_earlier, 1u << w);
                     } else {
