@@ -37,12 +37,16 @@
 // every run.
 //
 // What bounds it, measured with width 128.  Many decode rows: the codes' bytes (64 rows of up to 8192 keys, 8 kv heads of 2
-// heads: 138 us, 0.90 of the copy rate; 4 rows of up to 100003 keys, 8 kv heads of 4: 110 us, 0.89).  Listed blocks: the
-// same, in blocks that lie scattered, with a merge (64 rows x 4 kv heads x 64 blocks of 64: 58 us, 0.70).
+// heads: 139 us, 0.89 of the copy rate; 4 rows of up to 100003 keys, 8 kv heads of 4: 112 us, 0.88; 140 and 113 where the
+// board's power limit holds the clock at 1.67 GHz).  Listed blocks: the same, in blocks that lie scattered, with a merge (64 rows x 4 kv heads x 64 blocks of 64: 58 us, 0.70).
 // Drafted tokens, where 16 queries share each key: the instructions around the products (16 slots x 7 rows of up to 4099 keys,
 // 4 kv heads of 8: 53 us, 0.15 of the copy rate, an instruction in a third of the cycles from two warps a scheduler, which
 // is what their registers leave).  Fewer instructions a step also draw less power: at the board's limit, where the clock
 // gives way, 64 x 8192 went from 150 us to 142 with one look-up, copy and scale a step and two stages.
+// Width 256: sixteen queries' accumulators and digits do not fit 255 registers (840 and 932 bytes spill, in the cluster's
+// kernel 148 and 156).  A decode batch, which has one group of eight, is still bound by its bytes (32 rows of up to 8192
+// keys, 8 kv heads of 2: 145 us, 0.86); two groups are not (2 kv heads of 16: 83 us, 0.38; 16 x 7 drafted rows of up to
+// 4099 keys, 4 kv heads of 8: 114 us, 0.15).
 #include <cmath>
 
 #include "rows_q8.cuh"

@@ -286,10 +286,12 @@ constexpr int kAppendWarps = 4, kAppendThreads = kAppendWarps * 32;
 // prompt's 1000 rows 21.6 for 18.9.  A kernel of its own (GATHERS): 8165 rows took 42.7 us for 40.7 when one kernel did both.
 constexpr uint32_t kGathered = 1024;
 
-// Measured: 64 single rows with 16 + 8 + 8 heads of 128 take 6.1 us, most of it one load after another (slot, page, scale,
-// row, the block when the scale grows); 8165 rows of three prompts 40 us for 119 MB, 0.45 of the copy rate: the angles,
-// norms and roundings of 260,000 heads keep the schedulers busier than the memory.  Two values an instruction brought it
-// there from 43, five thread blocks an SM (92 registers, little spilled) from 41 with six (80 registers).
+// Measured over stores that are each written once: 64 single rows with 16 + 8 + 8 heads of 128 in blocks of 16 take 12.9 us
+// (about half of the scales grow), 6.4 where no scale grows, 13.3 where all do: one load after another (slot, page, scale,
+// row, then the block whose codes follow).  8165 rows of three prompts take 40.6 us for 119 MB, 0.45 of the copy rate, whether
+// scales grow or not: the angles, norms and roundings of 260,000 heads keep the schedulers busier than the memory.  Two
+// values an instruction brought it there from 43, five thread blocks an SM (96 registers, 24 to 64 bytes spilled at width
+// 128) from 41 with six (80 registers).
 template <int W, int B, bool GATHERS>
 __global__ void __launch_bounds__(kAppendThreads, W == 256 ? 4 : 5) append_q8_kernel(const AppendParams p) {
     constexpr int L = Lanes<W>::PER_HEAD, T = Lanes<W>::TOGETHER;
