@@ -339,3 +339,34 @@ def test_choices_on_both_sides_of_one_and_two_launches(width, kv_heads, rows, bl
     got = ops.select_blocks_q8(q, kv, dev_u32([0] * rows), dev_u32([pos[r % 3] for r in range(rows)]), kept, blocks * block, 40, first=1, recent=2)
     want = M.select(store, np64(three), [0, 0, 0], pos, blocks * block, 40, 1, 2)
     assert torch.equal(got, torch.from_numpy(want.astype(np.int32)).cuda()[which])
+
+
+def test_steps_of_dependent_launches_give_the_same_bits():
+    """Append, read back, attention and choice as programmatic dependent launches: each waits for what the one before wrote."""
+    from tessera_b200 import ops
+    case = (16, 8, 128, 16, 64, "paged")
+    heads, kv_heads, width = case[:3]
+
+    def steps():
+        rng = np.random.default_rng(40)
+        kv, kept, _ = attend_case(rng, case, [1500, 900, 60])
+        outs = []
+        for step in range(12):
+            slots = [0, 1, 2, 0, 1, 2] if step % 2 else [0, 1, 2]
+            pos = [[1400, 800, 10][s] + 2 * step + i // 3 for i, s in enumerate(slots)]
+            at = dev_u32(slots), dev_u32(pos)
+            qkv = bf16(rng, len(slots), (heads + 2 * kv_heads) * width, std=1 + step)
+            q = ops.qk_norm_rope_append_q8(qkv, None, None, inv_freq(width), *at, kv, kept, heads, eps=1e-6)
+            ids = ops.select_blocks_q8(q, kv, *at, kept, 1500, 20)
+            outs += [q, ops.attend_rows_q8(q, kv, *at, kept, 1500, scale=0.09), ids,
+                     ops.attend_blocks_q8(q, kv, ids, *at, kept, 1500, scale=0.09), *ops.rows_unpack_q8(kv, *at, kept)]
+        return outs + [kv.k.clone(), kv.v.clone(), kv.k_scale.clone(), kv.v_scale.clone(), kv.k_bounds.clone()]
+
+    want = steps()
+    ops.set_pdl(True)
+    try:
+        for _ in range(5):
+            assert all(torch.equal(a, b) for a, b in zip(steps(), want))
+    finally:
+        ops.set_pdl(False)
+    assert ops.device_status() == 0
