@@ -45,10 +45,13 @@ def workspace(nbytes: int, device) -> torch.Tensor | None:
     """A caller-owned scratch buffer, grown on demand and reused: one per host thread, device and stream, so that
     launches on two streams that may run side by side never share scratch, nor calls of two threads: the library runs
     without the interpreter's lock and may queue several kernels that meet in the scratch, and another thread's could
-    come to stand between them.  (Buffers stay when a thread ends: a captured graph may use them.)"""
+    come to stand between them.  A call that is being captured gets a buffer of its own, in the graph's pool: graphs
+    replay on any stream, and a buffer that later grows would leave the graph with memory that is no longer its own."""
     if nbytes == 0:
         return None
     dev = torch.device(device)
+    if dev.type == "cuda" and torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (dev.index or 0, torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else 0, get_ident())
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes:
@@ -281,8 +284,7 @@ _q8_scratch: dict = {}
 
 def _scratch(nbytes: int, dev: int, stream: int, like):
     """(address, owner) of scratch for one call: one buffer a host thread, device and stream (see `workspace`), which its
-    calls use one after another.  A call that is being captured gets its own, in the graph's pool: graphs replay on any
-    stream, and two of them at once must not share it."""
+    calls use one after another; a call that is being captured gets its own."""
     if nbytes == 0:
         return None, None
     if torch._C._cuda_isCurrentStreamCapturing():

@@ -65,3 +65,18 @@ def test_workspace_sizes_are_kept_by_device(ops, monkeypatch):
         assert [ops._q8_workspace("ts_size", dev, 5, 6) for dev in (0, 1, 0, 1)] == [1, 2, 1, 2]
     finally:
         ops._q8_workspace.cache_clear()
+
+
+def test_captured_calls_have_scratch_of_their_own(ops, monkeypatch):
+    """A graph keeps the addresses that its calls had: scratch shared with another graph, or with calls that may need more of
+    it later, would be written by both, or be somebody else's by then."""
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True)
+    made, empty = [], torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *shape, device=None, **more: made.append(device) or empty(*shape, **more))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: type("Stream", (), {"cuda_stream": 7}))
+    first, second = ops.workspace(100, "cuda:0"), ops.workspace(100, "cuda:0")
+    assert first.data_ptr() != second.data_ptr() and made == ["cuda:0"] * 2
+    like = torch.zeros(1)
+    a, b = ops._scratch(100, 0, 7, like), ops._scratch(100, 0, 7, like)
+    assert a[0] != b[0]
+    assert not ops._workspaces and not ops._q8_scratch
